@@ -4,7 +4,7 @@ Four operators, in the order a feed-forward block of a decoder layer runs them:
 
   norm      H = X + R, RMSNorm(H; gamma) in 8 bits
   gate_up   silu(X Wg^T) * (X Wu^T) in 8 bits, from 8-bit activations and weights
-  project   Y = R + X W^T in f32, from 8-bit activations and weights
+  project   Y = R + X W^T in f32, or X W^T in bf16, from 8-bit activations and weights
   quantize  a matrix in 8 bits: activations with a scale for each row, weights
             with a scale for each 128 rows
 
@@ -19,7 +19,7 @@ power of two with the block's largest finite magnitude at most 448 scales.
 ``prepare`` builds a program's inputs (library buffers when the library is
 called, plain tensors otherwise; the same values), ``run`` is one pass,
 ``work`` the bytes and operations it cannot do without, ``exact`` the same
-results in 64 bits.
+results in 64 bits, before their rounding to an output's type.
 """
 import math
 
@@ -30,29 +30,30 @@ own = False
 EPS = 1e-6
 BLOCK = 128
 TOP = 448.0  # e4m3's largest value
+TYPES = ["f32", "bf16"]
 
 
 # ---------------------------------------------------------------- the cases
 def listed():
     return [
         # One token's attention output (24 heads of 256) before its projection: the smallest call.
-        dict(name="quantize_token", kind="quantize", rows=1, cols=6144, block=1, bf16=False),
-        # A prompt's attention output, an odd number of tokens.
-        dict(name="quantize_prompt", kind="quantize", rows=1999, cols=6144, block=1, bf16=False),
+        dict(name="quantize_token", kind="quantize", rows=1, cols=6144, block=1, type="f32"),
         # A layer's bf16 weights (hidden 2560 to 10240 channels) once at load.
-        dict(name="quantize_weights", kind="quantize", rows=10240, cols=2560, block=128, bf16=True),
+        dict(name="quantize_weights", kind="quantize", rows=10240, cols=2560, block=128, type="bf16"),
         # A decode step of five sequences between two blocks.
-        dict(name="norm_batch5", kind="norm", rows=5, cols=2560, residual=True),
-        # A prompt between two blocks.
-        dict(name="norm_prompt", kind="norm", rows=4096, cols=2560, residual=True),
+        dict(name="norm_batch5", kind="norm", rows=5, cols=2560, residual=True, type="f32"),
+        # A prompt between two blocks: a sublayer's bf16 output into the f32 residual stream.
+        dict(name="norm_prompt", kind="norm", rows=4096, cols=2560, residual=True, type="bf16"),
         # One token's projection from the hidden state: latency and the weights' bytes.
-        dict(name="project_token", kind="project", tokens=1, cols=2560, rows=10240, residual=False),
-        # A decode step of 32 sequences: attention's output projection into the residual.
-        dict(name="project_batch32", kind="project", tokens=32, cols=6144, rows=2560, residual=True),
+        dict(name="project_token", kind="project", tokens=1, cols=2560, rows=10240, residual=False, type="f32"),
+        # A decode step of 32 sequences: attention's output projection into the residual stream.
+        dict(name="project_batch32", kind="project", tokens=32, cols=6144, rows=2560, residual=True, type="f32"),
         # A short prompt of ragged length, output rows that fill no tile.
-        dict(name="project_ragged", kind="project", tokens=333, cols=2500, rows=5003, residual=False),
+        dict(name="project_ragged", kind="project", tokens=333, cols=2500, rows=5003, residual=False, type="bf16"),
+        # A prompt's attention output into the residual stream, sums to f32.
+        dict(name="project_prompt_f32", kind="project", tokens=2048, cols=6144, rows=2560, residual=True, type="f32"),
         # Several long prompts in one batch.
-        dict(name="project_prompt", kind="project", tokens=8192, cols=2560, rows=10240, residual=False),
+        dict(name="project_prompt", kind="project", tokens=8192, cols=2560, rows=10240, residual=False, type="bf16"),
         # One token's feed-forward input.
         dict(name="gate_up_token", kind="gate_up", tokens=1, cols=2560, ff=8192),
         # A step of many sequences, a hidden size that ends inside a block.
@@ -76,13 +77,15 @@ def draw(rng):
     cols = _cols(rng)
     if kind == "quantize":
         return dict(kind=kind, rows=_log(rng, 1, min(16384, (1 << 26) // cols)), cols=cols, block=rng.choice([1, 128]),
-                    bf16=rng.random() < 0.5)
+                    type=rng.choice(TYPES))
     if kind == "norm":
-        return dict(kind=kind, rows=_log(rng, 1, min(16384, (1 << 25) // cols)), cols=cols, residual=rng.random() < 0.7)
+        return dict(kind=kind, rows=_log(rng, 1, min(16384, (1 << 25) // cols)), cols=cols, residual=rng.random() < 0.7,
+                    type=rng.choice(TYPES))
     if kind == "project":
         rows = _log(rng, 16, 12288)
+        kept = rng.choice(["f32", "f32 with R", "bf16"])
         return dict(kind=kind, tokens=_log(rng, 1, min(8192, 2 * 10 ** 11 // (cols * rows))), cols=cols, rows=rows,
-                    residual=rng.random() < 0.5)
+                    residual=kept == "f32 with R", type=kept[:4].strip())
     ff = _log(rng, 64, 8192)
     return dict(kind=kind, tokens=_log(rng, 1, min(8192, 10 ** 11 // (cols * ff))), cols=cols, ff=ff)
 
@@ -137,15 +140,19 @@ def _weights(rows, cols, seed):
     return w * torch.exp(_normal((rows, 1), seed + 1, 0.3))
 
 
+def _dtype(case):
+    return torch.bfloat16 if case["type"] == "bf16" else torch.float32
+
+
 def _inputs(case, seed):
     """The pass's inputs by name."""
     kind, seed = case["kind"], 100 * seed
     if kind == "quantize":
         x = _weights(case["rows"], case["cols"], seed) if case["block"] > 1 else _hidden(case["rows"], case["cols"], seed)
-        return {"X": x.to(torch.bfloat16) if case["bf16"] else x}
+        return {"X": x.to(_dtype(case))}
     cols = case["cols"]
     if kind == "norm":
-        t = {"X": _hidden(case["rows"], cols, seed), "gamma": 1 + _normal((cols,), seed + 5, 0.1)}
+        t = {"X": _hidden(case["rows"], cols, seed).to(_dtype(case)), "gamma": 1 + _normal((cols,), seed + 5, 0.1)}
         if case["residual"]:
             t["R"] = _hidden(case["rows"], cols, seed + 10)
         return t
@@ -224,7 +231,7 @@ def prepare(case, seed):
         if case["residual"]:
             s["H"] = _empty((case["rows"], case["cols"]), torch.float32)
     elif kind == "project":
-        s["Y"] = _empty((case["tokens"], case["rows"]), torch.float32)
+        s["Y"] = _empty((case["tokens"], case["rows"]), _dtype(case))
     else:
         s["codes"], s["scales"] = _empty_f8(case["tokens"], case["ff"])
         s["workspace"] = _empty((_backend().f8_gate_up_workspace_bytes(case["tokens"], case["ff"]),), torch.uint8)
@@ -238,16 +245,16 @@ def _run_own(s):
     t = {k: v[0] for k, v in s["in"].items()}
     if c["kind"] == "quantize":
         be.f8_quantize(t["X"], c["rows"], c["cols"], c["block"], s["codes"][0], s["scales"][0],
-                       type="bf16" if c["bf16"] else "f32")
+                       type=c["type"])
     elif c["kind"] == "norm":
         if c["residual"]:
             be.f8_norm(t["X"], t["gamma"], EPS, c["rows"], c["cols"], s["codes"][0], s["scales"][0], residual=t["R"],
-                       H=s["H"][0])
+                       H=s["H"][0], type=c["type"])
             return {"H": s["H"][1], "codes": s["codes"][1], "scales": s["scales"][1]}
-        be.f8_norm(t["X"], t["gamma"], EPS, c["rows"], c["cols"], s["codes"][0], s["scales"][0])
+        be.f8_norm(t["X"], t["gamma"], EPS, c["rows"], c["cols"], s["codes"][0], s["scales"][0], type=c["type"])
     elif c["kind"] == "project":
         be.f8_project(t["X"], t["Xs"], c["tokens"], c["cols"], t["W"], t["Ws"], c["rows"], s["Y"][0],
-                      residual=t.get("R"))
+                      residual=t.get("R"), type=c["type"])
         return {"Y": s["Y"][1]}
     else:
         be.f8_gate_up(t["X"], t["Xs"], c["tokens"], c["cols"], t["Wg"], t["Wgs"], t["Wu"], t["Wus"], c["ff"],
@@ -263,14 +270,14 @@ def run(state):
         codes, scales = _quantize(t["X"].float(), c["block"])
         return {"codes": codes, "scales": scales}
     if c["kind"] == "norm":
-        h = t["X"] + t["R"] if c["residual"] else t["X"]
+        h = t["X"].float() + t["R"] if c["residual"] else t["X"].float()
         y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + EPS) * t["gamma"]
         codes, scales = _quantize(y, 1)
         return {"H": h, "codes": codes, "scales": scales} if c["residual"] else {"codes": codes, "scales": scales}
     x = _dequantize(t["X"], t["Xs"], 1)
     if c["kind"] == "project":
         y = x @ _dequantize(t["W"], t["Ws"], BLOCK).T
-        return {"Y": y + t["R"] if c["residual"] else y}
+        return {"Y": y + t["R"] if c["residual"] else y.to(_dtype(c))}
     g, u = x @ _dequantize(t["Wg"], t["Wgs"], BLOCK).T, x @ _dequantize(t["Wu"], t["Wus"], BLOCK).T
     codes, scales = _quantize(g / (1 + torch.exp(-g)) * u, 1)
     return {"codes": codes, "scales": scales}
@@ -278,30 +285,24 @@ def run(state):
 
 # ---------------------------------------------------------------- the bound
 def work(case):
-    kind, cols = case["kind"], case["cols"]
+    kind, cols, size = case["kind"], case["cols"], 2 if case.get("type") == "bf16" else 4
     f8 = lambda rows, n, block: rows * n + _blocks(rows, block) * _blocks(n, BLOCK)  # noqa: E731
     if kind in ("quantize", "norm"):
         n = case["rows"] * cols
         if kind == "quantize":
-            return {"bytes": n * (2 if case["bf16"] else 4) + f8(case["rows"], cols, case["block"]), "flops": 3 * n}
-        return {"bytes": n * (12 if case["residual"] else 4) + 4 * cols + f8(case["rows"], cols, 1), "flops": 8 * n}
+            return {"bytes": n * size + f8(case["rows"], cols, case["block"]), "flops": 3 * n}
+        return {"bytes": n * (size + (8 if case["residual"] else 0)) + 4 * cols + f8(case["rows"], cols, 1), "flops": 8 * n}
     n = case["tokens"]
     if kind == "project":
         rows = case["rows"]
-        return {"bytes": f8(n, cols, 1) + f8(rows, cols, BLOCK) + 4 * n * rows * (2 if case["residual"] else 1),
+        return {"bytes": f8(n, cols, 1) + f8(rows, cols, BLOCK) + n * rows * size * (2 if case["residual"] else 1),
                 "flops": 2 * n * rows * cols}
     return {"bytes": f8(n, cols, 1) + 2 * f8(case["ff"], cols, BLOCK) + f8(n, case["ff"], 1), "flops": 4 * n * case["ff"] * cols}
 
 
 # ------------------------------------------------------------------ 64 bits
-def _round_e4m3(v):
-    """f64 to the nearest e4m3 value, ties to even: 4 significant bits from 2^-6 up, steps of 2^-9 below."""
-    e = torch.frexp(v)[1].clamp(min=-5).double() - 4
-    return torch.round(v * torch.exp2(-e)) * torch.exp2(e)
-
-
 def _exact_f8(y, block):
-    """The codes' and scales' values of y, from the definition."""
+    """What codes and scales stand for: y over its block's scale, not rounded, and the scale."""
     rows, cols = y.shape
     kb = _blocks(cols, BLOCK)
     wide = torch.nn.functional.pad(y, (0, kb * BLOCK - cols))
@@ -311,8 +312,7 @@ def _exact_f8(y, block):
     e = e + (amax > TOP * torch.exp2(e)).double() - (amax <= TOP * torch.exp2(e - 1)).double()
     scale = torch.exp2(torch.where(amax > 0, e, torch.zeros_like(e)))
     each = scale.repeat_interleave(block, 0)[:rows].repeat_interleave(BLOCK, 1)
-    scales = torch.nn.functional.pad(scale, (0, -kb % 4), value=1.0)
-    return {"codes": _round_e4m3(wide / each), "scales": scales}
+    return {"codes": wide / each, "scales": torch.nn.functional.pad(scale, (0, -kb % 4), value=1.0)}
 
 
 def _value(codes, scales, block):
