@@ -245,6 +245,68 @@ int sm_moe_block(sm_ctx *ctx, uint64_t H, int tokens, uint64_t gamma, float eps,
                  int experts, int topk, uint64_t Hout, uint64_t ids, uint64_t weights, uint64_t workspace,
                  uint64_t workspace_bytes);
 
+/* ------------------------------------------ 8-bit floating-point matrices */
+/* Dense products on the 8-bit matrix units (no reference counterpart; they
+ * stand beside strata_norm, strata_bf16_project and strata_quant_project).
+ *
+ * An f8 matrix [rows x cols] is two buffers. Codes: e4m3 bytes (OCP: largest
+ * value 448, no infinities), rows x pitch, pitch = cols rounded up to a
+ * multiple of 128, 0 past `cols`. Scales: powers of two as e8m0 bytes
+ * (2^(byte - 127)), one for each 128 columns of each `block_rows` rows,
+ * ceil(rows / block_rows) x spitch, spitch = pitch / 128 rounded up to a
+ * multiple of 4, 127 past the last block. block_rows is 1 for activations
+ * and 128 for weights. value = code * scale. A block's scale is the smallest
+ * power of two (2^-127 or more) with its largest finite magnitude at most
+ * 448 scales (1 where that magnitude is 0); codes are rounded to nearest,
+ * ties to even; a value that is not finite becomes NaN.
+ *
+ * Buffers that a caller fills itself must keep to this: the codes past
+ * `cols` are multiplied too. Every dimension is 1 to 2^21, rows * cols,
+ * tokens * rows and tokens * stride at most 2^33. Outputs must not be
+ * buffers that the call reads, except where an entry says so. Rows past the
+ * last and words outside an output slice are left as they were.
+ * Nothing is allocated and nothing waits: every entry may be captured. */
+#define SM_TYPE_F32 0
+#define SM_TYPE_BF16 1
+
+/* Bytes of an f8 matrix's two buffers. */
+int sm_f8_bytes(int rows, int cols, int block_rows, uint64_t *codes, uint64_t *scales);
+
+/* X [rows x cols] (f32 or bf16) as an f8 matrix; block_rows 1 or 128. */
+int sm_f8_quantize(sm_ctx *ctx, uint64_t X, int type, int rows, int cols, int block_rows, uint64_t codes,
+                   uint64_t scales);
+
+/* Per row: H = X + R (f32; R = 0: H is X itself), then
+ *   H / sqrt(mean(H^2) + eps) * gamma
+ * as an f8 matrix of block_rows 1. X is f32 or bf16, R, H [rows x cols] and
+ * gamma [cols] f32. H is written where it is not 0; it may be R, and X where
+ * that is f32. The mean is taken in f64. */
+int sm_f8_norm(sm_ctx *ctx, uint64_t X, int type, uint64_t R, uint64_t gamma, float eps, int rows, int cols, uint64_t H,
+               uint64_t codes, uint64_t scales);
+
+/* Y[t * stride + offset + r] = R[the same] + X[t, :] . W[r, :], t < tokens,
+ * r < rows; X an f8 matrix [tokens x cols] of block_rows 1, W one
+ * [rows x cols] of block_rows 128.
+ * type f32: Y is f32, the sums are f32's (the codes' products are exact). R
+ *   is f32, laid out like Y, 0 for none; it may be Y.
+ * type bf16: Y is bf16 and R must be 0; the sums are rounded once to bf16 and
+ *   their products may be cut off 2^13 below the largest of eight neighbours
+ *   (about 1e-5 of the sum), for up to twice the rate.
+ * The same inputs give the same bits. */
+int sm_f8_project(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int cols, uint64_t W, uint64_t w_scales,
+                  int rows, uint64_t R, uint64_t Y, int type, int64_t stride, int64_t offset);
+
+/* silu(X . Wg) * (X . Wu) as an f8 matrix [tokens x ff] of block_rows 1;
+ * silu(g) = g / (1 + exp(-g)); X as in sm_f8_project, Wg and Wu f8 matrices
+ * [ff x cols] of block_rows 128 (they may be one buffer). The sums are those
+ * of sm_f8_project's bf16 type before their rounding. The workspace holds
+ * sm_f8_gate_up_workspace(...) bytes; a call leaves nothing in it that a
+ * later call needs. */
+int sm_f8_gate_up_workspace(int tokens, int ff, uint64_t *bytes);
+int sm_f8_gate_up(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int cols, uint64_t Wg, uint64_t wg_scales,
+                  uint64_t Wu, uint64_t wu_scales, int ff, uint64_t codes, uint64_t scales, uint64_t workspace,
+                  uint64_t workspace_bytes);
+
 /* ---------------------------------------------------------------- timing */
 /* Events on the context's stream (the stream every launch above uses). */
 int sm_event_record(sm_ctx *ctx, int slot);          /* slot in [0, 64) */

@@ -25,6 +25,7 @@ ERRORS = {-1: "hip", -2: "argument", -3: "bounds", -4: "handle", -5: "no kernel"
 SM_E_FAULT = -8
 
 _TYPES = {"f32": np.float32, "i32": np.int32, "u32": np.uint32}
+_F8_TYPES = {"f32": 0, "bf16": 1}  # SM_TYPE_F32, SM_TYPE_BF16
 _lib = None
 
 
@@ -89,6 +90,12 @@ def lib():
             "sm_moe_route_stats": (i, [vp, u64, i, i, i, i, i, pu64, ctypes.POINTER(i)]),
             "sm_fused_reset": (i, [vp]),
             "sm_fused_test_hooks": (i, [vp, ctypes.c_uint32, i]),
+            "sm_f8_bytes": (i, [i, i, i, pu64, pu64]),
+            "sm_f8_quantize": (i, [vp, u64, i, i, i, i, u64, u64]),
+            "sm_f8_norm": (i, [vp, u64, i, u64, u64, ctypes.c_float, i, i, u64, u64, u64]),
+            "sm_f8_project": (i, [vp, u64, u64, i, i, u64, u64, i, u64, u64, i, ctypes.c_int64, ctypes.c_int64]),
+            "sm_f8_gate_up_workspace": (i, [i, i, pu64]),
+            "sm_f8_gate_up": (i, [vp, u64, u64, i, i, u64, u64, u64, u64, i, u64, u64, u64, u64]),
             "sm_prefetch_router": (i, [vp, ctypes.c_uint64, i, i]),
         }
         for name, (res, args) in sig.items():
@@ -341,6 +348,55 @@ class Backend:
                                        bias.handle if bias else 0, arena.handle, blob_stride, shared_blob.handle,
                                        Wsg.handle, width, ff, experts, topk, Hout.handle, ids.handle, weights.handle,
                                        workspace.handle, workspace.nbytes))
+
+    # ---------------------------------- 8-bit floating-point matrices
+    # Codes (e4m3) and scales (e8m0, one for 128 columns of 1 or 128 rows);
+    # include/strata_mi355x.h has the layout. `type` is "f32" or "bf16".
+    @staticmethod
+    def _f8_type(type):
+        if type not in _F8_TYPES:
+            raise ArgumentError(-2, "type must be f32 or bf16")
+        return _F8_TYPES[type]
+
+    @staticmethod
+    def f8_bytes(rows, cols, block_rows=1):
+        """Bytes of an f8 matrix's (codes, scales)."""
+        c, s = ctypes.c_uint64(), ctypes.c_uint64()
+        rc = lib().sm_f8_bytes(rows, cols, block_rows, ctypes.byref(c), ctypes.byref(s))
+        if rc != SM_OK:
+            raise ArgumentError(rc, "invalid f8 matrix")
+        return c.value, s.value
+
+    def f8_quantize(self, X, rows, cols, block_rows, codes, scales, type="f32"):
+        """X [rows x cols] as an f8 matrix (block_rows 1: activations, 128: weights)."""
+        self._check(lib().sm_f8_quantize(self._ctx, X.handle, self._f8_type(type), rows, cols, block_rows, codes.handle,
+                                         scales.handle))
+
+    def f8_norm(self, X, gamma, eps, rows, cols, codes, scales, residual=None, H=None, type="f32"):
+        """H = X + residual; RMSNorm(H; gamma, eps) as an f8 matrix. H may be the residual, or X where that is f32."""
+        self._check(lib().sm_f8_norm(self._ctx, X.handle, self._f8_type(type), residual.handle if residual else 0,
+                                     gamma.handle, eps, rows, cols, H.handle if H else 0, codes.handle, scales.handle))
+
+    def f8_project(self, X, x_scales, tokens, cols, W, w_scales, rows, Y, residual=None, type="f32", stride=None,
+                   offset=0):
+        """Y[t * stride + offset + r] = residual + X[t] . W[r]; a residual (it may be Y) needs type "f32"."""
+        self._check(lib().sm_f8_project(self._ctx, X.handle, x_scales.handle, tokens, cols, W.handle, w_scales.handle,
+                                        rows, residual.handle if residual else 0, Y.handle, self._f8_type(type),
+                                        rows if stride is None else stride, offset))
+
+    @staticmethod
+    def f8_gate_up_workspace_bytes(tokens, ff):
+        n = ctypes.c_uint64()
+        rc = lib().sm_f8_gate_up_workspace(tokens, ff, ctypes.byref(n))
+        if rc != SM_OK:
+            raise ArgumentError(rc, "invalid f8 gate_up geometry")
+        return n.value
+
+    def f8_gate_up(self, X, x_scales, tokens, cols, Wg, wg_scales, Wu, wu_scales, ff, codes, scales, workspace):
+        """silu(X . Wg) * (X . Wu) as an f8 matrix [tokens x ff]."""
+        self._check(lib().sm_f8_gate_up(self._ctx, X.handle, x_scales.handle, tokens, cols, Wg.handle, wg_scales.handle,
+                                        Wu.handle, wu_scales.handle, ff, codes.handle, scales.handle, workspace.handle,
+                                        workspace.nbytes))
 
     # ------------------------------------------------------------ timing
     STAGES = ["decode_route", "decode_gate_up", "decode_down_combine", "prefill_route", "prefill_dispatch",

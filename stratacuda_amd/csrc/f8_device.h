@@ -1,0 +1,78 @@
+// Device-side pieces of the 8-bit floating-point operators (f8_convert.hip,
+// f8_project.hip): e4m3 codes (OCP: 4 significant bits, largest 448, no
+// infinities) with one power-of-two scale for each block of 128 columns, held
+// as its e8m0 byte (2^(byte - 127)).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "internal.h"
+
+namespace f8 {
+
+// The byte of the smallest power of two 2^e with amax <= 448 * 2^e, e >= -127;
+// amax is finite and not negative, 0 takes the scale 1. From the bits: amax =
+// m * 2^x with 1 <= m < 2 and 448 = 1.75 * 2^8, so e = x - 8, one more where
+// m > 1.75. A subnormal amax (x < -126) lies below 448 * 2^-127.
+__device__ __forceinline__ uint32_t scale_byte(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int b = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
+    return u == 0 ? 127u : (uint32_t)max(b, 0);
+}
+// 2^-e of a scale byte that scale_byte gave (e <= 120): exact, normal.
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+__device__ __forceinline__ float finite_magnitude(float v) {
+    const float a = fabsf(v);
+    return a < INFINITY ? a : 0.0f;  // 0 for NaN too
+}
+// v * 2^-e is exact (or below e4m3's smallest step); the conversion rounds to
+// nearest, ties to even. A value that is not finite becomes NaN: e4m3 has no
+// infinity, and a saturated one would pass as a number.
+__device__ __forceinline__ uint32_t codes4(const float v[4], float inverse) {
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[i] = fabsf(v[i]) < INFINITY ? v[i] * inverse : NAN;
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], w, true);
+}
+
+// Largest of the 32 lanes of each half of a wave, in all of them.
+__device__ __forceinline__ float half_wave_max(float v) {
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) v = fmaxf(v, __shfl_xor(v, d, 64));
+    return v;
+}
+
+__device__ __forceinline__ float bf16_value(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
+
+// Four consecutive columns of a row, 0 past `cols`; `vec`: cols is a multiple
+// of 4, so that every four lie whole and aligned in the row.
+template <typename T>
+__device__ __forceinline__ void load4(const T *row, int col, int cols, bool vec, float v[4]) {
+    if (vec) {
+        if (col < cols) {
+            if constexpr (sizeof(T) == 4) {
+                const float4 q = *(const float4 *)(row + col);
+                v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+            } else {
+                const uint2 q = *(const uint2 *)(row + col);
+                v[0] = bf16_value(q.x & 0xffffu), v[1] = __uint_as_float(q.x & 0xffff0000u);
+                v[2] = bf16_value(q.y & 0xffffu), v[3] = __uint_as_float(q.y & 0xffff0000u);
+            }
+        } else {
+            v[0] = v[1] = v[2] = v[3] = 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[i] = 0.0f;
+            if (col + i < cols) {
+                if constexpr (sizeof(T) == 4) v[i] = row[col + i];
+                else v[i] = bf16_value(row[col + i]);
+            }
+        }
+    }
+}
+
+}  // namespace f8

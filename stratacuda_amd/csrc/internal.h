@@ -247,6 +247,29 @@ bool project_one_takes(int bits, int cols, int rows, uint64_t X, uint64_t codes,
 int project_one(sm_ctx *ctx, int bits, const float *X, const void *codes, const float *scales, const float *offsets, float *Y,
                 int cols, int rows, int group, int bias, int codebook, int has_offset);
 
+// ------------------------------------------ 8-bit floating-point matrices
+// Row pitch of the codes and of the scales, and the bytes of both.
+struct F8Layout {
+    uint64_t pitch, spitch, codes, scales;
+};
+inline F8Layout f8_layout(int64_t rows, int64_t cols, int block_rows) {
+    const uint64_t kb = (uint64_t)(cols + 127) / 128, up = (uint64_t)(rows + block_rows - 1) / block_rows;
+    return {kb * 128, (kb + 3) / 4 * 4, (uint64_t)rows * kb * 128, up * ((kb + 3) / 4 * 4)};
+}
+struct F8Operand {
+    const uint8_t *codes, *scales;
+};
+// Unchecked launchers on raw device pointers (f8_convert.hip, f8_project.hip).
+int f8_quantize_launch(sm_ctx *ctx, const void *X, bool bf16, int rows, int cols, int block_rows, uint8_t *codes,
+                       uint8_t *scales);
+int f8_norm_launch(sm_ctx *ctx, const void *X, bool bf16, const float *R, const float *gamma, float eps, int rows, int cols,
+                   float *H, uint8_t *codes, uint8_t *scales);
+int f8_project_launch(sm_ctx *ctx, const F8Operand &X, int tokens, int cols, const F8Operand &W, int rows, const float *R,
+                      void *Y, bool bf16, int64_t stride, int64_t offset);
+uint64_t f8_gate_up_workspace(int tokens, int ff);
+int f8_gate_up_launch(sm_ctx *ctx, const F8Operand &X, int tokens, int cols, const F8Operand &Wg, const F8Operand &Wu, int ff,
+                      uint8_t *codes, uint8_t *scales, void *workspace);
+
 // ------------------------------------------------ kernels by name (sm_run)
 // One 64-bit slot per reference parameter: a buffer handle, or the int32 /
 // float32 bit pattern in the low 32 bits.
