@@ -292,7 +292,9 @@ int sm_f8_norm(sm_ctx *ctx, uint64_t X, int type, uint64_t R, uint64_t gamma, fl
  * type bf16: Y is bf16 and R must be 0; the sums are rounded once to bf16 and
  *   their products may be cut off 2^13 below the largest of eight neighbours
  *   (about 1e-5 of the sum), for up to twice the rate.
- * The same inputs give the same bits. */
+ * The same inputs give the same bits. An output is not finite where a code of
+ * its token or row is NaN, and where a value (code * scale) or a partial sum
+ * passes f32's range. */
 int sm_f8_project(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int cols, uint64_t W, uint64_t w_scales,
                   int rows, uint64_t R, uint64_t Y, int type, int64_t stride, int64_t offset);
 

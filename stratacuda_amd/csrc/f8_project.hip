@@ -10,9 +10,9 @@
 //     off 13 bits below its leading bit before it adds the eights in f32
 //     (measured on one MI355X: 1.3e-5 of the result for normal values), far
 //     below those outputs' rounding (2^-9, 2^-4).
-//   f32 outputs: the codes as f16 (exact: 4 bits in 11, 2^-9 to 448) in
-//     v_mfma_f32_16x16x32_f16, whose sums are f32's (1e-7 measured), at half
-//     the rate; the block's sum is scaled once.
+//   f32 outputs: code times scale as bf16 (exact: 4 significant bits in 8, the
+//     exponent of f32) in v_mfma_f32_16x16x32_bf16, whose sums are f32's (1e-7
+//     measured), at half the rate.
 #include "f8_device.h"
 
 namespace {
@@ -21,8 +21,9 @@ using namespace smi;
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 
 enum Out { kF32, kBf16, kHidden };  // kHidden: silu(gate) * up in f32
 
@@ -31,34 +32,51 @@ __device__ __forceinline__ v8i load_frag(const uint8_t *p) {
     const v4i a = *(const v4i *)p, b = *(const v4i *)(p + 16);
     return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
-__device__ __forceinline__ v8h half8(int lo, int hi) {
-    const v2h a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
-    const v2h b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
-    const v2h c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
-    const v2h d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
-    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-// D (16 weight rows x 16 tokens): lane l holds token l % 16, rows 4 (l / 16) + i.
-// sw, sx: scale bytes of the lane's weight row and token.
+// An operand of one block of 128 columns: the codes with their scale, or
+// (EXACT) their values in bf16, 32 columns an instruction. Which 32 columns
+// lie in which instruction and lane is one order for both matrices.
+struct Codes {
+    v8i v;
+    int scale;
+};
+struct Values {
+    v8b q[4];
+};
 template <bool EXACT>
-__device__ __forceinline__ v4f multiply(v8i w, v8i x, v4f acc, uint32_t sw, uint32_t sx) {
+__device__ __forceinline__ auto operand(v8i c, uint32_t scale) {
     if constexpr (EXACT) {
-        v4f t = {0, 0, 0, 0};
+        Values r;
+        const float s = __uint_as_float(scale << 23);  // its exponent alone is used
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-            t = __builtin_amdgcn_mfma_f32_16x16x32_f16(half8(w[2 * q], w[2 * q + 1]), half8(x[2 * q], x[2 * q + 1]), t, 0, 0, 0);
-        const int e = (int)(sw + sx) - 254;  // one exponent for the tile's 16 weight rows
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = acc[i] + __builtin_amdgcn_ldexpf(t[i], e);
-        return acc;
+        for (int i = 0; i < 8; i++) {
+            const v2b lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], s, false);
+            const v2b hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], s, true);
+            r.q[i / 2][4 * (i % 2)] = lo[0], r.q[i / 2][4 * (i % 2) + 1] = lo[1];
+            r.q[i / 2][4 * (i % 2) + 2] = hi[0], r.q[i / 2][4 * (i % 2) + 3] = hi[1];
+        }
+        return r;
     } else {
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 0, 0, 0, (int)sw, 0, (int)sx);
+        return Codes{c, (int)scale};
     }
 }
+// acc[i] += w[i] . x, each 16 weight rows x 16 tokens: lane l holds token
+// l % 16, rows 4 (l / 16) on.
+template <int N>
+__device__ __forceinline__ void multiply(const Codes (&w)[N], const Codes &x, v4f *const (&acc)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        *acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[i].v, x.v, *acc[i], 0, 0, 0, w[i].scale, 0, x.scale);
+}
+template <int N>
+__device__ __forceinline__ void multiply(const Values (&w)[N], const Values &x, v4f *const (&acc)[N]) {
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+        for (int i = 0; i < N; i++) *acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[i].q[q], x.q[q], *acc[i], 0, 0, 0);
+}
 
-__device__ __forceinline__ uint16_t to_bf16(float f) {  // nearest, ties to even; NaN stays NaN
-    const uint32_t u = __float_as_uint(f);
-    return f != f ? (uint16_t)((u >> 16) | 64u) : (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {  // nearest, ties to even; NaN stays NaN
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
 }
 __device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
@@ -71,14 +89,28 @@ struct Product {
     int64_t stride, offset;
 };
 
-// Four consecutive rows r.. of token t.
+// 16 bytes of a token's outputs, aligned: eight in bf16, or four to which R is added.
 template <Out OUT>
-__device__ __forceinline__ void store4(const Product &a, int t, int r, v4f v) {
-    const int64_t at = t * a.stride + a.offset + r;
+__device__ __forceinline__ void store16(const Product &a, int64_t at, v4i v) {
+    if constexpr (OUT == kBf16) {
+        *(v4i *)((uint16_t *)a.Y + at) = v;
+    } else {
+        v4f y = __builtin_bit_cast(v4f, v);
+        if (a.R) {
+            const v4f o = *(const v4f *)(a.R + at);
+#pragma unroll
+            for (int i = 0; i < 4; i++) y[i] = o[i] + y[i];
+        }
+        *(v4f *)((float *)a.Y + at) = y;
+    }
+}
+// The first `n` of four, anywhere.
+template <Out OUT>
+__device__ __forceinline__ void store_some(const Product &a, int64_t at, int n, v4f v) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        if (r + i >= a.rows) break;
-        if constexpr (OUT == kBf16) ((uint16_t *)a.Y)[at + i] = to_bf16(v[i]);
+        if (i >= n) break;
+        if constexpr (OUT == kBf16) ((uint16_t *)a.Y)[at + i] = (uint16_t)bf16_pair(v[i], v[i]);
         else ((float *)a.Y)[at + i] = a.R ? a.R[at + i] + v[i] : v[i];
     }
 }
@@ -90,8 +122,11 @@ __device__ __forceinline__ void store4(const Product &a, int t, int r, v4f v) {
 // waves' order.
 constexpr int kWaves = 8;
 
+// Whether every n-th output of a token starts n aligned ones (buffers start aligned).
+bool aligned(const Product &a, int n) { return a.stride % n == 0 && a.offset % n == 0; }
+
 template <int TT, bool EXACT, Out OUT>
-__global__ void __launch_bounds__(64 * kWaves) k_f8_few(Product a) {
+__global__ void __launch_bounds__(64 * kWaves) k_f8_few(Product a, bool vec) {
     constexpr int M = OUT == kHidden ? 2 : 1;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, in = lane % 16, part = lane / 16;
     const int r0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * TT;
@@ -110,16 +145,14 @@ __global__ void __launch_bounds__(64 * kWaves) k_f8_few(Product a) {
         for (int m = 0; m < M; m++) acc[m][t] = v4f{0, 0, 0, 0};
     }
     for (int b = wave; b < a.kb; b += kWaves) {
-        v8i wf[M];
-        uint32_t sw[M];
+        decltype(operand<EXACT>(v8i{}, 0)) wf[M];
 #pragma unroll
-        for (int m = 0; m < M; m++) wf[m] = load_frag(w[m] + (uint64_t)b * 128), sw[m] = ws[m][b];
+        for (int m = 0; m < M; m++) wf[m] = operand<EXACT>(load_frag(w[m] + (uint64_t)b * 128), ws[m][b]);
 #pragma unroll
         for (int t = 0; t < TT; t++) {
-            const v8i xf = load_frag(x[t] + (uint64_t)b * 128);
-            const uint32_t sx = xs[t][b];
-#pragma unroll
-            for (int m = 0; m < M; m++) acc[m][t] = multiply<EXACT>(wf[m], xf, acc[m][t], sw[m], sx);
+            const auto xf = operand<EXACT>(load_frag(x[t] + (uint64_t)b * 128), xs[t][b]);
+            if constexpr (M == 2) multiply(wf, xf, {&acc[0][t], &acc[M - 1][t]});
+            else multiply(wf, xf, {&acc[0][t]});
         }
     }
 #pragma unroll
@@ -142,16 +175,327 @@ __global__ void __launch_bounds__(64 * kWaves) k_f8_few(Product a) {
 #pragma unroll
         for (int i = 0; i < 4; i++) v[0][i] = silu_times(v[0][i], v[M - 1][i]);
     const int t = t0 + 16 * wave + in;
-    if (t < a.tokens) store4<OUT>(a, t, r0 + 4 * part, v[0]);
+    if (t >= a.tokens) return;
+    const int64_t at = t * a.stride + a.offset + r0 + 4 * part;
+    if (vec && r0 + 16 <= a.rows) {
+        if constexpr (OUT == kBf16)
+            *(uint2 *)((uint16_t *)a.Y + at) = make_uint2(bf16_pair(v[0][0], v[0][1]), bf16_pair(v[0][2], v[0][3]));
+        else
+            store16<OUT>(a, at, __builtin_bit_cast(v4i, v[0]));
+    } else {
+        store_some<OUT>(a, at, a.rows - r0 - 4 * part, v[0]);
+    }
 }
 
 template <bool EXACT, Out OUT>
 void few(sm_ctx *ctx, const Product &a) {
     const int tiles = (a.tokens + 15) / 16, tt = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
+    const bool vec = aligned(a, 4);
     const dim3 grid((a.rows + 15) / 16, (tiles + tt - 1) / tt);
-    if (tt == 4) k_f8_few<4, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a);
-    else if (tt == 2) k_f8_few<2, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a);
-    else k_f8_few<1, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a);
+    if (tt == 4) k_f8_few<4, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a, vec);
+    else if (tt == 2) k_f8_few<2, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a, vec);
+    else k_f8_few<1, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a, vec);
+}
+
+// ------------------------------------------------------ many tokens: tiles
+// A workgroup of WT x WR waves makes BT tokens x BR weight rows (a gated pair:
+// BR / 2 rows of each matrix). Each step brings one block of 128 columns of
+// both into LDS by DMA (16 bytes a lane) while the step before is multiplied:
+// two buffers, one barrier a step. A row's 128 bytes lie in eight slots of 16
+// whose order goes by the row's number, so that the 16 lanes that read one
+// column of 16 rows meet all banks.
+typedef __attribute__((address_space(3))) void lds_void;
+// A tile's rows as a buffer: a load past its end gives zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_buffer(const uint8_t *base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes, 0x00027000);
+}
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t from, uint32_t lane_offset, uint32_t offset, void *lds) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void *)lds, 16, lane_offset, offset, 0, 0);
+}
+__device__ __forceinline__ void dma4(const uint8_t *src, void *lds) {
+    __builtin_amdgcn_global_load_lds(src, (lds_void *)lds, 4, 0, 0);
+}
+__device__ __forceinline__ int swizzle(int row) { return row & 7; }
+
+// The tiles in the order of the eight XCDs that workgroups go round: each XCD
+// takes neighbouring tiles, four of tokens by as many of rows, so that its L2
+// holds what they share.
+struct Tiles {
+    int tokens, rows, per_xcd;  // tiles; workgroups of an XCD (grid / 8, all of them if they are fewer than 8)
+    __device__ __forceinline__ void locate(int at, int &t, int &r) const {
+        const int panel = at / (4 * rows), width = min(4, tokens - 4 * panel), in_panel = at - panel * 4 * rows;
+        const int across = in_panel / width;
+        t = __builtin_amdgcn_readfirstlane(4 * panel + in_panel - across * width), r = __builtin_amdgcn_readfirstlane(across);
+    }
+};
+
+template <int BT, int BR, int WT, int WR, bool EXACT, Out OUT>
+__global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles, bool vec) {
+    constexpr int kThreads = 64 * WT * WR, NT = BT / WT / 16, M = OUT == kHidden ? 2 : 1, NR = BR / WR / 16 / M;
+    constexpr int kStage = (BT + BR) * 128, kRows = kThreads / 8;  // rows that the threads bring at a time
+    static_assert(BT % kRows == 0 && BR / M % kRows == 0 && kRows % 8 == 0 && BT % 64 == 0 && BT / 64 < WT * WR && NT >= 2, "");
+    // two variables, so that reads of one need not wait for the DMA into the other
+    __shared__ __attribute__((aligned(16))) uint8_t s_even[kStage], s_odd[kStage];
+    __shared__ uint32_t s_even_scale[BT + 64], s_odd_scale[BT + 64];
+    const int lane = threadIdx.x % 64, in = lane % 16, part = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wt = wave / WR, wr = wave % WR;
+    const int xcd = blockIdx.x % 8, n = tiles.tokens * tiles.rows;
+    const int first = xcd * (n / 8) + min(xcd, n % 8) + blockIdx.x / 8, end = (xcd + 1) * (n / 8) + min(xcd + 1, n % 8);
+    if (first >= end) return;
+
+    // ---- bringing steps, two ahead: past a tile's last they are the next tile's
+    // A thread brings 16 bytes of every kRows-th row: of row threadIdx.x / 8 on.
+    const uint32_t from = threadIdx.x / 8 * (uint32_t)a.pitch + ((threadIdx.x ^ swizzle(threadIdx.x / 8)) & 7) * 16;
+    const int slot = min(wave, BT / 64);
+    struct Place {
+        int t0, r0, x_rows, w_rows;  // rows of the matrices that are left from there; 0 past the last tile
+        const uint8_t *scale;
+    };
+    auto place = [&](int at) __attribute__((always_inline)) {
+        Place p;
+        tiles.locate(min(at, end - 1), p.t0, p.r0);
+        p.t0 *= BT, p.r0 *= BR / M;
+        p.x_rows = at < end ? a.tokens - p.t0 : 0, p.w_rows = at < end ? a.rows - p.r0 : 0;
+        // four blocks' scales of a token, or (the waves behind those) of a wave's weight rows, lane WR m + wr
+        p.scale = slot < BT / 64 ? a.Xs + (uint64_t)min(p.t0 + slot * 64 + lane, a.tokens - 1) * a.spitch
+                                 : (M == 2 && lane / WR % M ? a.Wus : a.Ws) +
+                                       (uint64_t)(min(p.r0 + lane % WR * NR * 16, a.rows - 1) / 128) * a.spitch;
+        return p;
+    };
+    // A step's loads one by one, [first, last) of them: kPieces - 1 times
+    // kRows rows, then the scales.
+    constexpr int kPieces = (BT + BR) / kRows + 1;
+    auto fetch = [&](const Place &p, int b, uint8_t *to, uint32_t *to_scale, int first_piece, int last_piece) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = first_piece; i < last_piece; i++) {
+            const int j = i * kRows;  // of the stage's rows
+            if (j == BT + BR) {
+                dma4(p.scale + (b & ~3), to_scale + slot * 64);
+                continue;
+            }
+            const int in_w = j - BT, row = in_w < 0 ? j : in_w % (BR / M);
+            const uint8_t *m = in_w < 0 ? a.X + (uint64_t)(p.t0 + row) * a.pitch
+                                        : (in_w < BR / M ? a.W : a.Wu) + (uint64_t)(p.r0 + row) * a.pitch;
+            const uint32_t n = (uint32_t)__builtin_amdgcn_readfirstlane(max(min((in_w < 0 ? p.x_rows : p.w_rows) - row, kRows), 0));
+            dma16(tile_buffer(m, n * (uint32_t)a.pitch), from, b * 128, to + wave * 1024 + j * 128);
+        }
+    };
+
+    // ---- multiplying them
+    v4f acc[M][NR][NT];
+    auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int m = 0; m < M; m++)
+#pragma unroll
+            for (int r = 0; r < NR; r++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[m][r][t] = v4f{0, 0, 0, 0};
+    };
+    const int s0 = in * 128 + (part ^ swizzle(in)) * 16, s1 = in * 128 + ((part + 4) ^ swizzle(in)) * 16;
+    auto frag = [&](const uint8_t *q) __attribute__((always_inline)) {
+        const v4i lo = *(const v4i *)(q + s0), hi = *(const v4i *)(q + s1);
+        return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    // A step's weights, its first 32 tokens and its scales are read while the
+    // step before still multiplies, later tokens 32 ahead.
+    decltype(operand<EXACT>(v8i{}, 0)) wf[M * NR];
+    v8i xf[2];
+    uint32_t sx[NT], sw[M];
+    auto weights = [&](const uint8_t *cur, int i) __attribute__((always_inline)) {
+        return operand<EXACT>(frag(cur + (BT + i / NR * (BR / 2)) * 128 + (wr * NR + i % NR) * 2048), sw[i / NR]);
+    };
+    auto scales = [&](int b, const uint32_t *scale) __attribute__((always_inline)) {
+        const int shift = 8 * (b & 3);
+#pragma unroll
+        for (int m = 0; m < M; m++) sw[m] = scale[BT + m * WR + wr] >> shift & 255u;
+#pragma unroll
+        for (int t = 0; t < NT; t++) sx[t] = scale[(wt * NT + t) * 16 + in] >> shift & 255u;
+    };
+    auto finish = [&](int t0, int r0) __attribute__((always_inline)) {
+        const int row = r0 + wr * NR * 16;
+        const bool whole = r0 + BR / M <= a.rows && vec;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int token = t0 + (wt * NT + t) * 16;
+            v4f h[NR];
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                h[r] = acc[0][r][t];
+                if constexpr (OUT == kHidden)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) h[r][i] = silu_times(h[r][i], acc[M - 1][r][t][i]);
+            }
+            if (!whole) {
+                if (token + in < a.tokens)
+#pragma unroll
+                    for (int r = 0; r < NR; r++)
+                        store_some<OUT>(a, (token + in) * a.stride + a.offset + row + 16 * r + 4 * part,
+                                        a.rows - row - 16 * r - 4 * part, h[r]);
+                continue;
+            }
+            // 16 bytes a lane at its token's row + `mine` and as much again at
+            // `mine` + `more`
+            v4i v[OUT == kBf16 ? NR / 2 : NR];
+            if constexpr (OUT == kBf16) {
+                // lanes 16 apart hold rows 4 on: of two sets of 16 rows one
+                // lane takes the first's eight rows, the other the second's
+#pragma unroll
+                for (int r = 0; r < NR; r += 2) {
+                    const auto lo = __builtin_amdgcn_permlane16_swap(bf16_pair(h[r][0], h[r][1]), bf16_pair(h[r + 1][0], h[r + 1][1]), false, false);
+                    const auto hi = __builtin_amdgcn_permlane16_swap(bf16_pair(h[r][2], h[r][3]), bf16_pair(h[r + 1][2], h[r + 1][3]), false, false);
+                    v[r / 2] = v4i{(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < NR; r++) v[r] = __builtin_bit_cast(v4i, h[r]);
+            }
+            constexpr int kMore = OUT == kBf16 ? 32 : 16;
+            const int mine = OUT == kBf16 ? 16 * (part % 2) + part / 2 * 8 : 4 * part;
+            constexpr int kSets = sizeof(v) / sizeof(v[0]);
+#pragma unroll
+            for (int k = 0; k + 1 < kSets; k += 2) {
+                // 128 bytes of a token in one store: the first stores the
+                // first eight tokens of both, the second the other eight
+                const bool low = in < 8;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int got = __builtin_amdgcn_update_dpp(0, low ? v[k + 1][i] : v[k][i], 0x128, 0xf, 0xf, true);  // of lane ^ 8
+                    v[k][i] = low ? v[k][i] : got;
+                    v[k + 1][i] = low ? got : v[k + 1][i];
+                }
+                const int64_t at = (token + in % 8) * a.stride + a.offset + row + mine + k * kMore + (low ? 0 : kMore);
+                if (token + in % 8 < a.tokens) store16<OUT>(a, at, v[k]);
+                if (token + in % 8 + 8 < a.tokens) store16<OUT>(a, at + 8 * a.stride, v[k + 1]);
+            }
+            if constexpr (kSets % 2)
+                if (token + in < a.tokens) store16<OUT>(a, (token + in) * a.stride + a.offset + row + mine, v[kSets - 1]);
+        }
+    };
+    auto part_of = [&](int t) __attribute__((always_inline)) {
+        v4f *to[M * NR];
+#pragma unroll
+        for (int i = 0; i < M * NR; i++) to[i] = &acc[i / NR][i % NR][t];
+        multiply<M * NR>(wf, operand<EXACT>(xf[t & 1], sx[t]), to);
+    };
+    auto load_first = [&](const uint8_t *cur, const uint32_t *scale) __attribute__((always_inline)) {
+        scales(0, scale);
+        xf[0] = frag(cur + wt * NT * 2048), xf[1] = frag(cur + (wt * NT + 1) * 2048);
+#pragma unroll
+        for (int i = 0; i < M * NR; i++) wf[i] = weights(cur, i);
+    };
+    static_assert(NT % 2 == 0, "");
+    int at = first;
+    Place here = place(at), then = place(at + tiles.per_xcd);
+    // The loads of the step after next begin when this one has been read, and
+    // go on between the next one's first products, so that no wave waits to
+    // issue them.
+    constexpr int kSpread = NT - 2 < 2 ? NT - 2 : 2, kTail = kSpread ? (kPieces + 1) / 2 : kPieces;
+    constexpr int kEach = kSpread ? (kPieces - kTail + kSpread - 1) / kSpread : 0;
+    auto fetch_step = [&](int b, uint8_t *to, uint32_t *to_scale, int first_piece, int last_piece) __attribute__((always_inline)) {
+        const bool over = b >= a.kb;
+        const Place p = {over ? then.t0 : here.t0, over ? then.r0 : here.r0, over ? then.x_rows : here.x_rows,
+                         over ? then.w_rows : here.w_rows, over ? then.scale : here.scale};
+        fetch(p, over ? b - a.kb : b, to, to_scale, first_piece, last_piece);
+    };
+    auto step = [&](int b, uint8_t *cur, uint32_t *scale, uint8_t *next, uint32_t *next_scale) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t + 2 < NT; t++) {
+            if (t < kSpread) fetch_step(b + 1, next, next_scale, min(kTail + t * kEach, kPieces), min(kTail + (t + 1) * kEach, kPieces));
+            part_of(t);
+            xf[t & 1] = frag(cur + (wt * NT + t + 2) * 2048);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): the next step is in LDS, this one is read
+        __builtin_amdgcn_s_barrier();
+        fetch_step(b + 2, cur, scale, 0, kTail);
+        part_of(NT - 2);
+        xf[0] = frag(next + wt * NT * 2048);
+        part_of(NT - 1);
+        scales(b + 1, next_scale);
+#pragma unroll
+        for (int i = 0; i < M * NR; i++) wf[i] = weights(next, i);
+        xf[1] = frag(next + (wt * NT + 1) * 2048);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // One tile whose first step lies in `one`; its last steps bring the next
+    // tile's first, so that its outputs are stored while those arrive.
+    auto tile = [&](uint8_t *one, uint32_t *one_scale, uint8_t *two, uint32_t *two_scale) __attribute__((always_inline)) {
+        load_first(one, one_scale);
+        clear();
+        int b = 0;
+        for (; b + 1 < a.kb; b += 2) {
+            step(b, one, one_scale, two, two_scale);
+            step(b + 1, two, two_scale, one, one_scale);
+        }
+        if (b < a.kb) step(b, one, one_scale, two, two_scale);
+        finish(here.t0, here.r0);
+        at += tiles.per_xcd;
+        here = then;
+        then = place(at + tiles.per_xcd);
+    };
+    fetch(here, 0, s_even, s_even_scale, 0, kPieces);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    fetch_step(1, s_odd, s_odd_scale, 0, kTail);
+    while (true) {
+        tile(s_even, s_even_scale, s_odd, s_odd_scale);
+        if (at >= end) break;
+        if (a.kb & 1) {
+            tile(s_odd, s_odd_scale, s_even, s_even_scale);
+            if (at >= end) break;
+        }
+    }
+}
+
+// A tile's size, the workgroups of it that a CU holds, and what a step of one
+// and of all of them takes, in us (one MI355X).
+struct Shape {
+    int tokens, rows, resident;
+    float one, all;
+};
+// Measured from whole calls of 20 and 48 steps. 8-bit: 64 x 64 10.4 us alone,
+// 46.4 for 2.5 rounds of four a CU; 128 x 128 18.0 and 68.0 for 2.5 rounds of
+// two; 256 x 128 25.5; 256 x 256 37.3, 210 for five rounds. bf16 values: 14.6 and
+// 74.9; 28.0 and 485 for ten rounds; 42; 62 and 395 for five rounds.
+constexpr Shape kShapes[2][4] = {{{64, 64, 4, 0.5f, 0.9f}, {128, 128, 2, 0.9f, 1.25f}, {256, 128, 1, 1.27f, 1.27f}, {256, 256, 1, 1.8f, 1.8f}},
+                                 {{64, 64, 4, 0.7f, 1.45f}, {128, 128, 2, 1.45f, 2.2f}, {256, 128, 1, 2.2f, 2.2f}, {256, 256, 1, 3.5f, 3.5f}}};
+
+template <int BT, int BR, int WT, int WR, bool EXACT, Out OUT>
+void tiles(sm_ctx *ctx, const Product &a, int cus, int resident) {
+    const int m = OUT == kHidden ? 2 : 1;
+    Tiles t = {(a.tokens + BT - 1) / BT, (a.rows + BR / m - 1) / (BR / m), 0};
+    // One block of columns: nothing is left of a tile's steps to bring the next in.
+    const int n = t.tokens * t.rows, grid = (a.kb < 2 ? (n + 7) / 8 : min((n + 7) / 8, max(cus / 8, 1) * resident)) * 8;
+    t.per_xcd = grid / 8;
+    k_f8_tile<BT, BR, WT, WR, EXACT, OUT><<<grid, 64 * WT * WR, 0, ctx->stream>>>(a, t, aligned(a, OUT == kBf16 ? 8 : 4));
+}
+
+// Up to 16 tokens, and where 16-row workgroups of 64 tokens are fewer than the
+// GPU's CUs, the waves that share out the columns (2560 x 2560, 64 tokens: 8.9
+// us against 10.6 in tiles; 2560 x 640, 256 tokens: 9.0 against 10.8; 2560 x
+// 10240, 32 tokens: 13.8 against 10.7). Else the tile whose rounds over the
+// GPU take least.
+template <bool EXACT, Out OUT>
+void multiply_by_size(sm_ctx *ctx, const Product &a) {
+    if (a.tokens <= 16 || (int64_t)((a.rows + 15) / 16) * ((a.tokens + 63) / 64) <= 200) return few<EXACT, OUT>(ctx, a);
+    int cus = 256, best = 0;
+    (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, ctx->device);
+    float least = 0.0f;
+    for (int i = 0; i < 4; i++) {
+        const Shape &s = kShapes[EXACT][i];
+        const int rows = OUT == kHidden ? s.rows / 2 : s.rows;
+        const int64_t n = (int64_t)((a.tokens + s.tokens - 1) / s.tokens) * ((a.rows + rows - 1) / rows);
+        const int64_t round = (int64_t)cus * s.resident, over = (n % round + cus - 1) / cus;  // workgroups of a CU in the last round
+        const float last = over == 0 ? 0.0f : s.resident == 1 ? s.one : s.one + (s.all - s.one) * (over - 1) / (s.resident - 1);
+        const float time = n / round * s.all + last;
+        if (i == 0 || time < least) least = time, best = i;
+    }
+    const int resident = kShapes[EXACT][best].resident;
+    if (best == 0) tiles<64, 64, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
+    else if (best == 1) tiles<128, 128, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
+    else if (best == 2) tiles<256, 128, 4, 2, EXACT, OUT>(ctx, a, cus, resident);
+    else tiles<256, 256, 2, 4, EXACT, OUT>(ctx, a, cus, resident);
 }
 
 Product product_of(const F8Operand &X, const F8Operand &W, int tokens, int cols, int rows) {
@@ -171,8 +515,8 @@ int f8_project_launch(sm_ctx *ctx, const F8Operand &X, int tokens, int cols, con
                       void *Y, bool bf16, int64_t stride, int64_t offset) {
     Product a = product_of(X, W, tokens, cols, rows);
     a.R = R, a.Y = Y, a.stride = stride, a.offset = offset;
-    if (bf16) few<false, kBf16>(ctx, a);
-    else few<true, kF32>(ctx, a);
+    if (bf16) multiply_by_size<false, kBf16>(ctx, a);
+    else multiply_by_size<true, kF32>(ctx, a);
     return launched(ctx);
 }
 
@@ -182,7 +526,7 @@ int f8_gate_up_launch(sm_ctx *ctx, const F8Operand &X, int tokens, int cols, con
                       uint8_t *codes, uint8_t *scales, void *workspace) {
     Product a = product_of(X, Wg, tokens, cols, ff);
     a.Wu = Wu.codes, a.Wus = Wu.scales, a.Y = workspace, a.stride = ff;
-    few<false, kHidden>(ctx, a);
+    multiply_by_size<false, kHidden>(ctx, a);
     if (int rc = launched(ctx)) return rc;
     return f8_quantize_launch(ctx, workspace, false, tokens, ff, 1, codes, scales);
 }
