@@ -27,12 +27,13 @@ __device__ __forceinline__ float finite_magnitude(float v) {
     return a < INFINITY ? a : 0.0f;  // 0 for NaN too
 }
 // v * 2^-e is exact (or below e4m3's smallest step); the conversion rounds to
-// nearest, ties to even. A value that is not finite becomes NaN: e4m3 has no
-// infinity, and a saturated one would pass as a number.
-__device__ __forceinline__ uint32_t codes4(const float v[4], float inverse) {
+// nearest, ties to even. A value that is not finite becomes NaN (v + 0 v is v,
+// or NaN): e4m3 has no infinity, and a saturated one would pass as a number.
+template <typename V>
+__device__ __forceinline__ uint32_t codes4(const V &v, float inverse) {
     float s[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) s[i] = fabsf(v[i]) < INFINITY ? v[i] * inverse : NAN;
+    for (int i = 0; i < 4; i++) s[i] = fmaf(v[i], inverse, v[i] * 0.0f);
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(s[0], s[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], w, true);
 }

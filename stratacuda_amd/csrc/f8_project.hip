@@ -25,7 +25,7 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
-enum Out { kF32, kBf16, kHidden };  // kHidden: silu(gate) * up in f32
+enum Out { kF32, kBf16, kHidden, kCodes };  // kHidden, kCodes: silu(gate) * up in f32, in 8 bits
 
 // 32 of a row's 128 codes: lane l holds row l % 16, columns 32 (l / 16) on.
 __device__ __forceinline__ v8i load_frag(const uint8_t *p) {
@@ -78,7 +78,19 @@ __device__ __forceinline__ void multiply(const Values (&w)[N], const Values &x, 
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {  // nearest, ties to even; NaN stays NaN
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2b));
 }
-__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// g / (1 + exp(-g)) * u, with t = exp(-|g|) <= 1: silu(g) = g / (1 + t), or
+// g t / (1 + t) below 0, so that nothing overflows and 1 + t lies in [1, 2].
+// |g| log2(e) in two parts (the second corrects t to first order), one Newton
+// step on the reciprocal: seven half steps of f32 at most, in half the time of
+// expf and a division.
+__device__ __forceinline__ float silu_times(float g, float u) {
+    const float a = fabsf(g), p = a * 1.44269502f;  // log2(e) = 1.44269502 + 1.92596303e-8
+    const float r = fmaf(a, 1.92596303e-8f, fmaf(a, 1.44269502f, -p));
+    const float e = __builtin_amdgcn_exp2f(-p);
+    const float t = fmaf(e, fmaxf(fminf(r * -0.693147182f, 1e-3f), -1e-3f), e);  // the bounds are for infinities alone
+    const float d = 1.0f + t, y0 = __builtin_amdgcn_rcpf(d), y = fmaf(fmaf(-d, y0, 1.0f), y0, y0);
+    return g * (g >= 0.0f ? y : t * y) * u;
+}
 
 struct Product {
     const uint8_t *X, *Xs, *W, *Ws, *Wu, *Wus;  // Wu, Wus: the second matrix of a gated pair
@@ -87,6 +99,8 @@ struct Product {
     int tokens, rows, kb;  // rows: of one matrix
     uint64_t pitch, spitch;
     int64_t stride, offset;
+    uint8_t *codes, *scales;  // kCodes: the outputs, and their rows' bytes
+    uint64_t codes_pitch, scales_pitch;
 };
 
 // 16 bytes of a token's outputs, aligned: eight in bf16, or four to which R is added.
@@ -215,7 +229,40 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t from, uint32_t lane
 __device__ __forceinline__ void dma4(const uint8_t *src, void *lds) {
     __builtin_amdgcn_global_load_lds(src, (lds_void *)lds, 4, 0, 0);
 }
+// The waves' barrier alone (the waits are the callers'); the compiler moves no memory access over it.
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 __device__ __forceinline__ int swizzle(int row) { return row & 7; }
+
+// silu(gate) * up of one token and column by one wave, in f32 sums.
+__device__ __forceinline__ float exact_hidden(const Product &a, int token, int col, int lane) {
+    const uint64_t ws = (uint64_t)(col / 128) * a.spitch;
+    const uint8_t *x = a.X + token * a.pitch, *w = a.W + col * a.pitch, *u = a.Wu + col * a.pitch;
+    const uint8_t *sx = a.Xs + token * a.spitch, *sw = a.Ws + ws, *su = a.Wus + ws;
+    float g = 0.0f, v = 0.0f;
+#pragma unroll 4
+    for (int k = lane * 16; k < a.kb * 128; k += 1024) {  // eight lanes a block of 128
+        const v4i xc = *(const v4i *)(x + k), wc = *(const v4i *)(w + k), uc = *(const v4i *)(u + k);
+        const int e = sx[k / 128] - 127, eg = e + sw[k / 128] - 127, ev = e + su[k / 128] - 127;
+        float pg = 0.0f, pv = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const v2f x0 = __builtin_amdgcn_cvt_pk_f32_fp8(xc[i], false), x1 = __builtin_amdgcn_cvt_pk_f32_fp8(xc[i], true);
+            const v2f w0 = __builtin_amdgcn_cvt_pk_f32_fp8(wc[i], false), w1 = __builtin_amdgcn_cvt_pk_f32_fp8(wc[i], true);
+            const v2f u0 = __builtin_amdgcn_cvt_pk_f32_fp8(uc[i], false), u1 = __builtin_amdgcn_cvt_pk_f32_fp8(uc[i], true);
+            pg = fmaf(x0[0], w0[0], fmaf(x0[1], w0[1], fmaf(x1[0], w1[0], fmaf(x1[1], w1[1], pg))));
+            pv = fmaf(x0[0], u0[0], fmaf(x0[1], u0[1], fmaf(x1[0], u1[0], fmaf(x1[1], u1[1], pv))));
+        }
+        g = g + __builtin_amdgcn_ldexpf(pg, eg);
+        v = v + __builtin_amdgcn_ldexpf(pv, ev);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) g = g + __shfl_xor(g, d, 64), v = v + __shfl_xor(v, d, 64);
+    return silu_times(g, v);
+}
 
 // The tiles in the order of the eight XCDs that workgroups go round: each XCD
 // takes neighbouring tiles, four of tokens by as many of rows, so that its L2
@@ -231,7 +278,7 @@ struct Tiles {
 
 template <int BT, int BR, int WT, int WR, bool EXACT, Out OUT>
 __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles, bool vec) {
-    constexpr int kThreads = 64 * WT * WR, NT = BT / WT / 16, M = OUT == kHidden ? 2 : 1, NR = BR / WR / 16 / M;
+    constexpr int kThreads = 64 * WT * WR, NT = BT / WT / 16, M = OUT >= kHidden ? 2 : 1, NR = BR / WR / 16 / M;
     constexpr int kStage = (BT + BR) * 128, kRows = kThreads / 8;  // rows that the threads bring at a time
     static_assert(BT % kRows == 0 && BR / M % kRows == 0 && kRows % 8 == 0 && BT % 64 == 0 && BT / 64 < WT * WR && NT >= 2, "");
     // two variables, so that reads of one need not wait for the DMA into the other
@@ -311,6 +358,111 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
         for (int m = 0; m < M; m++) sw[m] = scale[BT + m * WR + wr] >> shift & 255u;
 #pragma unroll
         for (int t = 0; t < NT; t++) sx[t] = scale[(wt * NT + t) * 16 + in] >> shift & 255u;
+    };
+    // 8-bit outputs: a tile's 128 columns are one block of scales. A wave has 32
+    // of them, so the largest magnitudes meet in LDS. The sums are near, not
+    // exact (above): where a token's largest lies so near to a scale's border
+    // that the exact one may lie past it, the columns that may hold it (the
+    // first eight of them) are summed again in f32, and the scale is theirs.
+    __shared__ float s_most[OUT == kCodes ? WR : 1][OUT == kCodes ? BT : 1];
+    __shared__ uint32_t s_columns[OUT == kCodes ? BT : 1][4], s_any;
+    auto finish_codes = [&](int t0, int r0) __attribute__((always_inline)) {
+        static_assert(OUT != kCodes || (NR == 2 && BR == 256 && BT <= 32 * WT * WR), "");
+        constexpr float kNear = 1.0f / 4096;  // the sums are off by about 2e-5
+        // within kNear of 1.75 * 2^x, by the bits: kNear of the 2^23 steps from 2^x to 2^(x + 1), times 1.75
+        auto near = [](float m) {
+            constexpr int kBits = (int)(kNear * 1.75f * 8388608.0f);
+            return abs((int)(__float_as_uint(m) & 0x7fffffu) - 0x600000) <= kBits;
+        };
+        auto wait = []() {
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+            barrier();
+        };
+        const int col = wr * 32 + 4 * part;  // of the block
+        if (threadIdx.x == 0) s_any = 0;
+        for (int i = threadIdx.x; i < BT * 4; i += kThreads) s_columns[0][i] = 0;
+        const bool whole = r0 + BR / M <= a.rows;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            float most = 0.0f;
+#pragma unroll
+            for (int r = 0; r < NR; r++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float h = silu_times(acc[0][r][t][i], acc[M - 1][r][t][i]);
+                    acc[0][r][t][i] = whole || r0 + col + 16 * r + i < a.rows ? h : 0.0f;
+                    most = fmaxf(most, fabsf(acc[0][r][t][i]));
+                }
+            if (__any(most == INFINITY)) {
+                most = 0.0f;
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) most = fmaxf(most, f8::finite_magnitude(acc[0][r][t][i]));
+            }
+            most = fmaxf(most, __shfl_xor(most, 16, 64));
+            most = fmaxf(most, __shfl_xor(most, 32, 64));
+            if (part == 0) s_most[wr][(wt * NT + t) * 16 + in] = most;
+        }
+        wait();
+        float most[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int token = (wt * NT + t) * 16 + in;
+            most[t] = s_most[0][token];
+#pragma unroll
+            for (int k = 1; k < WR; k++) most[t] = fmaxf(most[t], s_most[k][token]);
+            if (t0 + token < a.tokens && near(most[t])) {
+                uint32_t bits = 0;
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (f8::finite_magnitude(acc[0][r][t][i]) >= most[t] * (1.0f - 2 * kNear)) bits |= 1u << (16 * r + 4 * part + i);
+                if (bits) atomicOr(&s_columns[token][wr], bits);
+                s_any = 1;
+            }
+        }
+        wait();
+        if (__builtin_amdgcn_readfirstlane(s_any)) {
+            const int token = wave + lane * (WT * WR);
+            bool mine = false;
+            if (token < BT)
+#pragma unroll
+                for (int k = 0; k < 4; k++) mine |= s_columns[token][k] != 0;
+            uint64_t todo = __ballot(mine);
+            while (todo) {
+                const int one = wave + __builtin_ctzll(todo) * (WT * WR);
+                todo &= todo - 1;
+                float m = 0.0f;
+                int left = 8;
+                for (int k = 0; k < 4; k++) {
+                    uint32_t bits = __builtin_amdgcn_readfirstlane(s_columns[one][k]);
+                    for (; bits && left; bits &= bits - 1, left--)
+                        m = fmaxf(m, f8::finite_magnitude(exact_hidden(a, t0 + one, r0 + 32 * k + __builtin_ctz(bits), lane)));
+                }
+                if (lane == 0) s_most[0][one] = m;
+            }
+            wait();
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int token = t0 + (wt * NT + t) * 16 + in;
+            const float m = near(most[t]) ? s_most[0][(wt * NT + t) * 16 + in] : most[t];
+            const uint32_t byte = f8::scale_byte(m);
+            const float inverse = f8::inverse_scale(byte);
+            // of two sets of 16 columns one lane takes eight of the first, the other eight of the second
+            const auto v = __builtin_amdgcn_permlane16_swap(f8::codes4(acc[0][0][t], inverse), f8::codes4(acc[0][NR - 1][t], inverse), false, false);
+            if (token < a.tokens) {
+                *(uint2 *)(a.codes + token * a.codes_pitch + r0 + wr * 32 + 16 * (part % 2) + part / 2 * 8) = make_uint2(v[0], v[1]);
+                if (wr == 0 && part == 0) {
+                    uint8_t *to = a.scales + token * a.scales_pitch;
+                    to[r0 / 128] = (uint8_t)byte;
+                    if (r0 + 128 >= a.rows)
+                        for (uint32_t k = r0 / 128 + 1; k < a.scales_pitch; k++) to[k] = 127;
+                }
+            }
+        }
     };
     auto finish = [&](int t0, int r0) __attribute__((always_inline)) {
         const int row = r0 + wr * NR * 16;
@@ -407,7 +559,7 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): the next step is in LDS, this one is read
-        __builtin_amdgcn_s_barrier();
+        barrier();
         fetch_step(b + 2, cur, scale, 0, kTail);
         part_of(NT - 2);
         xf[0] = frag(next + wt * NT * 2048);
@@ -429,7 +581,8 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
             step(b + 1, two, two_scale, one, one_scale);
         }
         if (b < a.kb) step(b, one, one_scale, two, two_scale);
-        finish(here.t0, here.r0);
+        if constexpr (OUT == kCodes) finish_codes(here.t0, here.r0);
+        else finish(here.t0, here.r0);
         at += tiles.per_xcd;
         here = then;
         then = place(at + tiles.per_xcd);
@@ -463,7 +616,7 @@ constexpr Shape kShapes[2][4] = {{{64, 64, 4, 0.5f, 0.9f}, {128, 128, 2, 0.9f, 1
 
 template <int BT, int BR, int WT, int WR, bool EXACT, Out OUT>
 void tiles(sm_ctx *ctx, const Product &a, int cus, int resident) {
-    const int m = OUT == kHidden ? 2 : 1;
+    const int m = OUT >= kHidden ? 2 : 1;
     Tiles t = {(a.tokens + BT - 1) / BT, (a.rows + BR / m - 1) / (BR / m), 0};
     // One block of columns: nothing is left of a tile's steps to bring the next in.
     const int n = t.tokens * t.rows, grid = (a.kb < 2 ? (n + 7) / 8 : min((n + 7) / 8, max(cus / 8, 1) * resident)) * 8;
@@ -471,31 +624,65 @@ void tiles(sm_ctx *ctx, const Product &a, int cus, int resident) {
     k_f8_tile<BT, BR, WT, WR, EXACT, OUT><<<grid, 64 * WT * WR, 0, ctx->stream>>>(a, t, aligned(a, OUT == kBf16 ? 8 : 4));
 }
 
+int compute_units(sm_ctx *ctx) {
+    int cus = 0;
+    return hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, ctx->device) == hipSuccess && cus > 0 ? cus : 256;
+}
+
 // Up to 16 tokens, and where 16-row workgroups of 64 tokens are fewer than the
 // GPU's CUs, the waves that share out the columns (2560 x 2560, 64 tokens: 8.9
 // us against 10.6 in tiles; 2560 x 640, 256 tokens: 9.0 against 10.8; 2560 x
-// 10240, 32 tokens: 13.8 against 10.7). Else the tile whose rounds over the
-// GPU take least.
-template <bool EXACT, Out OUT>
-void multiply_by_size(sm_ctx *ctx, const Product &a) {
-    if (a.tokens <= 16 || (int64_t)((a.rows + 15) / 16) * ((a.tokens + 63) / 64) <= 200) return few<EXACT, OUT>(ctx, a);
-    int cus = 256, best = 0;
-    (void)hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, ctx->device);
-    float least = 0.0f;
+// 10240, 32 tokens: 13.8 against 10.7).
+bool takes_few(const Product &a) {
+    return a.tokens <= 16 || (int64_t)((a.rows + 15) / 16) * ((a.tokens + 63) / 64) <= 200;
+}
+// Else the tile whose rounds over the GPU take least: its index in kShapes and
+// the time of a step of all of them, in us.
+int best_shape(const Product &a, bool exact, int m, int cus, float *us) {
+    int best = 0;
     for (int i = 0; i < 4; i++) {
-        const Shape &s = kShapes[EXACT][i];
-        const int rows = OUT == kHidden ? s.rows / 2 : s.rows;
-        const int64_t n = (int64_t)((a.tokens + s.tokens - 1) / s.tokens) * ((a.rows + rows - 1) / rows);
+        const Shape &s = kShapes[exact][i];
+        const int64_t n = (int64_t)((a.tokens + s.tokens - 1) / s.tokens) * ((a.rows + s.rows / m - 1) / (s.rows / m));
         const int64_t round = (int64_t)cus * s.resident, over = (n % round + cus - 1) / cus;  // workgroups of a CU in the last round
         const float last = over == 0 ? 0.0f : s.resident == 1 ? s.one : s.one + (s.all - s.one) * (over - 1) / (s.resident - 1);
         const float time = n / round * s.all + last;
-        if (i == 0 || time < least) least = time, best = i;
+        if (i == 0 || time < *us) *us = time, best = i;
     }
-    const int resident = kShapes[EXACT][best].resident;
+    return best;
+}
+template <bool EXACT, Out OUT>
+void multiply_by_size(sm_ctx *ctx, const Product &a, int cus) {
+    if (takes_few(a)) return few<EXACT, OUT>(ctx, a);
+    float us = 0.0f;
+    const int best = best_shape(a, EXACT, OUT == kHidden ? 2 : 1, cus, &us), resident = kShapes[EXACT][best].resident;
     if (best == 0) tiles<64, 64, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
     else if (best == 1) tiles<128, 128, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
     else if (best == 2) tiles<256, 128, 4, 2, EXACT, OUT>(ctx, a, cus, resident);
     else tiles<256, 256, 2, 4, EXACT, OUT>(ctx, a, cus, resident);
+}
+
+// A gated pair: sums to f32 into the workspace and the conversion of rows, or
+// one kernel on the 8-bit matrix unit whose tiles of 128 columns end in codes.
+// That takes 1.6 us a step and 14 us a tile of 256 tokens, 1.0 and 6 of 128
+// (measured as above: 4096 tokens, 2560 to 8192, 308 us apart, 186 and 208;
+// 512 tokens 50, 49 and 32; 128 tokens 24, 44 and 30).
+int gate_up(sm_ctx *ctx, Product &a, uint8_t *codes, uint8_t *scales, void *workspace) {
+    const int cus = compute_units(ctx);
+    const F8Layout L = f8_layout(a.tokens, a.rows, 1);
+    a.codes = codes, a.scales = scales, a.codes_pitch = L.pitch, a.scales_pitch = L.spitch;
+    if (!takes_few(a)) {
+        auto rounds = [&](int tokens) { return ((int64_t)((a.tokens + tokens - 1) / tokens) * (int64_t)(L.pitch / 128) + cus - 1) / cus; };
+        float apart = 0.0f;
+        best_shape(a, true, 2, cus, &apart);
+        apart = apart * a.kb + 3.0f + 5.0f * a.tokens * a.rows / 4e6f;
+        const float wide = rounds(256) * (1.6f * a.kb + 14.0f), narrow = rounds(128) * (1.0f * a.kb + 6.0f);
+        if (wide < apart && wide < narrow) return tiles<256, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
+        if (narrow < apart) return tiles<128, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
+    }
+    a.Y = workspace, a.stride = a.rows;
+    multiply_by_size<true, kHidden>(ctx, a, cus);
+    if (int rc = launched(ctx)) return rc;
+    return f8_quantize_launch(ctx, workspace, false, a.tokens, a.rows, 1, codes, scales);
 }
 
 Product product_of(const F8Operand &X, const F8Operand &W, int tokens, int cols, int rows) {
@@ -515,8 +702,8 @@ int f8_project_launch(sm_ctx *ctx, const F8Operand &X, int tokens, int cols, con
                       void *Y, bool bf16, int64_t stride, int64_t offset) {
     Product a = product_of(X, W, tokens, cols, rows);
     a.R = R, a.Y = Y, a.stride = stride, a.offset = offset;
-    if (bf16) multiply_by_size<false, kBf16>(ctx, a);
-    else multiply_by_size<true, kF32>(ctx, a);
+    if (bf16) multiply_by_size<false, kBf16>(ctx, a, compute_units(ctx));
+    else multiply_by_size<true, kF32>(ctx, a, compute_units(ctx));
     return launched(ctx);
 }
 
@@ -525,10 +712,8 @@ uint64_t f8_gate_up_workspace(int tokens, int ff) { return (uint64_t)tokens * ff
 int f8_gate_up_launch(sm_ctx *ctx, const F8Operand &X, int tokens, int cols, const F8Operand &Wg, const F8Operand &Wu, int ff,
                       uint8_t *codes, uint8_t *scales, void *workspace) {
     Product a = product_of(X, Wg, tokens, cols, ff);
-    a.Wu = Wu.codes, a.Wus = Wu.scales, a.Y = workspace, a.stride = ff;
-    multiply_by_size<false, kHidden>(ctx, a);
-    if (int rc = launched(ctx)) return rc;
-    return f8_quantize_launch(ctx, workspace, false, tokens, ff, 1, codes, scales);
+    a.Wu = Wu.codes, a.Wus = Wu.scales;
+    return gate_up(ctx, a, codes, scales, workspace);
 }
 
 }  // namespace smi
