@@ -129,6 +129,69 @@ __device__ __forceinline__ void store_some(const Product &a, int64_t at, int n, 
     }
 }
 
+// A wave's sums: 16 NT tokens from `first_token` on, 16 NR rows from `row` on;
+// `whole`: all of the rows are there, and aligned.
+template <Out OUT, int M, int NR, int NT>
+__device__ __forceinline__ void store_tile(const Product &a, int first_token, int row, const v4f (&acc)[M][NR][NT], bool whole,
+                                           int in, int part) {
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const int token = first_token + t * 16;
+        v4f h[NR];
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            h[r] = acc[0][r][t];
+            if constexpr (OUT == kHidden)
+#pragma unroll
+                for (int i = 0; i < 4; i++) h[r][i] = silu_times(h[r][i], acc[M - 1][r][t][i]);
+        }
+        if (!whole) {
+            if (token + in < a.tokens)
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+                    store_some<OUT>(a, (token + in) * a.stride + a.offset + row + 16 * r + 4 * part,
+                                    a.rows - row - 16 * r - 4 * part, h[r]);
+            continue;
+        }
+        // 16 bytes a lane at its token's row + `mine` and as much again at
+        // `mine` + `more`
+        v4i v[OUT == kBf16 ? NR / 2 : NR];
+        if constexpr (OUT == kBf16) {
+            // lanes 16 apart hold rows 4 on: of two sets of 16 rows one
+            // lane takes the first's eight rows, the other the second's
+#pragma unroll
+            for (int r = 0; r < NR; r += 2) {
+                const auto lo = __builtin_amdgcn_permlane16_swap(bf16_pair(h[r][0], h[r][1]), bf16_pair(h[r + 1][0], h[r + 1][1]), false, false);
+                const auto hi = __builtin_amdgcn_permlane16_swap(bf16_pair(h[r][2], h[r][3]), bf16_pair(h[r + 1][2], h[r + 1][3]), false, false);
+                v[r / 2] = v4i{(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < NR; r++) v[r] = __builtin_bit_cast(v4i, h[r]);
+        }
+        constexpr int kMore = OUT == kBf16 ? 32 : 16;
+        const int mine = OUT == kBf16 ? 16 * (part % 2) + part / 2 * 8 : 4 * part;
+        constexpr int kSets = sizeof(v) / sizeof(v[0]);
+#pragma unroll
+        for (int k = 0; k + 1 < kSets; k += 2) {
+            // 128 bytes of a token in one store: the first stores the
+            // first eight tokens of both, the second the other eight
+            const bool low = in < 8;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int got = __builtin_amdgcn_update_dpp(0, low ? v[k + 1][i] : v[k][i], 0x128, 0xf, 0xf, true);  // of lane ^ 8
+                v[k][i] = low ? v[k][i] : got;
+                v[k + 1][i] = low ? got : v[k + 1][i];
+            }
+            const int64_t at = (token + in % 8) * a.stride + a.offset + row + mine + k * kMore + (low ? 0 : kMore);
+            if (token + in % 8 < a.tokens) store16<OUT>(a, at, v[k]);
+            if (token + in % 8 + 8 < a.tokens) store16<OUT>(a, at + 8 * a.stride, v[k + 1]);
+        }
+        if constexpr (kSets % 2)
+            if (token + in < a.tokens) store16<OUT>(a, (token + in) * a.stride + a.offset + row + mine, v[kSets - 1]);
+    }
+}
+
 // -------------------------------------------------------- few tokens
 // A workgroup's eight waves share 16 weight rows and 16 TT tokens and take
 // the blocks of 128 columns in turn, codes straight from memory into the
@@ -234,6 +297,9 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
 }
 __device__ __forceinline__ int swizzle(int row) { return row & 7; }
 
@@ -464,66 +530,6 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
             }
         }
     };
-    auto finish = [&](int t0, int r0) __attribute__((always_inline)) {
-        const int row = r0 + wr * NR * 16;
-        const bool whole = r0 + BR / M <= a.rows && vec;
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int token = t0 + (wt * NT + t) * 16;
-            v4f h[NR];
-#pragma unroll
-            for (int r = 0; r < NR; r++) {
-                h[r] = acc[0][r][t];
-                if constexpr (OUT == kHidden)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) h[r][i] = silu_times(h[r][i], acc[M - 1][r][t][i]);
-            }
-            if (!whole) {
-                if (token + in < a.tokens)
-#pragma unroll
-                    for (int r = 0; r < NR; r++)
-                        store_some<OUT>(a, (token + in) * a.stride + a.offset + row + 16 * r + 4 * part,
-                                        a.rows - row - 16 * r - 4 * part, h[r]);
-                continue;
-            }
-            // 16 bytes a lane at its token's row + `mine` and as much again at
-            // `mine` + `more`
-            v4i v[OUT == kBf16 ? NR / 2 : NR];
-            if constexpr (OUT == kBf16) {
-                // lanes 16 apart hold rows 4 on: of two sets of 16 rows one
-                // lane takes the first's eight rows, the other the second's
-#pragma unroll
-                for (int r = 0; r < NR; r += 2) {
-                    const auto lo = __builtin_amdgcn_permlane16_swap(bf16_pair(h[r][0], h[r][1]), bf16_pair(h[r + 1][0], h[r + 1][1]), false, false);
-                    const auto hi = __builtin_amdgcn_permlane16_swap(bf16_pair(h[r][2], h[r][3]), bf16_pair(h[r + 1][2], h[r + 1][3]), false, false);
-                    v[r / 2] = v4i{(int)lo[0], (int)hi[0], (int)lo[1], (int)hi[1]};
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < NR; r++) v[r] = __builtin_bit_cast(v4i, h[r]);
-            }
-            constexpr int kMore = OUT == kBf16 ? 32 : 16;
-            const int mine = OUT == kBf16 ? 16 * (part % 2) + part / 2 * 8 : 4 * part;
-            constexpr int kSets = sizeof(v) / sizeof(v[0]);
-#pragma unroll
-            for (int k = 0; k + 1 < kSets; k += 2) {
-                // 128 bytes of a token in one store: the first stores the
-                // first eight tokens of both, the second the other eight
-                const bool low = in < 8;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int got = __builtin_amdgcn_update_dpp(0, low ? v[k + 1][i] : v[k][i], 0x128, 0xf, 0xf, true);  // of lane ^ 8
-                    v[k][i] = low ? v[k][i] : got;
-                    v[k + 1][i] = low ? got : v[k + 1][i];
-                }
-                const int64_t at = (token + in % 8) * a.stride + a.offset + row + mine + k * kMore + (low ? 0 : kMore);
-                if (token + in % 8 < a.tokens) store16<OUT>(a, at, v[k]);
-                if (token + in % 8 + 8 < a.tokens) store16<OUT>(a, at + 8 * a.stride, v[k + 1]);
-            }
-            if constexpr (kSets % 2)
-                if (token + in < a.tokens) store16<OUT>(a, (token + in) * a.stride + a.offset + row + mine, v[kSets - 1]);
-        }
-    };
     auto part_of = [&](int t) __attribute__((always_inline)) {
         v4f *to[M * NR];
 #pragma unroll
@@ -582,7 +588,7 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
         }
         if (b < a.kb) step(b, one, one_scale, two, two_scale);
         if constexpr (OUT == kCodes) finish_codes(here.t0, here.r0);
-        else finish(here.t0, here.r0);
+        else store_tile<OUT>(a, here.t0 + wt * NT * 16, here.r0 + wr * NR * 16, acc, here.r0 + BR / M <= a.rows && vec, in, part);
         at += tiles.per_xcd;
         here = then;
         then = place(at + tiles.per_xcd);
@@ -601,18 +607,130 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
     }
 }
 
-// A tile's size, the workgroups of it that a CU holds, and what a step of one
-// and of all of them takes, in us (one MI355X).
+// ------------------------------------- some tokens: few tiles, one a workgroup
+// Where 64 x 64 tiles leave CUs idle, a step's latency is the time: four steps
+// in flight (S - 1 ahead, waited for by their number), and KG groups of four
+// waves that take a block of 128 columns each at a time, whose sums meet in LDS
+// in their order. 2560 columns to 2560 rows, 256 tokens, to bf16: 11.0 us in
+// the persistent tiles, 8.4 here.
+template <int KG, int S, bool EXACT, Out OUT>
+__global__ void __launch_bounds__(256 * KG) k_f8_deep(Product a, Tiles tiles, bool vec) {
+    constexpr int M = OUT >= kHidden ? 2 : 1, NT = 2, NR = 2 / M, kLoads = 5;
+    static_assert(S == 4, "");
+    __shared__ __attribute__((aligned(16))) uint8_t s_0[KG * 16384], s_1[KG * 16384], s_2[KG * 16384], s_3[KG * 16384];
+    __shared__ uint32_t s_c0[KG * 128], s_c1[KG * 128], s_c2[KG * 128], s_c3[KG * 128];
+    const int lane = threadIdx.x % 64, in = lane % 16, part = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = wave / 4, wt = wave / 2 % 2, wr = wave % 2;
+    const int xcd = blockIdx.x % 8, n = tiles.tokens * tiles.rows;
+    const int at = xcd * (n / 8) + min(xcd, n % 8) + blockIdx.x / 8, end = (xcd + 1) * (n / 8) + min(xcd + 1, n % 8);
+    if (at >= end) return;
+    int t0, r0;
+    tiles.locate(at, t0, r0);
+    t0 *= 64, r0 *= 64 / M;
+
+    const int thread = threadIdx.x % 256;
+    const uint32_t from = thread / 8 * (uint32_t)a.pitch + ((thread ^ swizzle(thread / 8)) & 7) * 16;
+    const uint8_t *from_scale = wave % 4 == 0 ? a.Xs + (uint64_t)min(t0 + lane, a.tokens - 1) * a.spitch
+                                              : (M == 2 && lane % 2 ? a.Wus : a.Ws) + (uint64_t)(r0 / 128) * a.spitch;
+    auto fetch = [&](int step, uint8_t *to, uint32_t *to_scale) __attribute__((always_inline)) {
+        const int b = step * KG + group;
+#pragma unroll
+        for (int j = 0; j < 128; j += 32) {
+            const int in_w = j - 64, row = in_w < 0 ? j : in_w % (64 / M);
+            const uint8_t *m = in_w < 0 ? a.X + (uint64_t)(t0 + row) * a.pitch : (in_w < 64 / M ? a.W : a.Wu) + (uint64_t)(r0 + row) * a.pitch;
+            const int left = (in_w < 0 ? a.tokens - t0 : a.rows - r0) - row;
+            const uint32_t rows = (uint32_t)__builtin_amdgcn_readfirstlane(b < a.kb ? max(min(left, 32), 0) : 0);
+            dma16(tile_buffer(m, rows * (uint32_t)a.pitch), from, b * 128, to + group * 16384 + (wave % 4) * 1024 + j * 128);
+        }
+        dma4(from_scale + (min(b, a.kb - 1) & ~3), to_scale + group * 128 + (wave % 4 == 0 ? 0 : 64));
+    };
+    v4f acc[M][NR][NT];
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i / 2 / NR][i / 2 % NR][i % 2] = v4f{0, 0, 0, 0};
+    const int s0 = in * 128 + (part ^ swizzle(in)) * 16, s1 = in * 128 + ((part + 4) ^ swizzle(in)) * 16;
+    const int steps = (a.kb + KG - 1) / KG;
+    auto step = [&](int i, const uint8_t *cur, const uint32_t *scale, uint8_t *free, uint32_t *free_scale) __attribute__((always_inline)) {
+        // this step's loads and this wave's reads of the step before are done
+        __builtin_amdgcn_s_waitcnt(0x0070 | (S - 2) * kLoads);
+        barrier();
+        fetch(i + S - 1, free, free_scale);
+        const int b = i * KG + group;
+        if (b >= a.kb) return;
+        // All of the step's reads in one block that waits for them: the
+        // compiler's own would wait for every load under way as well.
+        const uint32_t base = lds_address(cur) + group * 16384, x = base + wt * 4096, w = base + 8192 + wr * NR * 2048;
+        const uint32_t sc = lds_address(scale) + group * 512;
+        v4i v[8];
+        uint32_t c[4];
+        asm volatile(
+            "ds_read_b32 %8, %16\n\tds_read_b32 %9, %16 offset:64\n\tds_read_b32 %10, %17\n\tds_read_b32 %11, %17 offset:4\n\t"
+            "ds_read_b128 %0, %12\n\tds_read_b128 %1, %13\n\tds_read_b128 %2, %14\n\tds_read_b128 %3, %15\n\t"
+            "ds_read_b128 %4, %14 offset:%18\n\tds_read_b128 %5, %15 offset:%18\n\t"
+            "ds_read_b128 %6, %12 offset:2048\n\tds_read_b128 %7, %13 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(c[0]),
+              "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3])
+            : "v"(x + s0), "v"(x + s1), "v"(w + s0), "v"(w + s1), "v"(sc + (wt * 32 + in) * 4), "v"(sc + 256), "i"(M == 2 ? 4096 : 2048)
+            : "memory");
+        auto pair = [&](int i) __attribute__((always_inline)) {
+            return v8i{v[i][0], v[i][1], v[i][2], v[i][3], v[i + 1][0], v[i + 1][1], v[i + 1][2], v[i + 1][3]};
+        };
+        const int shift = 8 * (b & 3);
+        const decltype(operand<EXACT>(v8i{}, 0)) ws[2] = {operand<EXACT>(pair(2), c[2] >> shift & 255u),
+                                                          operand<EXACT>(pair(4), c[M == 2 ? 3 : 2] >> shift & 255u)};
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+            multiply<2>(ws, operand<EXACT>(pair(t ? 6 : 0), c[t] >> shift & 255u), {&acc[0][0][t], &acc[M - 1][NR - 1][t]});
+    };
+    fetch(0, s_0, s_c0), fetch(1, s_1, s_c1), fetch(2, s_2, s_c2);
+    for (int i = 0; i < steps; i += 4) {
+        step(i, s_0, s_c0, s_3, s_c3);
+        if (i + 1 < steps) step(i + 1, s_1, s_c1, s_0, s_c0);
+        if (i + 2 < steps) step(i + 2, s_2, s_c2, s_1, s_c1);
+        if (i + 3 < steps) step(i + 3, s_3, s_c3, s_2, s_c2);
+    }
+    if constexpr (KG > 1) {
+        __builtin_amdgcn_s_waitcnt(0x0070);  // no load is under way into what the sums take
+        barrier();
+        v4f *sums = (v4f *)s_0;
+        if (group)
+#pragma unroll
+            for (int i = 0; i < 4; i++) sums[((group - 1) * 4 + wave % 4) * 256 + i * 64 + lane] = acc[i / 2 / NR][i / 2 % NR][i % 2];
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        barrier();
+        if (group) return;
+#pragma unroll
+        for (int g = 1; g < KG; g++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const v4f o = sums[((g - 1) * 4 + wave) * 256 + i * 64 + lane];
+                v4f &mine = acc[i / 2 / NR][i / 2 % NR][i % 2];
+#pragma unroll
+                for (int j = 0; j < 4; j++) mine[j] = mine[j] + o[j];
+            }
+    }
+    store_tile<OUT>(a, t0 + wt * 32, r0 + wr * NR * 16, acc, r0 + 64 / M <= a.rows && vec, in, part);
+}
+
+// A tile's size, the workgroups of it that a CU holds (the first two rows: at
+// most; these kernels take one tile a workgroup), what a step of one of them
+// and of all of them takes and what a round over the GPU takes beside its
+// steps, in us (one MI355X). From whole calls of 20 and 48 steps, 8-bit sums
+// (f32 sums): 64 x 64 deep 8.0 and 13.4 (10.8, 19.9), two a CU 11.0 and 21.8
+// (17.5, 34.5); 64 x 64 three a CU 17.7 and 35.6 (25.6, 51.4), 2.5 rounds 46.4
+// and 105.8 (74.9, 176.6); 128 x 128 one 20.7 and 46.0 (31.3, 65.1), 2.5 rounds
+// 68 and 146 (102.6, 226); 256 x 128 25.5 and 52.3 (42, 82), three rounds 68
+// and 149 (115, 244); 256 x 256 37.3 and 71.8 (62, 127), two rounds 68 and 145
+// (125, 270).
 struct Shape {
     int tokens, rows, resident;
-    float one, all;
+    float one, all, round;
 };
-// Measured from whole calls of 20 and 48 steps. 8-bit: 64 x 64 10.4 us alone,
-// 46.4 for 2.5 rounds of four a CU; 128 x 128 18.0 and 68.0 for 2.5 rounds of
-// two; 256 x 128 25.5; 256 x 256 37.3, 210 for five rounds. bf16 values: 14.6 and
-// 74.9; 28.0 and 485 for ten rounds; 42; 62 and 395 for five rounds.
-constexpr Shape kShapes[2][4] = {{{64, 64, 4, 0.5f, 0.9f}, {128, 128, 2, 0.9f, 1.25f}, {256, 128, 1, 1.27f, 1.27f}, {256, 256, 1, 1.8f, 1.8f}},
-                                 {{64, 64, 4, 0.7f, 1.45f}, {128, 128, 2, 1.45f, 2.2f}, {256, 128, 1, 2.2f, 2.2f}, {256, 256, 1, 3.5f, 3.5f}}};
+constexpr int kShapeCount = 6;
+constexpr Shape kShapes[2][kShapeCount] = {
+    {{64, 64, 1, 0.19f, 0.19f, 4.2f}, {64, 64, 2, 0.36f, 0.36f, 3.8f}, {64, 64, 4, 0.35f, 0.85f, 3.0f},
+     {128, 128, 2, 0.75f, 0.97f, 6.0f}, {256, 128, 1, 0.96f, 0.96f, 4.5f}, {256, 256, 1, 1.35f, 1.35f, 9.0f}},
+    {{64, 64, 1, 0.33f, 0.33f, 4.3f}, {64, 64, 2, 0.60f, 0.60f, 5.4f}, {64, 64, 4, 0.50f, 1.42f, 3.0f},
+     {128, 128, 2, 1.15f, 1.80f, 7.0f}, {256, 128, 1, 1.50f, 1.50f, 11.0f}, {256, 256, 1, 2.50f, 2.50f, 11.0f}}};
 
 template <int BT, int BR, int WT, int WR, bool EXACT, Out OUT>
 void tiles(sm_ctx *ctx, const Product &a, int cus, int resident) {
@@ -629,35 +747,50 @@ int compute_units(sm_ctx *ctx) {
     return hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, ctx->device) == hipSuccess && cus > 0 ? cus : 256;
 }
 
-// Up to 16 tokens, and where 16-row workgroups of 64 tokens are fewer than the
-// GPU's CUs, the waves that share out the columns (2560 x 2560, 64 tokens: 8.9
-// us against 10.6 in tiles; 2560 x 640, 256 tokens: 9.0 against 10.8; 2560 x
-// 10240, 32 tokens: 13.8 against 10.7).
-bool takes_few(const Product &a) {
-    return a.tokens <= 16 || (int64_t)((a.rows + 15) / 16) * ((a.tokens + 63) / 64) <= 200;
+// Few tokens go to the waves that share out the columns. 8-bit sums: up to 4
+// tokens, and up to 32 while sixteens of tokens times rows stay under 5,120
+// (2560 columns, 2560 rows, 32 tokens 6.4 us against 8.0 in tiles, 48 tokens 9.0
+// against 8.0; 10240 rows, 1 token 6.8 against 7.8, 8 tokens 8.4 against 7.8).
+// f32 sums: up to 16 tokens, and while workgroups of 64 tokens and 16 rows are
+// fewer than the CUs (2560 rows, 64 tokens 9.5 against 10.8, 100 tokens 14.1
+// against 10.8; 10240 rows, 16 tokens 9.8 against 10.5, 32 tokens 14.1 against
+// 10.7).
+bool takes_few(const Product &a, bool exact) {
+    const int64_t sixteens = (a.tokens + 15) / 16;
+    if (exact) return a.tokens <= 16 || (int64_t)((a.rows + 15) / 16) * ((sixteens + 3) / 4) <= 200;
+    return a.tokens <= 4 || (a.tokens <= 32 && sixteens * a.rows <= 5120);
 }
-// Else the tile whose rounds over the GPU take least: its index in kShapes and
-// the time of a step of all of them, in us.
+// Else the tile whose rounds over the GPU take least: its index in kShapes, and
+// that time in us.
 int best_shape(const Product &a, bool exact, int m, int cus, float *us) {
-    int best = 0;
-    for (int i = 0; i < 4; i++) {
+    int best = -1;
+    for (int i = 0; i < kShapeCount; i++) {
         const Shape &s = kShapes[exact][i];
         const int64_t n = (int64_t)((a.tokens + s.tokens - 1) / s.tokens) * ((a.rows + s.rows / m - 1) / (s.rows / m));
-        const int64_t round = (int64_t)cus * s.resident, over = (n % round + cus - 1) / cus;  // workgroups of a CU in the last round
-        const float last = over == 0 ? 0.0f : s.resident == 1 ? s.one : s.one + (s.all - s.one) * (over - 1) / (s.resident - 1);
-        const float time = n / round * s.all + last;
-        if (i == 0 || time < *us) *us = time, best = i;
+        const int64_t slots = (int64_t)cus * s.resident, over = (n % slots + cus - 1) / cus;  // workgroups of a CU in the last round
+        if (i < 2 && n > slots) continue;
+        const float last = s.resident == 1 ? s.one : s.one + (s.all - s.one) * (over - 1) / (s.resident - 1);
+        const float time = n / slots * (s.all * a.kb + s.round) + (over ? last * a.kb + s.round : 0.0f);
+        if (best < 0 || time < *us) *us = time, best = i;
     }
     return best;
 }
+template <int KG, bool EXACT, Out OUT>
+void deep(sm_ctx *ctx, const Product &a) {
+    constexpr int kRows = OUT == kHidden ? 32 : 64;
+    const Tiles t = {(a.tokens + 63) / 64, (a.rows + kRows - 1) / kRows, 0};
+    k_f8_deep<KG, 4, EXACT, OUT><<<(t.tokens * t.rows + 7) / 8 * 8, 256 * KG, 0, ctx->stream>>>(a, t, aligned(a, OUT == kBf16 ? 8 : 4));
+}
 template <bool EXACT, Out OUT>
 void multiply_by_size(sm_ctx *ctx, const Product &a, int cus) {
-    if (takes_few(a)) return few<EXACT, OUT>(ctx, a);
+    if (takes_few(a, EXACT)) return few<EXACT, OUT>(ctx, a);
     float us = 0.0f;
     const int best = best_shape(a, EXACT, OUT == kHidden ? 2 : 1, cus, &us), resident = kShapes[EXACT][best].resident;
-    if (best == 0) tiles<64, 64, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
-    else if (best == 1) tiles<128, 128, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
-    else if (best == 2) tiles<256, 128, 4, 2, EXACT, OUT>(ctx, a, cus, resident);
+    if (best == 0) deep<2, EXACT, OUT>(ctx, a);
+    else if (best == 1) deep<1, EXACT, OUT>(ctx, a);
+    else if (best == 2) tiles<64, 64, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
+    else if (best == 3) tiles<128, 128, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
+    else if (best == 4) tiles<256, 128, 4, 2, EXACT, OUT>(ctx, a, cus, resident);
     else tiles<256, 256, 2, 4, EXACT, OUT>(ctx, a, cus, resident);
 }
 
@@ -670,11 +803,11 @@ int gate_up(sm_ctx *ctx, Product &a, uint8_t *codes, uint8_t *scales, void *work
     const int cus = compute_units(ctx);
     const F8Layout L = f8_layout(a.tokens, a.rows, 1);
     a.codes = codes, a.scales = scales, a.codes_pitch = L.pitch, a.scales_pitch = L.spitch;
-    if (!takes_few(a)) {
+    if (!takes_few(a, true)) {
         auto rounds = [&](int tokens) { return ((int64_t)((a.tokens + tokens - 1) / tokens) * (int64_t)(L.pitch / 128) + cus - 1) / cus; };
         float apart = 0.0f;
         best_shape(a, true, 2, cus, &apart);
-        apart = apart * a.kb + 3.0f + 5.0f * a.tokens * a.rows / 4e6f;
+        apart += 3.0f + 5.0f * a.tokens * a.rows / 4e6f;  // and the conversion
         const float wide = rounds(256) * (1.6f * a.kb + 14.0f), narrow = rounds(128) * (1.0f * a.kb + 6.0f);
         if (wide < apart && wide < narrow) return tiles<256, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
         if (narrow < apart) return tiles<128, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
