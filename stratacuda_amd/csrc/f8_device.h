@@ -38,11 +38,41 @@ __device__ __forceinline__ uint32_t codes4(const V &v, float inverse) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(s[2], s[3], w, true);
 }
 
+// The lane's value combined with that of the lanes 1, 2, 4, 8 and 16 (and 32)
+// away, by data-parallel moves: two swaps in quads, then mirrors of 8 and 16,
+// which give any lane of the other half since the halves are equal by then.
+template <int CTRL>
+__device__ __forceinline__ float moved(float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double moved(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kMirror8 = 0x141, kMirror16 = 0x140;
+__device__ __forceinline__ float max_of_16(float v) {
+    v = fmaxf(v, moved<kSwap1>(v));
+    v = fmaxf(v, moved<kSwap2>(v));
+    v = fmaxf(v, moved<kMirror8>(v));
+    return fmaxf(v, moved<kMirror16>(v));
+}
 // Largest of the 32 lanes of each half of a wave, in all of them.
 __device__ __forceinline__ float half_wave_max(float v) {
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) v = fmaxf(v, __shfl_xor(v, d, 64));
-    return v;
+    v = max_of_16(v);
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+// Sum over a wave, in all lanes.
+__device__ __forceinline__ double wave_sum(double v) {
+    v += moved<kSwap1>(v);
+    v += moved<kSwap2>(v);
+    v += moved<kMirror8>(v);
+    v += moved<kMirror16>(v);
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
 }
 
 __device__ __forceinline__ float bf16_value(uint32_t bits16) { return __uint_as_float(bits16 << 16); }
