@@ -302,9 +302,9 @@ int sm_f8_project(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int co
  * silu(g) = g / (1 + exp(-g)); X as in sm_f8_project, Wg and Wu f8 matrices
  * [ff x cols] of block_rows 128 (they may be one buffer). The sums are those
  * of sm_f8_project's type f32, or its bf16 type's before their rounding where
- * that is faster; the scales are those of the f32 sums either way (where more
- * than eight columns of a block lie within 2^-11 of its largest, of the first
- * eight of those). The workspace holds
+ * that is faster; the scales are those of the f32 sums then too, unless those
+ * are off by more than 2^-10 of a block's largest value (where more than eight
+ * columns lie within 2^-9 of it, the first eight decide). The workspace holds
  * sm_f8_gate_up_workspace(...) bytes; a call leaves nothing in it that a
  * later call needs. */
 int sm_f8_gate_up_workspace(int tokens, int ff, uint64_t *bytes);

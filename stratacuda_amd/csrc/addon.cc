@@ -421,6 +421,86 @@ napi_value MoeDispatch(napi_env env, napi_callback_info info) {
         return nullptr;
     return undefined(env);
 }
+// f8Bytes(rows, cols, blockRows): [bytes of the codes, bytes of the scales]
+napi_value F8Bytes(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(3)) return nullptr;
+    int rows = a.i32(0), cols = a.i32(1), block = a.i32(2);
+    if (!a.ok) return nullptr;
+    uint64_t codes = 0, scales = 0;
+    if (fail(env, nullptr, sm_f8_bytes(rows, cols, block, &codes, &scales))) return nullptr;
+    napi_value pair;
+    napi_create_array_with_length(env, 2, &pair);
+    napi_set_element(env, pair, 0, number(env, (double)codes));
+    napi_set_element(env, pair, 1, number(env, (double)scales));
+    return pair;
+}
+// f8Quantize(ctx, X, type, rows, cols, blockRows, codes, scales)
+napi_value F8Quantize(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(8)) return nullptr;
+    sm_ctx *ctx = a.ctx(0);
+    uint64_t X = a.u64(1);
+    int type = a.i32(2), rows = a.i32(3), cols = a.i32(4), block = a.i32(5);
+    uint64_t codes = a.u64(6), scales = a.u64(7);
+    if (!a.ok || fail(env, ctx, sm_f8_quantize(ctx, X, type, rows, cols, block, codes, scales))) return nullptr;
+    return undefined(env);
+}
+// f8Norm(ctx, X, type, R, gamma, eps, rows, cols, H, codes, scales)
+napi_value F8Norm(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(11)) return nullptr;
+    sm_ctx *ctx = a.ctx(0);
+    uint64_t X = a.u64(1);
+    int type = a.i32(2);
+    uint64_t R = a.u64(3), gamma = a.u64(4);
+    const float eps = (float)a.num(5);
+    int rows = a.i32(6), cols = a.i32(7);
+    uint64_t H = a.u64(8), codes = a.u64(9), scales = a.u64(10);
+    if (!a.ok || fail(env, ctx, sm_f8_norm(ctx, X, type, R, gamma, eps, rows, cols, H, codes, scales))) return nullptr;
+    return undefined(env);
+}
+// f8Project(ctx, X, xScales, tokens, cols, W, wScales, rows, R, Y, type, stride, offset)
+napi_value F8Project(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(13)) return nullptr;
+    sm_ctx *ctx = a.ctx(0);
+    uint64_t X = a.u64(1), xs = a.u64(2);
+    int tokens = a.i32(3), cols = a.i32(4);
+    uint64_t W = a.u64(5), ws = a.u64(6);
+    int rows = a.i32(7);
+    uint64_t R = a.u64(8), Y = a.u64(9);
+    int type = a.i32(10);
+    uint64_t stride = a.u64(11), offset = a.u64(12);
+    if (!a.ok || fail(env, ctx, sm_f8_project(ctx, X, xs, tokens, cols, W, ws, rows, R, Y, type, (int64_t)stride,
+                                              (int64_t)offset)))
+        return nullptr;
+    return undefined(env);
+}
+// f8GateUpWorkspace(tokens, ff)
+napi_value F8GateUpWorkspace(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(2)) return nullptr;
+    int tokens = a.i32(0), ff = a.i32(1);
+    if (!a.ok) return nullptr;
+    uint64_t n = 0;
+    if (fail(env, nullptr, sm_f8_gate_up_workspace(tokens, ff, &n))) return nullptr;
+    return number(env, (double)n);
+}
+// f8GateUp(ctx, X, xScales, tokens, cols, Wg, wgScales, Wu, wuScales, ff, codes, scales, workspace, workspaceBytes)
+napi_value F8GateUp(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(14)) return nullptr;
+    sm_ctx *ctx = a.ctx(0);
+    uint64_t X = a.u64(1), xs = a.u64(2);
+    int tokens = a.i32(3), cols = a.i32(4);
+    uint64_t Wg = a.u64(5), wgs = a.u64(6), Wu = a.u64(7), wus = a.u64(8);
+    int ff = a.i32(9);
+    uint64_t codes = a.u64(10), scales = a.u64(11), ws = a.u64(12), wsb = a.u64(13);
+    if (!a.ok || fail(env, ctx, sm_f8_gate_up(ctx, X, xs, tokens, cols, Wg, wgs, Wu, wus, ff, codes, scales, ws, wsb)))
+        return nullptr;
+    return undefined(env);
+}
 // synthNormal(ctx, dst, offsetBytes, n, seed, stream, sigma) and
 // synthUniformPm(ctx, dst, offsetBytes, n, seed, stream, amp)
 napi_value SynthNormal(napi_env env, napi_callback_info info) {
@@ -561,6 +641,12 @@ napi_value ModuleInit(napi_env env, napi_value exports) {
                {"moeBlock", MoeBlock},
                {"moeRoute", MoeRoute},
                {"moeDispatch", MoeDispatch},
+               {"f8Bytes", F8Bytes},
+               {"f8Quantize", F8Quantize},
+               {"f8Norm", F8Norm},
+               {"f8Project", F8Project},
+               {"f8GateUpWorkspace", F8GateUpWorkspace},
+               {"f8GateUp", F8GateUp},
                {"synthNormal", SynthNormal},
                {"synthUniformPm", SynthUniformPm},
                {"synthBlobs", SynthBlobs},

@@ -107,6 +107,12 @@ function parseSignature(sig) {
 }
 const f32bits = new Float32Array(1), u32bits = new Uint32Array(f32bits.buffer);
 
+function f8Type(type) {
+    const at = ['f32', 'bf16'].indexOf(type || 'f32');
+    if (at < 0) throw new RangeError('type must be f32 or bf16');
+    return at;
+}
+
 export class HipBackend {
     // create({device, addon}): addon defaults to the built strata_addon.node;
     // tests pass a stand-in with the same functions.
@@ -320,6 +326,60 @@ export class HipBackend {
         this.addon.moeDispatch(this.ctx, this.owned(a.ids, 'ids'), a.tokens, a.topK, a.experts,
             this.owned(a.offsets, 'offsets'), this.owned(a.rows, 'rows'), this.owned(a.parts, 'parts'),
             this.owned(a.where, 'where'), this.owned(a.workspace, 'workspace'), a.workspace.byteLength);
+        this.dispatches++;
+    }
+    // -------------------------------- 8-bit floating-point matrices (kind 'hip')
+    // An f8 matrix is {codes, scales, rows, cols, blockRows}: e4m3 bytes and a
+    // power of two for each 128 columns of blockRows rows (1: activations,
+    // 128: weights); include/strata_mi355x.h has the layout. f8Matrix allocates
+    // one; free its two buffers as any other.
+    f8Matrix(rows, cols, blockRows) {
+        blockRows = blockRows || 1;
+        const bytes = this.addon.f8Bytes(rows, cols, blockRows), plain = {zero: false};
+        return {codes: this.allocBytes(bytes[0], 'u32', plain), scales: this.allocBytes(bytes[1], 'u32', plain), rows, cols,
+            blockRows};
+    }
+    f8Owned(m, blockRows, what) {
+        if (!m || m.blockRows !== blockRows) throw Error('Invalid HIP f8 ' + what);
+        return [this.owned(m.codes, what), this.owned(m.scales, what)];
+    }
+    // X [out.rows x out.cols], f32 or (type 'bf16') bf16, into `out`.
+    f8Quantize(X, out, type) {
+        this.assertAlive();
+        const o = this.f8Owned(out, out && out.blockRows, 'output');
+        this.addon.f8Quantize(this.ctx, this.owned(X, 'X'), f8Type(type), out.rows, out.cols, out.blockRows, o[0], o[1]);
+        this.dispatches++;
+    }
+    // H = X + R, then RMSNorm(H; gamma, eps) into a.out. R and H may be left out; H may be R, or X where that is f32.
+    f8Norm(a) {
+        this.assertAlive();
+        const o = this.f8Owned(a.out, 1, 'output');
+        this.addon.f8Norm(this.ctx, this.owned(a.X, 'X'), f8Type(a.type), a.R ? this.owned(a.R, 'R') : 0,
+            this.owned(a.gamma, 'gamma'), a.eps, a.out.rows, a.out.cols, a.H ? this.owned(a.H, 'H') : 0, o[0], o[1]);
+        this.dispatches++;
+    }
+    // Y[t * stride + offset + r] = R[the same] + X[t] . W[r]; R (it may be Y) needs type 'f32'.
+    f8Project(a) {
+        this.assertAlive();
+        const x = this.f8Owned(a.X, 1, 'X'), w = this.f8Owned(a.W, 128, 'W');
+        if (a.X.cols !== a.W.cols) throw new RangeError('f8 project: X and W have different columns');
+        const stride = requireInteger(a.stride === undefined ? a.W.rows : a.stride, 'output stride', 1, Number.MAX_SAFE_INTEGER);
+        const offset = requireInteger(a.offset || 0, 'output offset', 0, Number.MAX_SAFE_INTEGER);
+        this.addon.f8Project(this.ctx, x[0], x[1], a.X.rows, a.X.cols, w[0], w[1], a.W.rows, a.R ? this.owned(a.R, 'R') : 0,
+            this.owned(a.Y, 'Y'), f8Type(a.type), stride, offset);
+        this.dispatches++;
+    }
+    f8GateUpWorkspaceBytes(tokens, ff) { return this.addon.f8GateUpWorkspace(tokens, ff); }
+    // silu(X . Wg) * (X . Wu) into a.out.
+    f8GateUp(a) {
+        this.assertAlive();
+        const x = this.f8Owned(a.X, 1, 'X'), g = this.f8Owned(a.Wg, 128, 'Wg'), u = this.f8Owned(a.Wu, 128, 'Wu');
+        const o = this.f8Owned(a.out, 1, 'output');
+        if (a.X.cols !== a.Wg.cols || a.X.cols !== a.Wu.cols || a.Wg.rows !== a.Wu.rows || a.out.rows !== a.X.rows ||
+            a.out.cols !== a.Wg.rows)
+            throw new RangeError('f8 gate_up: shapes disagree');
+        this.addon.f8GateUp(this.ctx, x[0], x[1], a.X.rows, a.X.cols, g[0], g[1], u[0], u[1], a.Wg.rows, o[0], o[1],
+            this.owned(a.workspace, 'workspace'), a.workspace.byteLength);
         this.dispatches++;
     }
     // Seeded synthetic data, bit-identical to the CPU oracle's generator.

@@ -129,14 +129,18 @@ def matrix(rng, rows, cols, block):
     return codes, scales, values(codes, scales, block)[:, :cols]
 
 
-def ordinary(rng, rows, cols, block):
-    """The same of normal values, some columns larger."""
-    x = rng.normal(0, 1, (rows, cols)) * np.exp(rng.normal(0, 0.8, cols))
-    v, scales = quantize(x, block)
+def of_values(v, scales, block, cols):
+    """(code bytes, scale bytes, the matrix) of code values [rows, pitch]."""
     order = np.argsort(CODES[:127])
     at = np.searchsorted(CODES[:127][order], np.abs(v))
     codes = (order[at] | np.where(np.signbit(v), 128, 0)).astype(np.uint8)
     return codes, scales, values(codes, scales, block)[:, :cols]
+
+
+def ordinary(rng, rows, cols, block):
+    """The same as matrix() of normal values, some columns larger."""
+    x = rng.normal(0, 1, (rows, cols)) * np.exp(rng.normal(0, 0.8, cols))
+    return of_values(*quantize(x, block), block, cols)
 
 
 def silu(g):
