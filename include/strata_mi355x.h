@@ -287,8 +287,9 @@ int sm_f8_norm(sm_ctx *ctx, uint64_t X, int type, uint64_t R, uint64_t gamma, fl
 /* Y[t * stride + offset + r] = R[the same] + X[t, :] . W[r, :], t < tokens,
  * r < rows; X an f8 matrix [tokens x cols] of block_rows 1, W one
  * [rows x cols] of block_rows 128.
- * type f32: Y is f32, the sums are f32's (the codes' products are exact). R
- *   is f32, laid out like Y, 0 for none; it may be Y.
+ * type f32: Y is f32, the sums are f32's (the codes' products are exact; code
+ *   times scale below 2^-126 may count as 0). R is f32, laid out like Y, 0 for
+ *   none; it may be Y.
  * type bf16: Y is bf16 and R must be 0; the sums are rounded once to bf16 and
  *   their products may be cut off 2^13 below the largest of eight neighbours
  *   (about 1e-5 of the sum), for up to twice the rate.
