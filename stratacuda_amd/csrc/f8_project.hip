@@ -27,11 +27,6 @@ typedef float v2f __attribute__((ext_vector_type(2)));
 
 enum Out { kF32, kBf16, kHidden, kCodes };  // kHidden, kCodes: silu(gate) * up in f32, in 8 bits
 
-// 32 of a row's 128 codes: lane l holds row l % 16, columns 32 (l / 16) on.
-__device__ __forceinline__ v8i load_frag(const uint8_t *p) {
-    const v4i a = *(const v4i *)p, b = *(const v4i *)(p + 16);
-    return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
 // An operand of one block of 128 columns: the codes with their scale, or
 // (EXACT) their values in bf16, 32 columns an instruction. Which 32 columns
 // lie in which instruction and lane is one order for both matrices.
@@ -141,9 +136,6 @@ __device__ __forceinline__ void store_tile(const Product &a, int first_token, in
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             h[r] = acc[0][r][t];
-            if constexpr (OUT == kHidden)
-#pragma unroll
-                for (int i = 0; i < 4; i++) h[r][i] = silu_times(h[r][i], acc[M - 1][r][t][i]);
         }
         if (!whole) {
             if (token + in < a.tokens)
@@ -192,66 +184,12 @@ __device__ __forceinline__ void store_tile(const Product &a, int first_token, in
     }
 }
 
-// -------------------------------------------------------- few tokens
-// A workgroup's eight waves share 16 weight rows and 16 TT tokens and take
-// the blocks of 128 columns in turn, codes straight from memory into the
-// matrix instruction's registers; their sums meet in LDS, added in the
-// waves' order.
-constexpr int kWaves = 8;
-
-// Whether every n-th output of a token starts n aligned ones (buffers start aligned).
-bool aligned(const Product &a, int n) { return a.stride % n == 0 && a.offset % n == 0; }
-
-template <int TT, bool EXACT, Out OUT>
-__global__ void __launch_bounds__(64 * kWaves) k_f8_few(Product a, bool vec) {
-    constexpr int M = OUT == kHidden ? 2 : 1;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, in = lane % 16, part = lane / 16;
-    const int r0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * TT;
-    __shared__ v4f s_sum[kWaves][M * TT][64];
-    const int wr = min(r0 + in, a.rows - 1);
-    const uint8_t *w[2] = {a.W + wr * a.pitch + 32 * part, M == 2 ? a.Wu + wr * a.pitch + 32 * part : nullptr};
-    const uint8_t *ws[2] = {a.Ws + (uint64_t)(r0 / 128) * a.spitch, M == 2 ? a.Wus + (uint64_t)(r0 / 128) * a.spitch : nullptr};
-    const uint8_t *x[TT], *xs[TT];
-    v4f acc[M][TT];
-#pragma unroll
-    for (int t = 0; t < TT; t++) {
-        const uint64_t row = min(t0 + 16 * t + in, a.tokens - 1);
-        x[t] = a.X + row * a.pitch + 32 * part;
-        xs[t] = a.Xs + row * a.spitch;
-#pragma unroll
-        for (int m = 0; m < M; m++) acc[m][t] = v4f{0, 0, 0, 0};
-    }
-    for (int b = wave; b < a.kb; b += kWaves) {
-        decltype(operand<EXACT>(v8i{}, 0)) wf[M];
-#pragma unroll
-        for (int m = 0; m < M; m++) wf[m] = operand<EXACT>(load_frag(w[m] + (uint64_t)b * 128), ws[m][b]);
-#pragma unroll
-        for (int t = 0; t < TT; t++) {
-            const auto xf = operand<EXACT>(load_frag(x[t] + (uint64_t)b * 128), xs[t][b]);
-            if constexpr (M == 2) multiply(wf, xf, {&acc[0][t], &acc[M - 1][t]});
-            else multiply(wf, xf, {&acc[0][t]});
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < M; m++)
-#pragma unroll
-        for (int t = 0; t < TT; t++) s_sum[wave][m * TT + t][lane] = acc[m][t];
-    __syncthreads();
-    if (wave >= TT) return;
-    v4f v[M];
-#pragma unroll
-    for (int m = 0; m < M; m++) {
-        v[m] = s_sum[0][m * TT + wave][lane];
-        for (int k = 1; k < kWaves; k++) {
-            const v4f o = s_sum[k][m * TT + wave][lane];
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[m][i] = v[m][i] + o[i];
-        }
-    }
+// The sums of 16 rows from r0 on for one token a lane group.
+template <Out OUT, int M>
+__device__ __forceinline__ void store_few(const Product &a, v4f (&v)[M], int t, int r0, int part, bool vec) {
     if constexpr (OUT == kHidden)
 #pragma unroll
         for (int i = 0; i < 4; i++) v[0][i] = silu_times(v[0][i], v[M - 1][i]);
-    const int t = t0 + 16 * wave + in;
     if (t >= a.tokens) return;
     const int64_t at = t * a.stride + a.offset + r0 + 4 * part;
     if (vec && r0 + 16 <= a.rows) {
@@ -264,15 +202,8 @@ __global__ void __launch_bounds__(64 * kWaves) k_f8_few(Product a, bool vec) {
     }
 }
 
-template <bool EXACT, Out OUT>
-void few(sm_ctx *ctx, const Product &a) {
-    const int tiles = (a.tokens + 15) / 16, tt = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1;
-    const bool vec = aligned(a, 4);
-    const dim3 grid((a.rows + 15) / 16, (tiles + tt - 1) / tt);
-    if (tt == 4) k_f8_few<4, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a, vec);
-    else if (tt == 2) k_f8_few<2, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a, vec);
-    else k_f8_few<1, EXACT, OUT><<<grid, 64 * kWaves, 0, ctx->stream>>>(a, vec);
-}
+// Whether every n-th output of a token starts n aligned ones (buffers start aligned).
+bool aligned(const Product &a, int n) { return a.stride % n == 0 && a.offset % n == 0; }
 
 // ------------------------------------------------------ many tokens: tiles
 // A workgroup of WT x WR waves makes BT tokens x BR weight rows (a gated pair:
@@ -344,7 +275,7 @@ struct Tiles {
 
 template <int BT, int BR, int WT, int WR, bool EXACT, Out OUT>
 __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles, bool vec) {
-    constexpr int kThreads = 64 * WT * WR, NT = BT / WT / 16, M = OUT >= kHidden ? 2 : 1, NR = BR / WR / 16 / M;
+    constexpr int kThreads = 64 * WT * WR, NT = BT / WT / 16, M = OUT == kCodes ? 2 : 1, NR = BR / WR / 16 / M;
     constexpr int kStage = (BT + BR) * 128, kRows = kThreads / 8;  // rows that the threads bring at a time
     static_assert(BT % kRows == 0 && BR / M % kRows == 0 && kRows % 8 == 0 && BT % 64 == 0 && BT / 64 < WT * WR && NT >= 2, "");
     // two variables, so that reads of one need not wait for the DMA into the other
@@ -609,134 +540,164 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
     }
 }
 
-// ------------------------------------- some tokens: few tiles, one a workgroup
-// Where 64 x 64 tiles leave CUs idle, a step's latency is the time: four steps
-// in flight (S - 1 ahead, waited for by their number), and KG groups of four
-// waves that take a block of 128 columns each at a time, whose sums meet in LDS
-// in their order. 2560 columns to 2560 rows, 256 tokens, to bf16: 11.0 us in
-// the persistent tiles, 8.4 here.
-template <int KG, int S, bool EXACT, Out OUT>
-__global__ void __launch_bounds__(256 * KG) k_f8_deep(Product a, Tiles tiles, bool vec) {
-    constexpr int M = OUT >= kHidden ? 2 : 1, NT = 2, NR = 2 / M, kLoads = 5;
-    static_assert(S == 4, "");
-    __shared__ __attribute__((aligned(16))) uint8_t s_0[KG * 16384], s_1[KG * 16384], s_2[KG * 16384], s_3[KG * 16384];
-    __shared__ uint32_t s_c0[KG * 128], s_c1[KG * 128], s_c2[KG * 128], s_c3[KG * 128];
-    const int lane = threadIdx.x % 64, in = lane % 16, part = lane / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), group = wave / 4, wt = wave / 2 % 2, wr = wave % 2;
-    const int xcd = blockIdx.x % 8, n = tiles.tokens * tiles.rows;
-    const int at = xcd * (n / 8) + min(xcd, n % 8) + blockIdx.x / 8, end = (xcd + 1) * (n / 8) + min(xcd + 1, n % 8);
-    if (at >= end) return;
-    int t0, r0;
-    tiles.locate(at, t0, r0);
-    t0 *= 64, r0 *= 64 / M;
+// ------------------------------------------------------ few tokens: streams
+// A workgroup's W waves share 16 RR weight rows (of a gated pair: of both
+// matrices) and 16 TT tokens and take the blocks of 128 columns in turn. A wave
+// brings its block into its own part of LDS by DMA, eight lanes to a row's 128
+// bytes, reads it into the matrix instructions' order, and has the next one under
+// way while it multiplies; it waits for no other wave. Their sums meet in LDS,
+// added in the waves' order. Bound by what L2 gives (16 TB/s) and, for one token,
+// by a step's latency, which many small workgroups on a CU hide better than two or
+// three blocks a wave under way (4 waves, 32 tokens, 2560 columns to 10,240 rows:
+// 8.2 us with two, 7.6 with one; 32 tokens, 6144 to 2560 7.2 and 6.6, with eight
+// waves 6.1). Fragments straight from memory, where every lane of an instruction
+// is in another line, take 11.8.
+struct Pair {
+    v4i v[4];
+};
+// Two fragments of 16 rows from LDS: lane part's chunks {part, part + 4} of each.
+template <int F, int G>
+__device__ __forceinline__ Pair read_pair(uint32_t first, uint32_t second) {
+    Pair p;
+    asm volatile(
+        "ds_read_b128 %0, %4 offset:%6\n\tds_read_b128 %1, %5 offset:%6\n\t"
+        "ds_read_b128 %2, %4 offset:%7\n\tds_read_b128 %3, %5 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(p.v[0]), "=&v"(p.v[1]), "=&v"(p.v[2]), "=&v"(p.v[3])
+        : "v"(first), "v"(second), "i"(2048 * F), "i"(2048 * G)
+        : "memory");
+    return p;
+}
+__device__ __forceinline__ v8i join(v4i a, v4i b) { return v8i{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
 
-    const int thread = threadIdx.x % 256;
-    const uint32_t from = thread / 8 * (uint32_t)a.pitch + ((thread ^ swizzle(thread / 8)) & 7) * 16;
-    const uint8_t *from_scale = wave % 4 == 0 ? a.Xs + (uint64_t)min(t0 + lane, a.tokens - 1) * a.spitch
-                                              : (M == 2 && lane % 2 ? a.Wus : a.Ws) + (uint64_t)(r0 / 128) * a.spitch;
-    auto fetch = [&](int step, uint8_t *to, uint32_t *to_scale) __attribute__((always_inline)) {
-        const int b = step * KG + group;
-#pragma unroll
-        for (int j = 0; j < 128; j += 32) {
-            const int in_w = j - 64, row = in_w < 0 ? j : in_w % (64 / M);
-            const uint8_t *m = in_w < 0 ? a.X + (uint64_t)(t0 + row) * a.pitch : (in_w < 64 / M ? a.W : a.Wu) + (uint64_t)(r0 + row) * a.pitch;
-            const int left = (in_w < 0 ? a.tokens - t0 : a.rows - r0) - row;
-            const uint32_t rows = (uint32_t)__builtin_amdgcn_readfirstlane(b < a.kb ? max(min(left, 32), 0) : 0);
-            dma16(tile_buffer(m, rows * (uint32_t)a.pitch), from, b * 128, to + group * 16384 + (wave % 4) * 1024 + j * 128);
-        }
-        dma4(from_scale + (min(b, a.kb - 1) & ~3), to_scale + group * 128 + (wave % 4 == 0 ? 0 : 64));
-    };
-    v4f acc[M][NR][NT];
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[i / 2 / NR][i / 2 % NR][i % 2] = v4f{0, 0, 0, 0};
-    const int s0 = in * 128 + (part ^ swizzle(in)) * 16, s1 = in * 128 + ((part + 4) ^ swizzle(in)) * 16;
-    const int steps = (a.kb + KG - 1) / KG;
-    auto step = [&](int i, const uint8_t *cur, const uint32_t *scale, uint8_t *free, uint32_t *free_scale) __attribute__((always_inline)) {
-        // this step's loads and this wave's reads of the step before are done
-        __builtin_amdgcn_s_waitcnt(0x0070 | (S - 2) * kLoads);
-        barrier();
-        fetch(i + S - 1, free, free_scale);
-        const int b = i * KG + group;
+template <int W, int RR, int TT, bool EXACT, Out OUT>
+__global__ void __launch_bounds__(64 * W) k_f8_stream(Product a, int row_tiles, int token_tiles, bool vec) {
+    constexpr int M = OUT == kHidden ? 2 : 1, kW = M * RR, kFrags = kW + TT, kStage = kFrags * 2048 + 512;
+    constexpr int kSums = kW * TT * 1024, kPart = kStage > kSums ? kStage : kSums;
+    static_assert(kFrags <= 8 && TT <= 4, "");
+    __shared__ __attribute__((aligned(16))) uint8_t s_lds[W * kPart];
+    const int lane = threadIdx.x % 64, in = lane % 16, part = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    // An XCD's workgroups take tiles that follow each other, all tokens of a weight tile first: its L2 holds it.
+    const int xcd = blockIdx.x % 8, n = row_tiles * token_tiles, at = xcd * (n / 8) + min(xcd, n % 8) + blockIdx.x / 8;
+    if ((int)(blockIdx.x / 8) >= n / 8 + (xcd < n % 8)) return;
+    const int r0 = at / token_tiles * 16 * RR, t0 = at % token_tiles * 16 * TT;
+    uint8_t *mine = s_lds + wave * kStage;
+    const uint32_t from = lane / 8 * (uint32_t)a.pitch + ((lane ^ (lane / 8)) & 7) * 16, from8 = from + 8 * (uint32_t)a.pitch;
+    const uint8_t *xs = a.Xs + (uint64_t)min(t0 + lane % (16 * TT), a.tokens - 1) * a.spitch;
+    const uint8_t *ws = (M == 2 && lane % 2 ? a.Wus : a.Ws) + (uint64_t)(r0 / 128) * a.spitch;
+    auto fetch = [&](int b) __attribute__((always_inline)) {
         if (b >= a.kb) return;
-        // All of the step's reads in one block that waits for them: the
-        // compiler's own would wait for every load under way as well.
-        const uint32_t base = lds_address(cur) + group * 16384, x = base + wt * 4096, w = base + 8192 + wr * NR * 2048;
-        const uint32_t sc = lds_address(scale) + group * 512;
-        v4i v[8];
-        uint32_t c[4];
-        asm volatile(
-            "ds_read_b32 %8, %16\n\tds_read_b32 %9, %16 offset:64\n\tds_read_b32 %10, %17\n\tds_read_b32 %11, %17 offset:4\n\t"
-            "ds_read_b128 %0, %12\n\tds_read_b128 %1, %13\n\tds_read_b128 %2, %14\n\tds_read_b128 %3, %15\n\t"
-            "ds_read_b128 %4, %14 offset:%18\n\tds_read_b128 %5, %15 offset:%18\n\t"
-            "ds_read_b128 %6, %12 offset:2048\n\tds_read_b128 %7, %13 offset:2048\n\ts_waitcnt lgkmcnt(0)"
-            : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(c[0]),
-              "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3])
-            : "v"(x + s0), "v"(x + s1), "v"(w + s0), "v"(w + s1), "v"(sc + (wt * 32 + in) * 4), "v"(sc + 256), "i"(M == 2 ? 4096 : 2048)
-            : "memory");
-        auto pair = [&](int i) __attribute__((always_inline)) {
-            return v8i{v[i][0], v[i][1], v[i][2], v[i][3], v[i + 1][0], v[i + 1][1], v[i + 1][2], v[i + 1][3]};
-        };
-        const int shift = 8 * (b & 3);
-        const decltype(operand<EXACT>(v8i{}, 0)) ws[2] = {operand<EXACT>(pair(2), c[2] >> shift & 255u),
-                                                          operand<EXACT>(pair(4), c[M == 2 ? 3 : 2] >> shift & 255u)};
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-            multiply<2>(ws, operand<EXACT>(pair(t ? 6 : 0), c[t] >> shift & 255u), {&acc[0][0][t], &acc[M - 1][NR - 1][t]});
+        for (int f = 0; f < kFrags; f++) {
+            const int m = f / RR, first = f < kW ? r0 + f % RR * 16 : t0 + 16 * (f - kW);
+            const uint8_t *src = f >= kW ? a.X : m ? a.Wu : a.W;
+            const uint32_t rows = (uint32_t)__builtin_amdgcn_readfirstlane(max(min((f < kW ? a.rows : a.tokens) - first, 16), 0));
+            const auto buffer = tile_buffer(src + (uint64_t)first * a.pitch, rows * (uint32_t)a.pitch);
+            dma16(buffer, from, b * 128, mine + f * 2048);
+            dma16(buffer, from8, b * 128, mine + f * 2048 + 1024);
+        }
+        dma4(xs + (b & ~3), mine + kFrags * 2048);
+        dma4(ws + (b & ~3), mine + kFrags * 2048 + 256);
     };
-    fetch(0, s_0, s_c0), fetch(1, s_1, s_c1), fetch(2, s_2, s_c2);
-    for (int i = 0; i < steps; i += 4) {
-        step(i, s_0, s_c0, s_3, s_c3);
-        if (i + 1 < steps) step(i + 1, s_1, s_c1, s_0, s_c0);
-        if (i + 2 < steps) step(i + 2, s_2, s_c2, s_1, s_c1);
-        if (i + 3 < steps) step(i + 3, s_3, s_c3, s_2, s_c2);
+    v4f acc[kW][TT];
+#pragma unroll
+    for (int m = 0; m < kW; m++)
+#pragma unroll
+        for (int t = 0; t < TT; t++) acc[m][t] = v4f{0, 0, 0, 0};
+    fetch(wave);
+    const uint32_t base = lds_address(mine);
+    const uint32_t s0 = base + in * 128 + (part ^ swizzle(in)) * 16, s1 = base + in * 128 + ((part + 4) ^ swizzle(in)) * 16;
+    for (int b = wave; b < a.kb; b += W) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): this block is in LDS
+        const uint32_t sc = base + kFrags * 2048;
+        uint32_t c[6];
+        asm volatile(
+            "ds_read_b32 %0, %6\n\tds_read_b32 %1, %6 offset:64\n\tds_read_b32 %2, %6 offset:128\n\t"
+            "ds_read_b32 %3, %6 offset:192\n\tds_read_b32 %4, %7\n\tds_read_b32 %5, %7 offset:4\n\ts_waitcnt lgkmcnt(0)"
+            : "=&v"(c[0]), "=&v"(c[1]), "=&v"(c[2]), "=&v"(c[3]), "=&v"(c[4]), "=&v"(c[5])
+            : "v"(sc + in * 4), "v"(sc + 256)
+            : "memory");
+        Pair p[4];
+        p[0] = read_pair<0, 1>(s0, s1);
+        if constexpr (kFrags > 2) p[1] = read_pair<2, kFrags == 3 ? 2 : 3>(s0, s1);
+        if constexpr (kFrags > 4) p[2] = read_pair<4, kFrags == 5 ? 4 : 5>(s0, s1);
+        if constexpr (kFrags > 6) p[3] = read_pair<6, kFrags == 7 ? 6 : 7>(s0, s1);
+        fetch(b + W);  // it has been read
+        const int shift = 8 * (b & 3);
+        auto pair = [&](int f) __attribute__((always_inline)) { return join(p[f / 2].v[f % 2 * 2], p[f / 2].v[f % 2 * 2 + 1]); };
+        decltype(operand<EXACT>(v8i{}, 0)) w[kW];
+#pragma unroll
+        for (int m = 0; m < kW; m++) w[m] = operand<EXACT>(pair(m), c[4 + m / RR] >> shift & 255u);
+#pragma unroll
+        for (int t = 0; t < TT; t++) {
+            const auto x = operand<EXACT>(pair(kW + t), c[t] >> shift & 255u);
+            if constexpr (kW == 4) multiply(w, x, {&acc[0][t], &acc[kW - 3][t], &acc[kW - 2][t], &acc[kW - 1][t]});
+            else if constexpr (kW == 2) multiply(w, x, {&acc[0][t], &acc[kW - 1][t]});
+            else multiply(w, x, {&acc[0][t]});
+        }
     }
-    if constexpr (KG > 1) {
-        __builtin_amdgcn_s_waitcnt(0x0070);  // no load is under way into what the sums take
-        barrier();
-        v4f *sums = (v4f *)s_0;
-        if (group)
+    barrier();  // every wave has read its blocks
+    v4f *sums = (v4f *)s_lds;
 #pragma unroll
-            for (int i = 0; i < 4; i++) sums[((group - 1) * 4 + wave % 4) * 256 + i * 64 + lane] = acc[i / 2 / NR][i / 2 % NR][i % 2];
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-        barrier();
-        if (group) return;
+    for (int m = 0; m < kW; m++)
 #pragma unroll
-        for (int g = 1; g < KG; g++)
+        for (int t = 0; t < TT; t++) sums[((wave * kW + m) * TT + t) * 64 + lane] = acc[m][t];
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    barrier();
+    for (int i = wave; i < RR * TT; i += W) {
+        v4f v[M];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const v4f o = sums[((g - 1) * 4 + wave) * 256 + i * 64 + lane];
-                v4f &mine = acc[i / 2 / NR][i / 2 % NR][i % 2];
+        for (int m = 0; m < M; m++) {
+            v[m] = sums[(m * RR * TT + i) * 64 + lane];
+            for (int k = 1; k < W; k++) {
+                const v4f o = sums[((k * M + m) * RR * TT + i) * 64 + lane];
 #pragma unroll
-                for (int j = 0; j < 4; j++) mine[j] = mine[j] + o[j];
+                for (int j = 0; j < 4; j++) v[m][j] = v[m][j] + o[j];
             }
+        }
+        store_few<OUT>(a, v, t0 + 16 * (i % TT) + in, r0 + 16 * (i / TT), part, vec);
     }
-    store_tile<OUT>(a, t0 + wt * 32, r0 + wr * NR * 16, acc, r0 + 64 / M <= a.rows && vec, in, part);
 }
 
-// A tile's size, the workgroups of it that a CU holds (the first two rows: at
-// most; these kernels take one tile a workgroup), what a step of one of them
-// and of all of them takes and what a round over the GPU takes beside its
-// steps, in us (one MI355X). From whole calls of 20 and 48 steps, 8-bit sums
-// (f32 sums): 64 x 64 deep 8.0 and 13.4 (10.8, 19.9), two a CU 11.0 and 21.8
-// (17.5, 34.5); 64 x 64 three a CU 17.7 and 35.6 (25.6, 51.4), 2.5 rounds 46.4
-// and 105.8 (74.9, 176.6); 128 x 128 one 20.7 and 46.0 (31.3, 65.1), 2.5 rounds
-// 68 and 146 (102.6, 226); 256 x 128 25.5 and 52.3 (42, 82), three rounds 68
-// and 149 (115, 244); 256 x 256 37.3 and 71.8 (62, 127), two rounds 68 and 145
-// (125, 270).
+// A way to share out a product: a workgroup's tokens and rows (of each matrix),
+// how many of them a CU holds, the blocks of 128 columns in a step of theirs,
+// what a step takes where a CU has one of them and where it has all, and what a
+// round over the GPU takes beside its steps, in us: fitted to whole calls on one
+// MI355X, 1 to 1024 tokens, 640 to 20,480 rows, 1280 to 10,240 columns. Over
+// those the choice is 1.5% slower than the best shape on average (to f32; to
+// bf16 1.7%, a gated pair 0.4%), 25% at worst (512 tokens, 8192 x 8192, to bf16).
+// Both sides in us, to f32: 16 x 16 against 32 x 32 for 1 token, 2560 columns to
+// 10,240 rows 5.9 and 7.0, 16 tokens, 8192 x 8192 15.0 and 13.1; 32 x 16 against
+// 16 x 16 for 32 tokens, 6144 to 2560 6.5 and 7.9; 64 x 32 against 64 x 64 for 64
+// tokens, 8192 x 8192 17.0 and 22.2, for 256 51.5 and 37.9; 32 x 64 against 64 x 64
+// for 256 tokens, 2560 to 10,240 21.2 and 22.7; 64 x 64 of streams against tiles
+// of 128 x 128 there 22.7 and 30.2. To bf16, 512 tokens: streams 26.7, tiles of
+// 64 x 64 27.2, of 256 x 128 25.3; 1024 tokens, 4096 x 4096 tiles of 64 x 64 30.6,
+// of 128 x 128 36.9.
 struct Shape {
-    int tokens, rows, resident;
+    int tokens, rows, resident, blocks;
     float one, all, round;
 };
-constexpr int kShapeCount = 6;
-constexpr Shape kShapes[2][kShapeCount] = {
-    {{64, 64, 1, 0.19f, 0.19f, 4.2f}, {64, 64, 2, 0.36f, 0.36f, 3.8f}, {64, 64, 4, 0.35f, 0.85f, 3.0f},
-     {128, 128, 2, 0.75f, 0.97f, 6.0f}, {256, 128, 1, 0.96f, 0.96f, 4.5f}, {256, 256, 1, 1.35f, 1.35f, 9.0f}},
-    {{64, 64, 1, 0.33f, 0.33f, 4.3f}, {64, 64, 2, 0.60f, 0.60f, 5.4f}, {64, 64, 4, 0.50f, 1.42f, 3.0f},
-     {128, 128, 2, 1.15f, 1.80f, 7.0f}, {256, 128, 1, 1.50f, 1.50f, 11.0f}, {256, 256, 1, 2.50f, 2.50f, 11.0f}}};
+constexpr int kShapeCount = 10;
+constexpr Shape kShapes[3][kShapeCount] = {  // by Out
+    {{16, 16, 4, 8, 0.73f, 2.56f, 0.0f}, {32, 16, 3, 8, 0.89f, 2.27f, 0.5f}, {32, 32, 2, 8, 1.18f, 2.16f, 0.7f},
+     {64, 32, 1, 8, 1.55f, 1.55f, 1.9f}, {32, 64, 3, 4, 0.78f, 2.10f, 3.7f}, {64, 64, 2, 4, 1.19f, 2.10f, 4.2f},
+     {128, 128, 2, 1, 1.15f, 1.80f, 7.0f}, {256, 128, 1, 1, 1.50f, 1.50f, 11.0f}, {256, 256, 1, 1, 2.50f, 2.50f, 11.0f}},
+    {{16, 16, 4, 8, 0.68f, 2.53f, 0.0f}, {32, 16, 3, 8, 0.88f, 2.26f, 0.0f}, {32, 32, 2, 8, 1.15f, 2.16f, 0.0f},
+     {64, 32, 1, 8, 1.50f, 1.50f, 1.0f}, {32, 64, 3, 4, 0.69f, 1.93f, 3.1f}, {64, 64, 2, 4, 0.94f, 1.83f, 3.3f},
+     {128, 128, 2, 1, 0.75f, 0.97f, 6.0f}, {256, 128, 1, 1, 0.96f, 0.96f, 4.5f}, {256, 256, 1, 1, 1.35f, 1.35f, 9.0f},
+     {64, 64, 4, 1, 0.35f, 0.85f, 3.0f}},
+    {{16, 16, 3, 8, 0.94f, 2.58f, 0.0f}, {32, 16, 2, 8, 1.14f, 2.02f, 0.4f}, {32, 32, 1, 8, 1.40f, 1.40f, 1.9f},
+     {64, 32, 2, 4, 1.12f, 2.05f, 3.3f}}};
 
+template <int W, int RR, int TT, bool EXACT, Out OUT>
+void stream(sm_ctx *ctx, const Product &a) {
+    const int row_tiles = (a.rows + 16 * RR - 1) / (16 * RR), token_tiles = (a.tokens + 16 * TT - 1) / (16 * TT);
+    k_f8_stream<W, RR, TT, EXACT, OUT><<<(row_tiles * token_tiles + 7) / 8 * 8, 64 * W, 0, ctx->stream>>>(a, row_tiles, token_tiles, aligned(a, 4));
+}
 template <int BT, int BR, int WT, int WR, bool EXACT, Out OUT>
 void tiles(sm_ctx *ctx, const Product &a, int cus, int resident) {
-    const int m = OUT >= kHidden ? 2 : 1;
+    const int m = OUT == kCodes ? 2 : 1;
     Tiles t = {(a.tokens + BT - 1) / BT, (a.rows + BR / m - 1) / (BR / m), 0};
     // One block of columns: nothing is left of a tile's steps to bring the next in.
     const int n = t.tokens * t.rows, grid = (a.kb < 2 ? (n + 7) / 8 : min((n + 7) / 8, max(cus / 8, 1) * resident)) * 8;
@@ -749,71 +710,57 @@ int compute_units(sm_ctx *ctx) {
     return hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, ctx->device) == hipSuccess && cus > 0 ? cus : 256;
 }
 
-// Few tokens go to the waves that share out the columns. 8-bit sums: up to 4
-// tokens, and up to 32 while sixteens of tokens times rows stay under 5,120
-// (2560 columns, 2560 rows, 32 tokens 6.4 us against 8.0 in tiles, 48 tokens 9.0
-// against 8.0; 10240 rows, 1 token 6.8 against 7.8, 8 tokens 8.4 against 7.8).
-// f32 sums: up to 16 tokens, and while workgroups of 64 tokens and 16 rows are
-// fewer than the CUs (2560 rows, 64 tokens 9.5 against 10.8, 100 tokens 14.1
-// against 10.8; 10240 rows, 16 tokens 9.8 against 10.5, 32 tokens 14.1 against
-// 10.7).
-bool takes_few(const Product &a, bool exact) {
-    const int64_t sixteens = (a.tokens + 15) / 16;
-    if (exact) return a.tokens <= 16 || (int64_t)((a.rows + 15) / 16) * ((sixteens + 3) / 4) <= 200;
-    return a.tokens <= 4 || (a.tokens <= 32 && sixteens * a.rows <= 5120);
-}
-// Else the tile whose rounds over the GPU take least: its index in kShapes, and
-// that time in us.
-int best_shape(const Product &a, bool exact, int m, int cus, float *us) {
+// The shape whose rounds over the GPU take least: its index in kShapes, and that time in us.
+int best_shape(const Product &a, Out out, int cus, float *us) {
     int best = -1;
     for (int i = 0; i < kShapeCount; i++) {
-        const Shape &s = kShapes[exact][i];
-        const int64_t n = (int64_t)((a.tokens + s.tokens - 1) / s.tokens) * ((a.rows + s.rows / m - 1) / (s.rows / m));
+        const Shape &s = kShapes[out][i];
+        if (s.tokens == 0) continue;
+        const int64_t n = (int64_t)((a.tokens + s.tokens - 1) / s.tokens) * ((a.rows + s.rows - 1) / s.rows);
         const int64_t slots = (int64_t)cus * s.resident, over = (n % slots + cus - 1) / cus;  // workgroups of a CU in the last round
-        if (i < 2 && n > slots) continue;
+        const int steps = (a.kb + s.blocks - 1) / s.blocks;
         const float last = s.resident == 1 ? s.one : s.one + (s.all - s.one) * (over - 1) / (s.resident - 1);
-        const float time = n / slots * (s.all * a.kb + s.round) + (over ? last * a.kb + s.round : 0.0f);
+        const float time = n / slots * (s.all * steps + s.round) + (over ? last * steps + s.round : 0.0f);
         if (best < 0 || time < *us) *us = time, best = i;
     }
     return best;
 }
-template <int KG, bool EXACT, Out OUT>
-void deep(sm_ctx *ctx, const Product &a) {
-    constexpr int kRows = OUT == kHidden ? 32 : 64;
-    const Tiles t = {(a.tokens + 63) / 64, (a.rows + kRows - 1) / kRows, 0};
-    k_f8_deep<KG, 4, EXACT, OUT><<<(t.tokens * t.rows + 7) / 8 * 8, 256 * KG, 0, ctx->stream>>>(a, t, aligned(a, OUT == kBf16 ? 8 : 4));
-}
 template <bool EXACT, Out OUT>
 void multiply_by_size(sm_ctx *ctx, const Product &a, int cus) {
-    if (takes_few(a, EXACT)) return few<EXACT, OUT>(ctx, a);
     float us = 0.0f;
-    const int best = best_shape(a, EXACT, OUT == kHidden ? 2 : 1, cus, &us), resident = kShapes[EXACT][best].resident;
-    if (best == 0) deep<2, EXACT, OUT>(ctx, a);
-    else if (best == 1) deep<1, EXACT, OUT>(ctx, a);
-    else if (best == 2) tiles<64, 64, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
-    else if (best == 3) tiles<128, 128, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
-    else if (best == 4) tiles<256, 128, 4, 2, EXACT, OUT>(ctx, a, cus, resident);
-    else tiles<256, 256, 2, 4, EXACT, OUT>(ctx, a, cus, resident);
+    const int best = best_shape(a, OUT, cus, &us), resident = kShapes[OUT][best].resident;
+    if (best == 0) return stream<8, 1, 1, EXACT, OUT>(ctx, a);
+    if (best == 1) return stream<8, 1, 2, EXACT, OUT>(ctx, a);
+    if (best == 2) return stream<8, 2, 2, EXACT, OUT>(ctx, a);
+    if constexpr (OUT == kHidden) {
+        stream<4, 2, 4, EXACT, OUT>(ctx, a);
+    } else {
+        if (best == 3) return stream<8, 2, 4, EXACT, OUT>(ctx, a);
+        if (best == 4) return stream<4, 4, 2, EXACT, OUT>(ctx, a);
+        if (best == 5) return stream<4, 4, 4, EXACT, OUT>(ctx, a);
+        if (best == 6) return tiles<128, 128, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
+        if (best == 7) return tiles<256, 128, 4, 2, EXACT, OUT>(ctx, a, cus, resident);
+        if (best == 8) return tiles<256, 256, 2, 4, EXACT, OUT>(ctx, a, cus, resident);
+        if constexpr (OUT == kBf16) tiles<64, 64, 2, 2, EXACT, OUT>(ctx, a, cus, resident);
+    }
 }
 
 // A gated pair: sums to f32 into the workspace and the conversion of rows, or
 // one kernel on the 8-bit matrix unit whose tiles of 128 columns end in codes.
-// That takes 1.6 us a step and 14 us a tile of 256 tokens, 1.0 and 6 of 128
-// (measured as above: 4096 tokens, 2560 to 8192, 308 us apart, 186 and 208;
-// 512 tokens 50, 49 and 32; 128 tokens 24, 44 and 30).
+// That takes 1.6 us a step and 14 us a tile of 256 tokens, 1.05 and 9 of 128
+// (measured as above: 4096 tokens, 2560 to 8192, 186 and 208 us; 768 tokens, 4096
+// to 4096 46 of 128 tokens, 61 apart; 256 tokens, 2560 to 6144 31 and 26).
 int gate_up(sm_ctx *ctx, Product &a, uint8_t *codes, uint8_t *scales, void *workspace) {
     const int cus = compute_units(ctx);
     const F8Layout L = f8_layout(a.tokens, a.rows, 1);
     a.codes = codes, a.scales = scales, a.codes_pitch = L.pitch, a.scales_pitch = L.spitch;
-    if (!takes_few(a, true)) {
-        auto rounds = [&](int tokens) { return ((int64_t)((a.tokens + tokens - 1) / tokens) * (int64_t)(L.pitch / 128) + cus - 1) / cus; };
-        float apart = 0.0f;
-        best_shape(a, true, 2, cus, &apart);
-        apart += 3.0f + 5.0f * a.tokens * a.rows / 4e6f;  // and the conversion
-        const float wide = rounds(256) * (1.6f * a.kb + 14.0f), narrow = rounds(128) * (1.0f * a.kb + 6.0f);
-        if (wide < apart && wide < narrow) return tiles<256, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
-        if (narrow < apart) return tiles<128, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
-    }
+    auto rounds = [&](int tokens) { return ((int64_t)((a.tokens + tokens - 1) / tokens) * (int64_t)(L.pitch / 128) + cus - 1) / cus; };
+    float apart = 0.0f;
+    best_shape(a, kHidden, cus, &apart);
+    apart += 3.0f + 5.0f * a.tokens * a.rows / 4e6f;  // and the conversion
+    const float wide = rounds(256) * (1.6f * a.kb + 14.0f), narrow = rounds(128) * (1.05f * a.kb + 9.0f);
+    if (wide < apart && wide < narrow) return tiles<256, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
+    if (narrow < apart) return tiles<128, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
     a.Y = workspace, a.stride = a.rows;
     multiply_by_size<true, kHidden>(ctx, a, cus);
     if (int rc = launched(ctx)) return rc;
