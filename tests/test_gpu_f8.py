@@ -508,3 +508,73 @@ def test_two_contexts(backend):
             assert np.array_equal(get(be, Y, np.float32, (tokens, rows)), want)
     finally:
         other.dispose()
+
+
+# ----------------------------------------- products whose waves share out the columns
+STREAMS = [  # tokens, cols, rows: workgroups of (tokens x rows; to f32, to bf16, gated), the last ones ending inside
+    (5, 2570, 4003),    # 16 x 16
+    (2003, 260, 20),    # the same, tokens over the XCDs, fewer blocks than waves
+    (19, 1300, 2505),   # 32 x 16
+    (70, 1290, 2503),   # 32 x 32 (gated 32 x 16)
+    (17, 2500, 5003),   # gated 32 x 32
+    (97, 1300, 2503),   # 64 x 32
+    (131, 260, 5003),   # 32 x 64 (gated 64 x 32)
+    (3, 6010, 10003),   # to bf16 32 x 64
+    (205, 2600, 2503)]  # 64 x 64 (gated 64 x 32)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("extra,offset", [(3, 2), (5, 4)])
+@pytest.mark.parametrize("tokens,cols,rows", STREAMS)
+def test_project_streams(backend, tokens, cols, rows, type, extra, offset):
+    rng = np.random.default_rng(tokens + cols + rows)
+    X, W = p.matrix(rng, tokens, cols, 1), p.matrix(rng, rows, cols, 128)
+    got, rest = product(backend, X, W, tokens, cols, rows, type, rows + extra, offset)
+    want = X[2].astype(np.float32) @ W[2].astype(np.float32).T  # exact in f32: every partial sum is
+    assert np.array_equal(got, want if type == "f32" else p.bf16(want).astype(np.float32))
+    assert np.all(rest == -7)
+
+
+@pytest.mark.parametrize("tokens,cols,rows", STREAMS)
+def test_project_streams_residual(backend, tokens, cols, rows):
+    rng = np.random.default_rng(tokens + cols + rows)
+    X, W = p.matrix(rng, tokens, cols, 1), p.matrix(rng, rows, cols, 128)
+    r = rng.normal(0, 100, tokens * rows + 3).astype(np.float32)
+    Y = put(backend, r)
+    got, rest = product(backend, X, W, tokens, cols, rows, "f32", rows, 0, residual=Y, Y=Y)
+    assert np.array_equal(got, r[:-3].reshape(tokens, rows) + X[2].astype(np.float32) @ W[2].astype(np.float32).T)
+    assert np.array_equal(rest, r[-3:])
+
+
+@pytest.mark.parametrize("tokens,cols,ff", STREAMS)
+def test_gate_up_streams(backend, tokens, cols, ff):
+    rng = np.random.default_rng(tokens + cols + ff)
+    X, Wg, Wu = p.matrix(rng, tokens, cols, 1), p.matrix(rng, ff, cols, 128), p.matrix(rng, ff, cols, 128)
+    Wg[1][:] -= 5
+    g, u = (X[2].astype(np.float32) @ w[2].astype(np.float32).T for w in (Wg, Wu))  # exact
+    p.check_f8(*gate_up(backend, X, Wg, Wu, tokens, cols, ff), p.silu(g.astype(np.float64) / 32) * u, 8 * HALF24)
+
+
+@pytest.mark.parametrize("tokens,cols,rows", [(3, 6010, 10003), (97, 1300, 2503), (205, 2600, 2503)])
+def test_project_streams_nan(backend, tokens, cols, rows):
+    """A NaN code of the last token and one of the last row, in the last block: no other output sees them."""
+    rng = np.random.default_rng(rows)
+    X, W = p.matrix(rng, tokens, cols, 1), p.matrix(rng, rows, cols, 128)
+    X[0][tokens - 1, cols - 1] = 0x7f
+    W[0][rows - 1, cols - 1] = 0xff
+    for type in ("f32", "bf16"):
+        got, _ = product(backend, X, W, tokens, cols, rows, type, rows, 0)
+        nan = np.isnan(got)
+        assert nan[-1].all() and nan[:, -1].all() and not nan[:-1, :-1].any()
+
+
+@pytest.mark.parametrize("tokens,cols,rows", [(17, 2500, 5003), (97, 1300, 2503), (205, 2600, 2503)])
+def test_project_streams_ordinary(backend, tokens, cols, rows):
+    rng = np.random.default_rng(tokens + cols + rows)
+    X, W = p.ordinary(rng, tokens, cols, 1), p.ordinary(rng, rows, cols, 128)
+    want, size = X[2] @ W[2].T, np.abs(X[2]) @ np.abs(W[2]).T
+    for type in ("f32", "bf16"):
+        got, _ = product(backend, X, W, tokens, cols, rows, type, rows, 0)
+        # as in test_project_ordinary: 128 additions in a block, one a block, one a wave
+        sums = (128 + p.blocks(cols, 128) + 8) * 2.0 ** -23 * size
+        assert np.all(np.abs(got - want) <= (sums if type == "f32" else sums + largest_cut(X[2], W[2]) + 2.0 ** -8 * np.abs(want)))
