@@ -259,6 +259,19 @@ inline F8Layout f8_layout(int64_t rows, int64_t cols, int block_rows) {
 struct F8Operand {
     const uint8_t *codes, *scales;
 };
+// A column block of up to `most` rows of codes, `left` of them there (none, or
+// fewer than none, past the matrix's end), as a buffer from the first row on:
+// its bytes and the offset that all lanes read from. A lane's 16 bytes at
+// `at` are read where at < bytes - offset in unsigned arithmetic, and are zeros
+// elsewhere. A buffer of no rows takes the offset 0: any other would make that
+// difference wrap, and lanes past the matrix's end would read.
+struct F8Piece {
+    uint32_t bytes, offset;
+};
+constexpr F8Piece f8_piece(int left, int most, uint32_t pitch, int block) {
+    const uint32_t bytes = (uint32_t)(left < 0 ? 0 : left < most ? left : most) * pitch, offset = (uint32_t)block * 128;
+    return {bytes, offset < bytes ? offset : bytes};
+}
 // Unchecked launchers on raw device pointers (f8_convert.hip, f8_project.hip).
 int f8_quantize_launch(sm_ctx *ctx, const void *X, bool bf16, int rows, int cols, int block_rows, uint8_t *codes,
                        uint8_t *scales);
