@@ -213,12 +213,11 @@ bool aligned(const Product &a, int n) { return a.stride % n == 0 && a.offset % n
 // whose order goes by the row's number, so that the 16 lanes that read one
 // column of 16 rows meet all banks.
 typedef __attribute__((address_space(3))) void lds_void;
-// A tile's rows as a buffer: a load past its end gives zeros (f8_piece).
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_buffer(const uint8_t *base, F8Piece p) {
-    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, p.bytes, 0x00027000);
-}
-__device__ __forceinline__ F8Piece piece_of(int left, int most, uint64_t pitch, int block) {
-    return f8_piece(__builtin_amdgcn_readfirstlane(left), most, (uint32_t)pitch, block);
+// Rows of codes as a buffer: a load of other rows gives zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t piece_buffer(const uint8_t *m, int first, int left, int rows, int most, uint64_t pitch) {
+    const F8Piece p = f8_piece(first, left, rows, most);
+    const uint32_t at = __builtin_amdgcn_readfirstlane(p.first), count = __builtin_amdgcn_readfirstlane(p.count);
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(m + at * pitch), 0, count * (uint32_t)pitch, 0x00027000);
 }
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t from, uint32_t lane_offset, uint32_t offset, void *lds) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void *)lds, 16, lane_offset, offset, 0, 0);
@@ -322,10 +321,9 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
                 continue;
             }
             const int in_w = j - BT, row = in_w < 0 ? j : in_w % (BR / M);
-            const uint8_t *m = in_w < 0 ? a.X + (uint64_t)(p.t0 + row) * a.pitch
-                                        : (in_w < BR / M ? a.W : a.Wu) + (uint64_t)(p.r0 + row) * a.pitch;
-            const F8Piece piece = piece_of((in_w < 0 ? p.x_rows : p.w_rows) - row, kRows, a.pitch, b);
-            dma16(tile_buffer(m, piece), from, piece.offset, to + wave * 1024 + j * 128);
+            const auto buffer = in_w < 0 ? piece_buffer(a.X, p.t0 + row, p.x_rows - row, a.tokens, kRows, a.pitch)
+                                         : piece_buffer(in_w < BR / M ? a.W : a.Wu, p.r0 + row, p.w_rows - row, a.rows, kRows, a.pitch);
+            dma16(buffer, from, b * 128, to + wave * 1024 + j * 128);
         }
     };
 
@@ -597,10 +595,10 @@ __global__ void __launch_bounds__(64 * W) k_f8_stream(Product a, int row_tiles, 
         for (int f = 0; f < kFrags; f++) {
             const int m = f / RR, first = f < kW ? r0 + f % RR * 16 : t0 + 16 * (f - kW);
             const uint8_t *src = f >= kW ? a.X : m ? a.Wu : a.W;
-            const F8Piece piece = piece_of((f < kW ? a.rows : a.tokens) - first, 16, a.pitch, b);
-            const auto buffer = tile_buffer(src + (uint64_t)first * a.pitch, piece);
-            dma16(buffer, from, piece.offset, mine + f * 2048);
-            dma16(buffer, from8, piece.offset, mine + f * 2048 + 1024);
+            const int rows = f < kW ? a.rows : a.tokens;
+            const auto buffer = piece_buffer(src, first, rows - first, rows, 16, a.pitch);
+            dma16(buffer, from, b * 128, mine + f * 2048);
+            dma16(buffer, from8, b * 128, mine + f * 2048 + 1024);
         }
         dma4(xs + (b & ~3), mine + kFrags * 2048);
         dma4(ws + (b & ~3), mine + kFrags * 2048 + 256);

@@ -259,18 +259,17 @@ inline F8Layout f8_layout(int64_t rows, int64_t cols, int block_rows) {
 struct F8Operand {
     const uint8_t *codes, *scales;
 };
-// A column block of up to `most` rows of codes, `left` of them there (none, or
-// fewer than none, past the matrix's end), as a buffer from the first row on:
-// its bytes and the offset that all lanes read from. A lane's 16 bytes at
-// `at` are read where at < bytes - offset in unsigned arithmetic, and are zeros
-// elsewhere. A buffer of no rows takes the offset 0: any other would make that
-// difference wrap, and lanes past the matrix's end would read.
+// The rows that one load of codes takes as a buffer: of up to `most` from
+// `first` on the `left` that are there (no more than rows - first); the buffer
+// gives zeros for the others. Where none is there, one row of the matrix, the
+// last at most, whose values are not used: a raw buffer takes the column
+// block's scalar offset from its bytes in unsigned arithmetic, which wraps if
+// it has none, and lanes past the matrix's end would read.
 struct F8Piece {
-    uint32_t bytes, offset;
+    int first, count;
 };
-constexpr F8Piece f8_piece(int left, int most, uint32_t pitch, int block) {
-    const uint32_t bytes = (uint32_t)(left < 0 ? 0 : left < most ? left : most) * pitch, offset = (uint32_t)block * 128;
-    return {bytes, offset < bytes ? offset : bytes};
+constexpr F8Piece f8_piece(int first, int left, int rows, int most) {
+    return {first < rows ? first : rows - 1, left < 1 ? 1 : left < most ? left : most};
 }
 // Unchecked launchers on raw device pointers (f8_convert.hip, f8_project.hip).
 int f8_quantize_launch(sm_ctx *ctx, const void *X, bool bf16, int rows, int cols, int block_rows, uint8_t *codes,

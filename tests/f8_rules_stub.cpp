@@ -4,7 +4,7 @@
 
 #include "../stratacuda_amd/csrc/internal.h"
 
-extern "C" void rule_piece(int left, int most, uint32_t pitch, int block, uint32_t *bytes, uint32_t *offset) {
-    const smi::F8Piece p = smi::f8_piece(left, most, pitch, block);
-    *bytes = p.bytes, *offset = p.offset;
+extern "C" void rule_piece(int first, int left, int rows, int most, int *to) {
+    const smi::F8Piece p = smi::f8_piece(first, left, rows, most);
+    to[0] = p.first, to[1] = p.count;
 }

@@ -18,34 +18,31 @@ def rules(tmp_path_factory):
     return ctypes.CDLL(out)
 
 
-def piece(rules, left, most, pitch, block):
-    b, o = ctypes.c_uint32(), ctypes.c_uint32()
-    rules.rule_piece(left, most, pitch, block, ctypes.byref(b), ctypes.byref(o))
-    return b.value, o.value
-
-
-def readable(bytes_, offset, at):
+def readable(nbytes, scalar, at):
     """Whether a lane at `at` reads memory: the range check of a raw buffer, which takes the scalar offset from the bytes
     in unsigned arithmetic."""
-    return at < (bytes_ - offset) % 2 ** 32
+    return at < (nbytes - scalar) % 2 ** 32
 
 
-@pytest.mark.parametrize("most", [8, 16, 32, 64])  # rows that one load brings: of a stream's wave 8 and 16, of a tile 32 and 64
-@pytest.mark.parametrize("pitch", [128, 256, 640, 2 ** 21])
-def test_pieces_stay_in_the_matrix(rules, most, pitch):
-    """Rows that are there are read whole, at their column block; none past the matrix's end, where a tile is
-    partly or wholly behind it too."""
-    last = pitch // 128 - 1
-    for left in (-2 ** 21, -300, -1, 0, 1, 2, most - 1, most, most + 1, 300, 2 ** 21):
-        for block in {0, last // 2, last}:
-            bytes_, offset = piece(rules, left, most, pitch, block)
-            assert bytes_ <= max(left, 0) * pitch
-            for row in range(most):
-                for column in (0, 16, 112):
-                    at = row * pitch + column
-                    assert readable(bytes_, offset, at) == (row < left), (left, block, row)
-                    if row < left:
-                        assert offset + at == row * pitch + block * 128 + column
-                        assert offset + at + 16 <= bytes_
-    # a buffer of no rows at any other offset would be read
-    assert readable(0, 128, 0) and not readable(0, 0, 0)
+@pytest.mark.parametrize("most", [16, 32, 64])  # rows of one load: of a stream's wave, of four and eight waves of a tile
+@pytest.mark.parametrize("rows,pitch", [(1, 128), (7, 256), (33, 640), (200, 384), (2 ** 12, 2 ** 21)])
+def test_loads_stay_in_the_matrix(rules, most, rows, pitch):
+    """Rows that are there are read whole, at their column block, and what lies past the matrix's end is not: for loads
+    partly and wholly behind it, and for a workgroup past its last tile (none left, wherever it stands)."""
+    last, to = pitch // 128 - 1, (ctypes.c_int * 2)()
+    for first in sorted({0, 1, most - 1, most, max(rows - most, 0), max(rows - 1, 0), rows, rows + 1, rows + 255}):
+        for left in {rows - first, min(rows - first, 0) - 5, min(rows - first, 0)}:
+            rules.rule_piece(first, left, rows, most, to)
+            base, nbytes = to[0], to[1] * pitch
+            assert 0 <= base and base + to[1] <= rows
+            assert left < 1 or base == first
+            for block in {0, last // 2, last}:
+                for row in range(most):
+                    for column in (0, 16, 112):
+                        at = row * pitch + column
+                        if readable(nbytes, block * 128, at):
+                            assert base * pitch + block * 128 + at + 16 <= rows * pitch
+                            assert row < max(left, 1)
+                        else:
+                            assert row >= left
+    assert readable(0, 128, 0)  # what a scalar offset does to a buffer of no rows
