@@ -301,13 +301,10 @@ int sm_f8_project(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int co
 
 /* silu(X . Wg) * (X . Wu) as an f8 matrix [tokens x ff] of block_rows 1;
  * silu(g) = g / (1 + exp(-g)); X as in sm_f8_project, Wg and Wu f8 matrices
- * [ff x cols] of block_rows 128 (they may be one buffer). The sums are those
- * of sm_f8_project's type f32, or its bf16 type's before their rounding where
- * that is faster; the scales are those of the f32 sums then too, unless those
- * are off by more than 2^-10 of a block's largest value (where more than eight
- * columns lie within 2^-9 of it, the first eight decide). The workspace holds
- * sm_f8_gate_up_workspace(...) bytes; a call leaves nothing in it that a
- * later call needs. */
+ * [ff x cols] of block_rows 128 (they may be one buffer). The sums are f32's
+ * as in sm_f8_project's type f32, for any number of tokens. The workspace holds
+ * sm_f8_gate_up_workspace(...) bytes, which calls of many tokens may leave
+ * untouched; a call leaves nothing in it that a later call needs. */
 int sm_f8_gate_up_workspace(int tokens, int ff, uint64_t *bytes);
 int sm_f8_gate_up(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int cols, uint64_t Wg, uint64_t wg_scales,
                   uint64_t Wu, uint64_t wu_scales, int ff, uint64_t codes, uint64_t scales, uint64_t workspace,

@@ -3,16 +3,19 @@
 //
 //   Y[t, n] = sum_b 2^(ex[t, b] + ew[n / 128, b]) * sum_{k in block b} x[t, k] w[n, k]
 //
-// Two ways to multiply, by what the output keeps:
-//   8-bit and bf16 outputs: v_mfma_scale_f32_16x16x128_f8f6f4, one instruction
-//     a block of 128, which takes the two scales as operands. It aligns the
-//     products of each eight neighbours to the largest of them and cuts them
-//     off 13 bits below its leading bit before it adds the eights in f32
-//     (measured on one MI355X: 1.3e-5 of the result for normal values), far
-//     below those outputs' rounding (2^-9, 2^-4).
-//   f32 outputs: code times scale as bf16 (exact: 4 significant bits in 8, the
-//     exponent of f32) in v_mfma_f32_16x16x32_bf16, whose sums are f32's (1e-7
-//     measured), at half the rate.
+// Two ways to multiply:
+//   f32 and gated outputs: code times scale as bf16 (exact: 4 significant bits in
+//     8, the exponent of f32) in v_mfma_f32_16x16x32_bf16, whose sums are f32's
+//     (1e-7 measured).
+//   bf16 outputs: v_mfma_scale_f32_16x16x128_f8f6f4, one instruction a block of
+//     128, which takes the two scales as operands, at twice the rate. It aligns
+//     the products of each eight neighbours to the largest of them and cuts them
+//     off 13 bits below its leading bit before it adds the eights in f32: off by
+//     7 * 2^-13 of the sum of magnitudes at most (measured on one MI355X: 1.3e-5
+//     of the result for normal values, where rounding to bf16 costs 1e-3).
+// A gated pair takes f32 sums at every size: its scales are a decision on the
+// largest of 128 sums, and what is left of sums that cancel, times what is left
+// of others, is held to its own size by the codes.
 #include "f8_device.h"
 
 namespace {
@@ -236,33 +239,6 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 }
 __device__ __forceinline__ int swizzle(int row) { return row & 7; }
 
-// silu(gate) * up of one token and column by one wave, in f32 sums.
-__device__ __forceinline__ float exact_hidden(const Product &a, int token, int col, int lane) {
-    const uint64_t ws = (uint64_t)(col / 128) * a.spitch;
-    const uint8_t *x = a.X + token * a.pitch, *w = a.W + col * a.pitch, *u = a.Wu + col * a.pitch;
-    const uint8_t *sx = a.Xs + token * a.spitch, *sw = a.Ws + ws, *su = a.Wus + ws;
-    float g = 0.0f, v = 0.0f;
-#pragma unroll 4
-    for (int k = lane * 16; k < a.kb * 128; k += 1024) {  // eight lanes a block of 128
-        const v4i xc = *(const v4i *)(x + k), wc = *(const v4i *)(w + k), uc = *(const v4i *)(u + k);
-        const int e = sx[k / 128] - 127, eg = e + sw[k / 128] - 127, ev = e + su[k / 128] - 127;
-        float pg = 0.0f, pv = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const v2f x0 = __builtin_amdgcn_cvt_pk_f32_fp8(xc[i], false), x1 = __builtin_amdgcn_cvt_pk_f32_fp8(xc[i], true);
-            const v2f w0 = __builtin_amdgcn_cvt_pk_f32_fp8(wc[i], false), w1 = __builtin_amdgcn_cvt_pk_f32_fp8(wc[i], true);
-            const v2f u0 = __builtin_amdgcn_cvt_pk_f32_fp8(uc[i], false), u1 = __builtin_amdgcn_cvt_pk_f32_fp8(uc[i], true);
-            pg = fmaf(x0[0], w0[0], fmaf(x0[1], w0[1], fmaf(x1[0], w1[0], fmaf(x1[1], w1[1], pg))));
-            pv = fmaf(x0[0], u0[0], fmaf(x0[1], u0[1], fmaf(x1[0], u1[0], fmaf(x1[1], u1[1], pv))));
-        }
-        g = g + __builtin_amdgcn_ldexpf(pg, eg);
-        v = v + __builtin_amdgcn_ldexpf(pv, ev);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) g = g + __shfl_xor(g, d, 64), v = v + __shfl_xor(v, d, 64);
-    return silu_times(g, v);
-}
-
 // The tiles in the order of the eight XCDs that workgroups go round: each XCD
 // takes neighbouring tiles, four of tokens by as many of rows, so that its L2
 // holds what they share.
@@ -358,29 +334,11 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
         for (int t = 0; t < NT; t++) sx[t] = scale[(wt * NT + t) * 16 + in] >> shift & 255u;
     };
     // 8-bit outputs: a tile's 128 columns are one block of scales. A wave has 32
-    // of them, so the largest magnitudes meet in LDS. The sums are near, not
-    // exact (above): where a token's largest lies so near to a scale's border
-    // that the exact one may lie past it, the columns that may hold it (the
-    // first eight of them) are summed again in f32, and the scale is theirs.
+    // of them, so the largest magnitudes meet in LDS.
     __shared__ float s_most[OUT == kCodes ? WR : 1][OUT == kCodes ? BT : 1];
-    __shared__ uint32_t s_columns[OUT == kCodes ? BT : 1][4], s_any;
     auto finish_codes = [&](int t0, int r0) __attribute__((always_inline)) {
-        static_assert(OUT != kCodes || (NR == 2 && BR == 256 && BT <= 32 * WT * WR), "");
-        // The sums are off by about 2e-5, by 1e-4 and more beside large neighbours.
-        // 4096 tokens, 4096 to 8192: 254 us without a second look, 256 with it.
-        constexpr float kNear = 1.0f / 1024;
-        // within kNear of 1.75 * 2^x, by the bits: kNear of the 2^23 steps from 2^x to 2^(x + 1), times 1.75
-        auto near = [](float m) {
-            constexpr int kBits = (int)(kNear * 1.75f * 8388608.0f);
-            return abs((int)(__float_as_uint(m) & 0x7fffffu) - 0x600000) <= kBits;
-        };
-        auto wait = []() {
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-            barrier();
-        };
+        static_assert(OUT != kCodes || (NR == 2 && BR == 256), "");
         const int col = wr * 32 + 4 * part;  // of the block
-        if (threadIdx.x == 0) s_any = 0;
-        for (int i = threadIdx.x; i < BT * 4; i += kThreads) s_columns[0][i] = 0;
         const bool whole = r0 + BR / M <= a.rows;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -391,65 +349,21 @@ __global__ void __launch_bounds__(64 * WT * WR) k_f8_tile(Product a, Tiles tiles
                 for (int i = 0; i < 4; i++) {
                     const float h = silu_times(acc[0][r][t][i], acc[M - 1][r][t][i]);
                     acc[0][r][t][i] = whole || r0 + col + 16 * r + i < a.rows ? h : 0.0f;
-                    most = fmaxf(most, fabsf(acc[0][r][t][i]));
+                    most = fmaxf(most, f8::finite_magnitude(acc[0][r][t][i]));
                 }
-            if (__any(most == INFINITY)) {
-                most = 0.0f;
-#pragma unroll
-                for (int r = 0; r < NR; r++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) most = fmaxf(most, f8::finite_magnitude(acc[0][r][t][i]));
-            }
             most = fmaxf(most, __shfl_xor(most, 16, 64));
             most = fmaxf(most, __shfl_xor(most, 32, 64));
             if (part == 0) s_most[wr][(wt * NT + t) * 16 + in] = most;
         }
-        wait();
-        float most[NT];
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const int token = (wt * NT + t) * 16 + in;
-            most[t] = s_most[0][token];
-#pragma unroll
-            for (int k = 1; k < WR; k++) most[t] = fmaxf(most[t], s_most[k][token]);
-            if (t0 + token < a.tokens && near(most[t])) {
-                uint32_t bits = 0;
-#pragma unroll
-                for (int r = 0; r < NR; r++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (f8::finite_magnitude(acc[0][r][t][i]) >= most[t] * (1.0f - 2 * kNear)) bits |= 1u << (16 * r + 4 * part + i);
-                if (bits) atomicOr(&s_columns[token][wr], bits);
-                s_any = 1;
-            }
-        }
-        wait();
-        if (__builtin_amdgcn_readfirstlane(s_any)) {
-            const int token = wave + lane * (WT * WR);
-            bool mine = false;
-            if (token < BT)
-#pragma unroll
-                for (int k = 0; k < 4; k++) mine |= s_columns[token][k] != 0;
-            uint64_t todo = __ballot(mine);
-            while (todo) {
-                const int one = wave + __builtin_ctzll(todo) * (WT * WR);
-                todo &= todo - 1;
-                float m = 0.0f;
-                int left = 8;
-                for (int k = 0; k < 4; k++) {
-                    uint32_t bits = __builtin_amdgcn_readfirstlane(s_columns[one][k]);
-                    for (; bits && left; bits &= bits - 1, left--)
-                        m = fmaxf(m, f8::finite_magnitude(exact_hidden(a, t0 + one, r0 + 32 * k + __builtin_ctz(bits), lane)));
-                }
-                if (lane == 0) s_most[0][one] = m;
-            }
-            wait();
-        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        barrier();
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const int token = t0 + (wt * NT + t) * 16 + in;
-            const float m = near(most[t]) ? s_most[0][(wt * NT + t) * 16 + in] : most[t];
-            const uint32_t byte = f8::scale_byte(m);
+            float most = s_most[0][(wt * NT + t) * 16 + in];
+#pragma unroll
+            for (int k = 1; k < WR; k++) most = fmaxf(most, s_most[k][(wt * NT + t) * 16 + in]);
+            const uint32_t byte = f8::scale_byte(most);
             const float inverse = f8::inverse_scale(byte);
             // of two sets of 16 columns one lane takes eight of the first, the other eight of the second
             const auto v = __builtin_amdgcn_permlane16_swap(f8::codes4(acc[0][0][t], inverse), f8::codes4(acc[0][NR - 1][t], inverse), false, false);
@@ -750,10 +664,12 @@ void multiply_by_size(sm_ctx *ctx, const Product &a, int cus) {
 }
 
 // A gated pair: sums to f32 into the workspace and the conversion of rows, or
-// one kernel on the 8-bit matrix unit whose tiles of 128 columns end in codes.
-// That takes 1.6 us a step and 14 us a tile of 256 tokens, 1.05 and 9 of 128
-// (measured as above: 4096 tokens, 2560 to 8192, 186 and 208 us; 768 tokens, 4096
-// to 4096 46 of 128 tokens, 61 apart; 256 tokens, 2560 to 6144 31 and 26).
+// one kernel whose tiles of 128 columns end in codes: 2.6 us a step and 16 us a
+// round of tiles of 256 tokens, 1.55 and 9 of 128. Fitted as above, 96 to 8192
+// tokens, 640 to 8192 columns out, 1280 to 6144 in: 0.2% slower than the best of
+// the three on average, 7% at worst. In us, of 256 tokens, of 128, apart: 4096
+// tokens, 2560 to 8192 268, 288 and 394; 1536 tokens, 2560 to 2560 63, 40 and 56;
+// 256 tokens, 2560 to 8192 61, 38 and 32.
 int gate_up(sm_ctx *ctx, Product &a, uint8_t *codes, uint8_t *scales, void *workspace) {
     const int cus = compute_units(ctx);
     const F8Layout L = f8_layout(a.tokens, a.rows, 1);
@@ -762,9 +678,9 @@ int gate_up(sm_ctx *ctx, Product &a, uint8_t *codes, uint8_t *scales, void *work
     float apart = 0.0f;
     best_shape(a, kHidden, cus, &apart);
     apart += 3.0f + 5.0f * a.tokens * a.rows / 4e6f;  // and the conversion
-    const float wide = rounds(256) * (1.6f * a.kb + 14.0f), narrow = rounds(128) * (1.05f * a.kb + 9.0f);
-    if (wide < apart && wide < narrow) return tiles<256, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
-    if (narrow < apart) return tiles<128, 256, 2, 4, false, kCodes>(ctx, a, cus, 1), launched(ctx);
+    const float wide = rounds(256) * (2.6f * a.kb + 16.0f), narrow = rounds(128) * (1.55f * a.kb + 9.0f);
+    if (wide < apart && wide < narrow) return tiles<256, 256, 2, 4, true, kCodes>(ctx, a, cus, 1), launched(ctx);
+    if (narrow < apart) return tiles<128, 256, 2, 4, true, kCodes>(ctx, a, cus, 1), launched(ctx);
     a.Y = workspace, a.stride = a.rows;
     multiply_by_size<true, kHidden>(ctx, a, cus);
     if (int rc = launched(ctx)) return rc;
