@@ -79,15 +79,21 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {  // nearest, t
 // g / (1 + exp(-g)) * u, with t = exp(-|g|) <= 1: silu(g) = g / (1 + t), or
 // g t / (1 + t) below 0, so that nothing overflows and 1 + t lies in [1, 2].
 // |g| log2(e) in two parts (the second corrects t to first order), one Newton
-// step on the reciprocal: seven half steps of f32 at most, in half the time of
-// expf and a division.
+// step on the reciprocal: eight half steps of f32 at most, in half the time of
+// expf and a division. Powers of two come last: t is 2^-n times e in [0.7, 1.5]
+// and u its fraction times 2^k, so that a gate whose exp(-|g|) lies below f32's
+// range (|g| > 87) keeps its bits until u has brought the product back into it.
 __device__ __forceinline__ float silu_times(float g, float u) {
     const float a = fabsf(g), p = a * 1.44269502f;  // log2(e) = 1.44269502 + 1.92596303e-8
     const float r = fmaf(a, 1.92596303e-8f, fmaf(a, 1.44269502f, -p));
-    const float e = __builtin_amdgcn_exp2f(-p);
-    const float t = fmaf(e, fmaxf(fminf(r * -0.693147182f, 1e-3f), -1e-3f), e);  // the bounds are for infinities alone
-    const float d = 1.0f + t, y0 = __builtin_amdgcn_rcpf(d), y = fmaf(fmaf(-d, y0, 1.0f), y0, y0);
-    return g * (g >= 0.0f ? y : t * y) * u;
+    const float q = fminf(p, 1024.0f), whole = rintf(q);  // 2^-1024 brings the largest g and u to 0
+    const float near = __builtin_amdgcn_exp2f(whole - q);
+    const float e = fmaf(near, fmaxf(fminf(r * -0.693147182f, 1e-3f), -1e-3f), near);  // the bounds are for infinities alone
+    const int n = -(int)whole;
+    const float d = 1.0f + __builtin_amdgcn_ldexpf(e, n), y0 = __builtin_amdgcn_rcpf(d), y = fmaf(fmaf(-d, y0, 1.0f), y0, y0);
+    const bool below = !(g >= 0.0f);
+    const float h = g * (below ? e * y : y) * __builtin_amdgcn_frexp_mantf(u);
+    return __builtin_amdgcn_ldexpf(h, __builtin_amdgcn_frexp_expf(u) + (below ? n : 0));
 }
 
 struct Product {

@@ -63,3 +63,28 @@ def test_gate_up_scale_of_many_near_its_border(backend, tokens, cols, ff):
     p.check_f8(codes, scales, h, 8 * HALF24)
     holds = np.bincount(np.arange(ff) // 128, past) > 0
     assert np.array_equal(scales[:, : len(holds)], np.broadcast_to(np.where(holds, 138, 137), (tokens, len(holds))))
+
+
+@pytest.mark.parametrize("tokens", [3, 131, 1000, 3000])
+def test_gate_up_far_gates(backend, tokens):
+    """One product a sum: gates from -88 to -192, whose exp passes f32's range, with up to 2^121 of u so that the products
+    lie inside it and decide their blocks' scales."""
+    cols, ff = 128, 7 * 128
+    gates = {0: (-88, -96), 20: (-88, -96, -104), 60: (-96, -104, -112, -120), 100: (-104, -112, -128, -144),
+             110: (-112, -128, -144, -160), 120: (-128, -144, -160, -176), 121: (-176, -192)}
+    rng = np.random.default_rng(tokens)
+    x, g, u = np.zeros((tokens, cols)), np.zeros((ff, cols)), np.zeros((ff, cols))
+    at = np.arange(tokens) % cols
+    x[np.arange(tokens), at] = 1
+    X = matrix(x, 1, 127)
+    u[:] = rng.choice([1, 1.25, -1.75], (ff, cols))
+    scales = np.full((ff // 128, 4), 127, np.uint8)
+    for b, (k, choice) in enumerate(gates.items()):
+        g[b * 128:(b + 1) * 128] = rng.choice(choice, (128, cols))
+        scales[b, 0] = 127 + k
+    Wg, Wu = matrix(g, 128, 127), p.of_values(u, scales, 128, cols)
+    codes, got = gate_up(backend, X, Wg, Wu, tokens, cols, ff)
+    a, b = g[:, at].T, Wu[2][:, at].T
+    h = a / (1 + np.exp(-a)) * b
+    assert np.abs(h).reshape(tokens, -1, 128).max((0, 2)).min() > 2.0 ** -133  # every block has values that f32 holds
+    p.check_f8(codes, got, h, 8 * HALF24)
