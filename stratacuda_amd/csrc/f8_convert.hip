@@ -135,7 +135,10 @@ __global__ void __launch_bounds__(1024) k_f8_norm(const T *X, const float *R, co
         sum = 0.0;
         for (int i = 0; i < waves; i++) sum += s_sum[i];
     }
-    const float inv = (float)(1.0 / sqrt(sum / (double)cols + (double)eps));
+    // its power of two apart: 1 / sqrt of a row of subnormal values passes f32's range
+    const double root = 1.0 / sqrt(sum / (double)cols + (double)eps);
+    const float inv = (float)__builtin_amdgcn_frexp_mant(root);
+    const int inv_exp = __builtin_amdgcn_frexp_exp(root);
     for (int s = 0; s < steps; s++) {
         const int first = (s * waves + wave) * 256 + 4 * lane;
         if (NI == 0) {
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(1024) k_f8_norm(const T *X, const float *R, co
             if (NI == 0) f8::load4(gamma, col, cols, vec, g[i]);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                v[i][j] = col + j < cols ? v[i][j] * inv * g[i][j] : 0.0f;
+                v[i][j] = col + j < cols ? __builtin_amdgcn_ldexpf(v[i][j], inv_exp) * inv * g[i][j] : 0.0f;
                 m = fmaxf(m, f8::finite_magnitude(v[i][j]));
             }
             const uint32_t byte = f8::scale_byte(f8::half_wave_max(m));
