@@ -336,8 +336,13 @@ export class HipBackend {
     f8Matrix(rows, cols, blockRows) {
         blockRows = blockRows || 1;
         const bytes = this.addon.f8Bytes(rows, cols, blockRows), plain = {zero: false};
-        return {codes: this.allocBytes(bytes[0], 'u32', plain), scales: this.allocBytes(bytes[1], 'u32', plain), rows, cols,
-            blockRows};
+        const codes = this.allocBytes(bytes[0], 'u32', plain);
+        try {
+            return {codes, scales: this.allocBytes(bytes[1], 'u32', plain), rows, cols, blockRows};
+        } catch (e) {
+            this.free(codes);
+            throw e;
+        }
     }
     f8Owned(m, blockRows, what) {
         if (!m || m.blockRows !== blockRows) throw Error('Invalid HIP f8 ' + what);
