@@ -17,6 +17,7 @@
 // largest of 128 sums, and what is left of sums that cancel, times what is left
 // of others, is held to its own size by the codes.
 #include "f8_device.h"
+#include "f8_shapes.h"
 
 namespace {
 using namespace smi;
@@ -28,7 +29,7 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef __bf16 v2b __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 
-enum Out { kF32, kBf16, kHidden, kCodes };  // kHidden, kCodes: silu(gate) * up in f32, in 8 bits
+using namespace f8;
 
 // An operand of one block of 128 columns: the codes with their scale, or
 // (EXACT) their values in bf16, 32 columns an instruction. Which 32 columns
@@ -583,37 +584,6 @@ __global__ void __launch_bounds__(64 * W) k_f8_stream(Product a, int row_tiles, 
     }
 }
 
-// A way to share out a product: a workgroup's tokens and rows (of each matrix),
-// how many of them a CU holds, the blocks of 128 columns in a step of theirs,
-// what a step takes where a CU has one of them and where it has all, and what a
-// round over the GPU takes beside its steps, in us: fitted to whole calls on one
-// MI355X, 1 to 1024 tokens, 640 to 20,480 rows, 1280 to 10,240 columns. Over
-// those the choice is 1.5% slower than the best shape on average (to f32; to
-// bf16 1.7%, a gated pair 0.4%), 25% at worst (512 tokens, 8192 x 8192, to bf16).
-// Both sides in us, to f32: 16 x 16 against 32 x 32 for 1 token, 2560 columns to
-// 10,240 rows 5.9 and 7.0, 16 tokens, 8192 x 8192 15.0 and 13.1; 32 x 16 against
-// 16 x 16 for 32 tokens, 6144 to 2560 6.5 and 7.9; 64 x 32 against 64 x 64 for 64
-// tokens, 8192 x 8192 17.0 and 22.2, for 256 51.5 and 37.9; 32 x 64 against 64 x 64
-// for 256 tokens, 2560 to 10,240 21.2 and 22.7; 64 x 64 of streams against tiles
-// of 128 x 128 there 22.7 and 30.2. To bf16, 512 tokens: streams 26.7, tiles of
-// 64 x 64 27.2, of 256 x 128 25.3; 1024 tokens, 4096 x 4096 tiles of 64 x 64 30.6,
-// of 128 x 128 36.9.
-struct Shape {
-    int tokens, rows, resident, blocks;
-    float one, all, round;
-};
-constexpr int kShapeCount = 10;
-constexpr Shape kShapes[3][kShapeCount] = {  // by Out
-    {{16, 16, 4, 8, 0.73f, 2.56f, 0.0f}, {32, 16, 3, 8, 0.89f, 2.27f, 0.5f}, {32, 32, 2, 8, 1.18f, 2.16f, 0.7f},
-     {64, 32, 1, 8, 1.55f, 1.55f, 1.9f}, {32, 64, 3, 4, 0.78f, 2.10f, 3.7f}, {64, 64, 2, 4, 1.19f, 2.10f, 4.2f},
-     {128, 128, 2, 1, 1.15f, 1.80f, 7.0f}, {256, 128, 1, 1, 1.50f, 1.50f, 11.0f}, {256, 256, 1, 1, 2.50f, 2.50f, 11.0f}},
-    {{16, 16, 4, 8, 0.68f, 2.53f, 0.0f}, {32, 16, 3, 8, 0.88f, 2.26f, 0.0f}, {32, 32, 2, 8, 1.15f, 2.16f, 0.0f},
-     {64, 32, 1, 8, 1.50f, 1.50f, 1.0f}, {32, 64, 3, 4, 0.69f, 1.93f, 3.1f}, {64, 64, 2, 4, 0.94f, 1.83f, 3.3f},
-     {128, 128, 2, 1, 0.75f, 0.97f, 6.0f}, {256, 128, 1, 1, 0.96f, 0.96f, 4.5f}, {256, 256, 1, 1, 1.35f, 1.35f, 9.0f},
-     {64, 64, 4, 1, 0.35f, 0.85f, 3.0f}},
-    {{16, 16, 3, 8, 0.94f, 2.58f, 0.0f}, {32, 16, 2, 8, 1.14f, 2.02f, 0.4f}, {32, 32, 1, 8, 1.40f, 1.40f, 1.9f},
-     {64, 32, 2, 4, 1.12f, 2.05f, 3.3f}}};
-
 template <int W, int RR, int TT, bool EXACT, Out OUT>
 void stream(sm_ctx *ctx, const Product &a) {
     const int row_tiles = (a.rows + 16 * RR - 1) / (16 * RR), token_tiles = (a.tokens + 16 * TT - 1) / (16 * TT);
@@ -623,8 +593,7 @@ template <int BT, int BR, int WT, int WR, bool EXACT, Out OUT>
 void tiles(sm_ctx *ctx, const Product &a, int cus, int resident) {
     const int m = OUT == kCodes ? 2 : 1;
     Tiles t = {(a.tokens + BT - 1) / BT, (a.rows + BR / m - 1) / (BR / m), 0};
-    // One block of columns: nothing is left of a tile's steps to bring the next in.
-    const int n = t.tokens * t.rows, grid = (a.kb < 2 ? (n + 7) / 8 : min((n + 7) / 8, max(cus / 8, 1) * resident)) * 8;
+    const int grid = tile_grid(t.tokens * t.rows, a.kb, cus, resident);
     t.per_xcd = grid / 8;
     k_f8_tile<BT, BR, WT, WR, EXACT, OUT><<<grid, 64 * WT * WR, 0, ctx->stream>>>(a, t, aligned(a, OUT == kBf16 ? 8 : 4));
 }
@@ -634,25 +603,10 @@ int compute_units(sm_ctx *ctx) {
     return hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, ctx->device) == hipSuccess && cus > 0 ? cus : 256;
 }
 
-// The shape whose rounds over the GPU take least: its index in kShapes, and that time in us.
-int best_shape(const Product &a, Out out, int cus, float *us) {
-    int best = -1;
-    for (int i = 0; i < kShapeCount; i++) {
-        const Shape &s = kShapes[out][i];
-        if (s.tokens == 0) continue;
-        const int64_t n = (int64_t)((a.tokens + s.tokens - 1) / s.tokens) * ((a.rows + s.rows - 1) / s.rows);
-        const int64_t slots = (int64_t)cus * s.resident, over = (n % slots + cus - 1) / cus;  // workgroups of a CU in the last round
-        const int steps = (a.kb + s.blocks - 1) / s.blocks;
-        const float last = s.resident == 1 ? s.one : s.one + (s.all - s.one) * (over - 1) / (s.resident - 1);
-        const float time = n / slots * (s.all * steps + s.round) + (over ? last * steps + s.round : 0.0f);
-        if (best < 0 || time < *us) *us = time, best = i;
-    }
-    return best;
-}
 template <bool EXACT, Out OUT>
 void multiply_by_size(sm_ctx *ctx, const Product &a, int cus) {
     float us = 0.0f;
-    const int best = best_shape(a, OUT, cus, &us), resident = kShapes[OUT][best].resident;
+    const int best = best_shape(a.tokens, a.rows, a.kb, OUT, cus, &us), resident = kShapes[OUT][best].resident;
     if (best == 0) return stream<8, 1, 1, EXACT, OUT>(ctx, a);
     if (best == 1) return stream<8, 1, 2, EXACT, OUT>(ctx, a);
     if (best == 2) return stream<8, 2, 2, EXACT, OUT>(ctx, a);
@@ -669,24 +623,14 @@ void multiply_by_size(sm_ctx *ctx, const Product &a, int cus) {
     }
 }
 
-// A gated pair: sums to f32 into the workspace and the conversion of rows, or
-// one kernel whose tiles of 128 columns end in codes: 2.6 us a step and 16 us a
-// round of tiles of 256 tokens, 1.55 and 9 of 128. Fitted as above, 96 to 8192
-// tokens, 640 to 8192 columns out, 1280 to 6144 in: 0.2% slower than the best of
-// the three on average, 7% at worst. In us, of 256 tokens, of 128, apart: 4096
-// tokens, 2560 to 8192 268, 288 and 394; 1536 tokens, 2560 to 2560 63, 40 and 56;
-// 256 tokens, 2560 to 8192 61, 38 and 32.
+// A gated pair, in one kernel or two (f8_shapes.h).
 int gate_up(sm_ctx *ctx, Product &a, uint8_t *codes, uint8_t *scales, void *workspace) {
     const int cus = compute_units(ctx);
     const F8Layout L = f8_layout(a.tokens, a.rows, 1);
     a.codes = codes, a.scales = scales, a.codes_pitch = L.pitch, a.scales_pitch = L.spitch;
-    auto rounds = [&](int tokens) { return ((int64_t)((a.tokens + tokens - 1) / tokens) * (int64_t)(L.pitch / 128) + cus - 1) / cus; };
-    float apart = 0.0f;
-    best_shape(a, kHidden, cus, &apart);
-    apart += 3.0f + 5.0f * a.tokens * a.rows / 4e6f;  // and the conversion
-    const float wide = rounds(256) * (2.6f * a.kb + 16.0f), narrow = rounds(128) * (1.55f * a.kb + 9.0f);
-    if (wide < apart && wide < narrow) return tiles<256, 256, 2, 4, true, kCodes>(ctx, a, cus, 1), launched(ctx);
-    if (narrow < apart) return tiles<128, 256, 2, 4, true, kCodes>(ctx, a, cus, 1), launched(ctx);
+    const int tile = gated_tile(a.tokens, a.rows, a.kb, cus);
+    if (tile == 256) return tiles<256, 256, 2, 4, true, kCodes>(ctx, a, cus, 1), launched(ctx);
+    if (tile == 128) return tiles<128, 256, 2, 4, true, kCodes>(ctx, a, cus, 1), launched(ctx);
     a.Y = workspace, a.stride = a.rows;
     multiply_by_size<true, kHidden>(ctx, a, cus);
     if (int rc = launched(ctx)) return rc;

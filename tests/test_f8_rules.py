@@ -1,21 +1,18 @@
 """The rules that the 8-bit products' kernels go by, without a GPU: which bytes a
-load of a tile's rows may read."""
+load of a tile's rows may read, and which kernel the sizes of the GPU tests take."""
 import ctypes
-import os
-import subprocess
 
 import pytest
 
-from conftest import ROOT
+import f8_rules
+import test_gpu_f8
+import test_gpu_f8_gated
+from test_gpu_f8_tiles import GATED, TILES
 
 
 @pytest.fixture(scope="module")
 def rules(tmp_path_factory):
-    out = str(tmp_path_factory.mktemp("f8") / "f8_rules.so")
-    subprocess.run(["/opt/rocm/bin/amdclang++", "-x", "c++", "-std=c++17", "-O1", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__",
-                    "-I/opt/rocm/include", "-I" + os.path.join(ROOT, "include"), os.path.join(ROOT, "tests", "f8_rules_stub.cpp"),
-                    "-Wl,-Bsymbolic", "-o", out], check=True, capture_output=True)
-    return ctypes.CDLL(out)
+    return f8_rules.build(tmp_path_factory.mktemp("f8"))
 
 
 def readable(nbytes, scalar, at):
@@ -46,3 +43,42 @@ def test_loads_stay_in_the_matrix(rules, most, rows, pitch):
                         else:
                             assert row >= left
     assert readable(0, 128, 0)  # what a scalar offset does to a buffer of no rows
+
+
+@pytest.mark.parametrize("type,tokens,cols,rows,tile_tokens,tile_rows,tiles,steps", TILES + GATED)
+def test_sizes_take_their_tiles(rules, type, tokens, cols, rows, tile_tokens, tile_rows, tiles, steps):
+    w = f8_rules.way(rules, type, tokens, cols, rows)
+    assert w.persistent and (w.tokens, w.rows, w.tiles, w.steps) == (tile_tokens, tile_rows, tiles, steps), w
+
+
+def test_every_kernel_has_sizes(rules):
+    """Every shape of the tables is taken by a GPU test's size: shares of the columns by its lists of them, tiles by one
+    step, by several tiles of an even number of steps and by several of an odd one."""
+    to = (ctypes.c_int * 4)()
+    known = {"f32": 9, "bf16": 10, "hidden": 4}
+    tiles = {(c[0],) + c[4:6] for c in TILES + GATED}
+    streams = set()
+    for s in test_gpu_f8.SHAPES + test_gpu_f8.STREAMS + test_gpu_f8_gated.SIZES:
+        for type in ("f32", "bf16", "gated"):
+            w = f8_rules.way(rules, type, *s)
+            if not w.persistent:
+                streams.add((w.kind, w.tokens, w.rows))
+    for type, count in known.items():
+        for i in range(count):
+            rules.rule_listed(f8_rules.OUT[type], i, to)
+            assert to[0] > 0
+            shape = (type, to[0], to[1])
+            assert shape in (streams if to[3] > 1 else tiles), shape
+        if count < 10:
+            rules.rule_listed(f8_rules.OUT[type], count, to)
+            assert to[0] == 0
+    for t in tiles | {("gated", 128, 128), ("gated", 256, 128)}:
+        runs = {(c[6] > 1, c[7] == 1, c[7] % 2) for c in TILES + GATED if (c[0],) + c[4:6] == t}
+        assert {(True, False, 0), (True, False, 1)} <= runs, t
+        # f32 tiles of 256 x 128 are chosen from fourteen steps on
+        assert (False, True, 1) in runs or t == ("f32", 256, 128), t
+
+
+def test_gated_sizes(rules):
+    ways = [f8_rules.way(rules, "gated", *s) for s in test_gpu_f8_gated.SIZES]
+    assert [(w.tokens, w.rows) for w in ways] == [(16, 16), (32, 16), (128, 128), (256, 128)], ways

@@ -9,7 +9,7 @@ from test_gpu_f8 import gate_up
 
 pytestmark = pytest.mark.gpu
 
-# 16 x 16 and 64 x 32 shares of the columns, and tiles of 128 and of 256 tokens
+# 16 x 16 and 32 x 16 outputs of shared columns, and tiles of 128 and of 256 tokens
 SIZES = [(3, 300, 200), (131, 260, 1003), (1990, 384, 2000), (4000, 900, 3990)]
 
 
