@@ -290,9 +290,12 @@ int sm_f8_norm(sm_ctx *ctx, uint64_t X, int type, uint64_t R, uint64_t gamma, fl
  * type f32: Y is f32, the sums are f32's (the codes' products are exact; code
  *   times scale below 2^-126 may count as 0). R is f32, laid out like Y, 0 for
  *   none; it may be Y.
- * type bf16: Y is bf16 and R must be 0; the sums are rounded once to bf16 and
- *   their products may be cut off 2^13 below the largest of eight neighbours
- *   (about 1e-5 of the sum), for up to twice the rate.
+ * type bf16: Y is bf16 and R must be 0; for up to twice the rate the products
+ *   go through the 8-bit matrix unit, which cuts each off 2^13 below the largest
+ *   of eight neighbours. Before its one rounding to bf16 an output is off by up
+ *   to 7 * 2^-13 of the sum of its products' magnitudes: about 1e-5 of the sum
+ *   for ordinary values, but all of a sum whose large products cancel. Where
+ *   such sums matter, type f32 has them.
  * The same inputs give the same bits. An output is not finite where a code of
  * its token or row is NaN, and where a value (code * scale) or a partial sum
  * passes f32's range. */

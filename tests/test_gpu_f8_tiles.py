@@ -6,7 +6,9 @@ import pytest
 
 import f8_plain as p
 from f8_plain import HALF24
-from test_gpu_f8 import gate_up, product, put
+from test_gpu_f8 import gate_up, largest_cut, product, put
+from test_gpu_f8_gated import matrix as of_scale
+from test_gpu_f8_gated import small
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +143,20 @@ def test_same_call_same_bits(backend, type, tokens, cols, rows):
     for _ in range(2):
         again, _ = product(backend, X, W, tokens, cols, rows, type, rows, 0)
         assert np.array_equal(first, again)
+
+
+@pytest.mark.parametrize("tokens,cols,rows", [(5, 260, 200), (205, 1000, 2503), (903, 250, 8397), (1413, 380, 10948), (2068, 380, 11058)])
+def test_cancelling_products(backend, tokens, cols, rows):
+    """Two products of up to 2^17 that cancel in every eight, and whole numbers below 64 beside them: exact to f32; to
+    bf16, off by what is cut from the products, 7 * 2^-13 of their magnitudes, and one rounding."""
+    rng = np.random.default_rng(tokens)
+    x, w = small(rng, tokens, cols), small(rng, rows, cols)
+    x[:, 0:cols - 8:8], x[:, 1:cols - 8:8] = 256, -256
+    w[:, 1:cols - 8:8] = w[:, 0:cols - 8:8] = rng.choice([-448, 256, 448], (rows, len(range(0, cols - 8, 8))))
+    X, W = of_scale(x, 1, 127), of_scale(w, 128, 127)
+    want = exact(X, W).astype(np.float64)
+    got, _ = product(backend, X, W, tokens, cols, rows, "f32", rows, 0)
+    assert np.array_equal(got, want)
+    got, _ = product(backend, X, W, tokens, cols, rows, "bf16", rows, 0)
+    sums = (128 + p.blocks(cols, 128) + 8) * 2.0 ** -23 * (np.abs(X[2]) @ np.abs(W[2]).T)
+    assert np.all(np.abs(got - want) <= (sums + largest_cut(X[2], W[2])) * (1 + 2.0 ** -8) + 2.0 ** -8 * np.abs(want))
