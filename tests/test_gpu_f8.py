@@ -209,15 +209,15 @@ def test_project_residual(backend, tokens, cols, rows):
 
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 @pytest.mark.parametrize("tokens,cols,rows", [
-    (2000, 300, 2500),   # 256 x 128 tiles in one round
-    (2100, 300, 10300),  # and in three, three steps a tile: the next tile begins in the other buffer (f32: 128 x 128)
+    (2000, 300, 2500),   # tiles of 256 x 128 (f32: 128 x 128) in one round
+    (2100, 300, 10300),  # of 256 x 128 in three, three steps a tile: the next tile begins in the other buffer (f32: 256 x 256 in two)
     (2100, 3840, 9600),  # 128 x 128 tiles, two a CU, in two and a half rounds (f32 too)
-    (1000, 260, 10200),  # 256 x 256 tiles in one round
+    (1000, 260, 10200),  # 256 x 256 tiles in one round (f32 too, and in the next three)
     (5600, 300, 5800),   # and in two, three steps a tile
     (5600, 200, 5800),   # two steps
     (5600, 100, 5800),   # one step: a tile a workgroup
-    (700, 513, 2100),    # 64 x 64 tiles, two to four a CU
-    (1100, 640, 4200)])
+    (700, 513, 2100),    # 64 x 64 tiles, two to four a CU (f32: shared columns, 32 x 64)
+    (1100, 640, 4200)])  # 256 x 128 (f32: 128 x 128)
 def test_project_exact_many(backend, tokens, cols, rows, type):
     """The same over sizes that every tile takes, over several rounds; rows and tokens past the last tile's middle."""
     rng = np.random.default_rng(tokens + cols + rows)
@@ -246,7 +246,8 @@ def test_project_ordinary(backend, tokens, cols, rows, type):
     sums = (128 + p.blocks(cols, 128) + 8) * 2.0 ** -23 * (np.abs(X[2]) @ np.abs(W[2]).T)
     bound = sums if type == "f32" else sums + largest_cut(X[2], W[2]) + 2.0 ** -8 * np.abs(want)
     assert np.all(np.abs(got - want) <= bound)
-    # and on the whole: 4e-7 allows each output two steps of f32, 2^-9 / sqrt(3) is what rounding to bf16 costs
+    # and on the whole: 80 roundings (four instructions a block, 20 blocks) to f32 at random are 9 * 2^-24 = 5e-7 of an
+    # output's size, and 2e-6 allows four times that; 2^-9 / sqrt(3) is what rounding to bf16 costs
     off = np.linalg.norm(got - want) / np.linalg.norm(want)
     assert off <= (2e-6 if type == "f32" else 2.0 ** -8)
 
@@ -311,8 +312,8 @@ def gate_up(be, X, Wg, Wu, tokens, cols, ff):
     return out.read()
 
 
-# 128-token tiles in one round and two; 256-token tiles in two rounds of an odd number of steps; a hidden size that ends
-# inside a tile and its block
+# 128-token tiles in one round; 256-token tiles in one round, and in two of an even number of steps; a hidden size that
+# ends inside a tile and its block (test_gpu_f8_tiles.py has the other rounds and steps)
 FUSED = [(2000, 300, 2000), (1990, 512, 4000), (4000, 900, 3990)]
 
 
@@ -518,8 +519,8 @@ STREAMS = [  # tokens, cols, rows: workgroups of (tokens x rows; to f32, to bf16
     (70, 1290, 2503),   # 32 x 32 (gated 32 x 16)
     (17, 2500, 5003),   # gated 32 x 32
     (97, 1300, 2503),   # 64 x 32
-    (131, 260, 5003),   # 32 x 64 (gated 64 x 32)
-    (3, 6010, 10003),   # to bf16 32 x 64
+    (131, 260, 5003),   # 32 x 64 (to bf16 tiles of 64 x 64, gated 64 x 32)
+    (3, 6010, 10003),   # to bf16 32 x 64 (the others 16 x 16)
     (205, 2600, 2503)]  # 64 x 64 (gated 64 x 32)
 
 
