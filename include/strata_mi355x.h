@@ -261,10 +261,11 @@ int sm_moe_block(sm_ctx *ctx, uint64_t H, int tokens, uint64_t gamma, float eps,
  * ties to even; a value that is not finite becomes NaN.
  *
  * Buffers that a caller fills itself must keep to this: the codes past
- * `cols` are multiplied too, and 255 is no scale's byte. Every dimension is 1 to 2^21, rows * cols,
- * tokens * rows and tokens * stride at most 2^33. Outputs must not be
- * buffers that the call reads, except where an entry says so. Rows past the
- * last and words outside an output slice are left as they were.
+ * `cols` are multiplied too, and 255 is no scale's byte. Every dimension is
+ * 1 to 2^21, rows * cols, tokens * rows and tokens * stride at most 2^33.
+ * Outputs must not be buffers that the call reads, except where an entry says
+ * so. Rows past the last and words outside an output slice are left as they
+ * were.
  * Nothing is allocated and nothing waits: every entry may be captured. */
 #define SM_TYPE_F32 0
 #define SM_TYPE_BF16 1
