@@ -314,6 +314,98 @@ int sm_f8_gate_up(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int co
                   uint64_t Wu, uint64_t wu_scales, int ff, uint64_t codes, uint64_t scales, uint64_t workspace,
                   uint64_t workspace_bytes);
 
+/* -------------------------------------- attention over a 4-bit cache */
+/* A decoder's attention between its projections, over a key-value cache held
+ * in 4 bits (no reference counterpart; they stand beside strata_norm,
+ * strata_rope_position, strata_kv_append and strata_attention[_batch]).
+ *
+ * The cache is a pool of pages of SM_KV4_PAGE positions. A page holds for each
+ * key-value head a tile of 68 * pitch bytes, pitch = dim rounded up to a
+ * multiple of 64, in blocks of 32 dimensions (nb = pitch / 32):
+ *   key codes    [64 positions][pitch / 2]   dimensions 2j (low half), 2j + 1 in byte j
+ *   value codes  [nb][4 q][16 r][4 g][4 i]   position 16g + 4q + i, dimensions 32b + r (low half), 32b + 16 + r
+ *   key scales   [nb][16 n][4 g]             position 16g + n
+ *   value scales [nb][4 q][4 g][4 i]         position 16g + 4q + i
+ * A code is e2m1 (a sign, then 0, 1/2, 1, 3/2, 2, 3, 4, 6), a scale the e8m0
+ * byte of a power of two (2^(byte - 127)) for 32 dimensions of one position;
+ * value = code * scale. sm_kv4_write takes the smallest power of two from
+ * 2^-125 to 2^125 with the block's largest magnitude at most 6 scales (1 where
+ * that is 0; larger ones become 6 * 2^125) and rounds to nearest, ties to
+ * even; a block with a value that is not finite is marked by byte 255 and
+ * stands for 32 NaN. Dimensions past dim are zeros. Pools that a caller fills
+ * itself keep to this (no byte 0, 1, 253 or 254) in positions that a call
+ * reads; what lies in others does not matter.
+ *
+ * Sequences. A call has `tokens` rows. Sequence s of `count` has the rows
+ * starts[s] to starts[s + 1] - 1 (int32 [count + 1]); they are the last of its
+ * lengths[s] positions (int32 [count]), which count them in. Its positions
+ * 64 i .. 64 i + 63 lie in page table[s * table_pages + i] (int32). `longest`
+ * is at least every sequence's number of rows. These numbers are read on the
+ * GPU, so a captured graph takes those that stand there when it runs, and
+ * none can make a call leave its buffers: a sequence with starts that do not
+ * ascend within [0, tokens], with more than `longest` rows or with a length
+ * outside [0, 64 * table_pages] is left out (its rows stay as they were), a
+ * page number outside [0, pages) stands for positions that are not there, and
+ * a row before a sequence's position 0 has none. Rows of no sequence stay as
+ * they were. Tables that give two written positions the same place leave
+ * either's bytes there, or a mixture.
+ *
+ * Types are SM_TYPE_F32 or SM_TYPE_BF16, one for all tensors of a call. dim is
+ * a multiple of 8 from 8 to 256. A view is {stride, head, offset}: row t, head
+ * h, dimension d lies at t * stride + h * head + offset + d, in values; all
+ * three are >= 0, rows of an output do not overlap; 0 (no view): rows of
+ * heads of dim values. Outputs must not be buffers that the call reads.
+ * count is at most 2^15; count * table_pages, tokens * heads and pages at most
+ * 2^24.
+ * Nothing is allocated and nothing waits: every entry may be captured. */
+#define SM_KV4_PAGE 64
+
+/* Queries and keys of `tokens` rows, each head normed and turned by its row's
+ * position: n = x / sqrt(mean(x^2) + eps) * gamma, then for d < rotary / 2 and
+ * e = d + rotary / 2
+ *   y[d] = n[d] c - n[e] s,  y[e] = n[e] c + n[d] s,  c, s = Cos, Sin[position][d]
+ * and y = n from `rotary` on. Cos and Sin are f32 [context x rotary / 2] as
+ * strata_rope_table makes them, rotary even from 2 to dim; positions int32
+ * [tokens], gammas f32 [dim]. The mean is taken in f64. A position outside
+ * [0, context) makes its row's turned dimensions NaN. Yq [tokens x heads x
+ * dim] and Yk [tokens x kv_heads x dim] are without gaps. */
+int sm_qk_norm_rope(sm_ctx *ctx, uint64_t Q, const int64_t *q_view, uint64_t K, const int64_t *k_view, int type, int tokens,
+                    int heads, int kv_heads, int dim, uint64_t q_gamma, uint64_t k_gamma, float eps, uint64_t Cos,
+                    uint64_t Sin, int rotary, int context, uint64_t positions, uint64_t Yq, uint64_t Yk);
+
+/* Bytes of a pool. */
+int sm_kv4_bytes(int pages, int kv_heads, int dim, uint64_t *bytes);
+
+/* The rows' keys and values into their positions. Other positions of the
+ * pages stay as they were. */
+int sm_kv4_write(sm_ctx *ctx, uint64_t K, const int64_t *k_view, uint64_t V, const int64_t *v_view, int type, int tokens,
+                 int count, int longest, uint64_t starts, uint64_t lengths, uint64_t table, int table_pages, int kv_heads,
+                 int dim, uint64_t pool, int pages);
+
+/* The rows' positions as numbers (exact in both types); 0 for a position that
+ * is not there. */
+int sm_kv4_read(sm_ctx *ctx, uint64_t pool, int pages, int kv_heads, int dim, int tokens, int count, int longest,
+                uint64_t starts, uint64_t lengths, uint64_t table, int table_pages, uint64_t K, const int64_t *k_view,
+                uint64_t V, const int64_t *v_view, int type);
+
+/* For the row of position p: Y = softmax over t of (scale * q . k_t) times
+ * v_t, over the positions t <= p that are there, t > p - window where window
+ * is not 0; times sigmoid(G) where G is not 0. heads is a multiple of
+ * kv_heads; key-value head h serves the heads from h * heads / kv_heads on.
+ * scale is finite and > 0. Rows that have no position, or only scores of
+ * -infinity, are 0. What positions outside a row's range hold does not count,
+ * whatever it is. Sums and the softmax are in f32; for bf16 the probabilities
+ * are rounded to bf16, for f32 nothing is rounded to fewer bits. Y [tokens x
+ * heads x dim] is without gaps. The same inputs give the same bits. The
+ * workspace holds sm_kv4_attention_workspace(...) bytes (0 where that is 0);
+ * a call leaves nothing in it that a later call needs. */
+int sm_kv4_attention_workspace(int tokens, int count, int longest, int table_pages, int heads, int kv_heads, int dim,
+                               uint64_t *bytes);
+int sm_kv4_attention(sm_ctx *ctx, uint64_t Q, const int64_t *q_view, int type, int tokens, int count, int longest,
+                     uint64_t starts, uint64_t lengths, uint64_t table, int table_pages, uint64_t pool, int pages, int heads,
+                     int kv_heads, int dim, float scale, int window, uint64_t G, const int64_t *g_view, uint64_t Y,
+                     uint64_t workspace, uint64_t workspace_bytes);
+
 /* ---------------------------------------------------------------- timing */
 /* Events on the context's stream (the stream every launch above uses). */
 int sm_event_record(sm_ctx *ctx, int slot);          /* slot in [0, 64) */

@@ -9,6 +9,7 @@ points (``moe_layer``, ``moe_route``, ``moe_dispatch``) run the whole stage on
 the device. There is no CPU fallback: without the built library or a GPU the
 constructor raises.
 """
+import collections
 import ctypes
 import json
 import os
@@ -47,7 +48,7 @@ def lib():
             raise RuntimeError("libstrata_mi355x.so is not built; run __graft_entry__.build()")
         L = ctypes.CDLL(LIB_PATH)
         u64, i, vp = ctypes.c_uint64, ctypes.c_int, ctypes.c_void_p
-        pu64 = ctypes.POINTER(ctypes.c_uint64)
+        pu64, view = ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_int64)
         sig = {
             "sm_init": (i, [i, ctypes.POINTER(vp)]),
             "sm_shutdown": (None, [vp]),
@@ -96,6 +97,14 @@ def lib():
             "sm_f8_project": (i, [vp, u64, u64, i, i, u64, u64, i, u64, u64, i, ctypes.c_int64, ctypes.c_int64]),
             "sm_f8_gate_up_workspace": (i, [i, i, pu64]),
             "sm_f8_gate_up": (i, [vp, u64, u64, i, i, u64, u64, u64, u64, i, u64, u64, u64, u64]),
+            "sm_qk_norm_rope": (i, [vp, u64, view, u64, view, i, i, i, i, i, u64, u64, ctypes.c_float, u64, u64, i, i, u64,
+                                    u64, u64]),
+            "sm_kv4_bytes": (i, [i, i, i, pu64]),
+            "sm_kv4_write": (i, [vp, u64, view, u64, view, i, i, i, i, u64, u64, u64, i, i, i, u64, i]),
+            "sm_kv4_read": (i, [vp, u64, i, i, i, i, i, i, u64, u64, u64, i, u64, view, u64, view, i]),
+            "sm_kv4_attention_workspace": (i, [i, i, i, i, i, i, i, pu64]),
+            "sm_kv4_attention": (i, [vp, u64, view, i, i, i, i, u64, u64, u64, i, u64, i, i, i, i, ctypes.c_float, i, u64,
+                                     view, u64, u64, u64]),
             "sm_prefetch_router": (i, [vp, ctypes.c_uint64, i, i]),
         }
         for name, (res, args) in sig.items():
@@ -138,6 +147,11 @@ class Buffer:
 
     def __repr__(self):
         return "Buffer(0x%x, %d bytes, %s)" % (self.handle, self.nbytes, self.type)
+
+
+Sequences = collections.namedtuple("Sequences", "count tokens longest starts lengths table table_pages")
+Sequences.__doc__ = """The sequences of a call over a 4-bit cache (include/strata_mi355x.h): `count` of them with `tokens`
+rows in all and at most `longest` each; int32 buffers starts [count + 1], lengths [count] and table [count x table_pages]."""
 
 
 class Backend:
@@ -397,6 +411,64 @@ class Backend:
         self._check(lib().sm_f8_gate_up(self._ctx, X.handle, x_scales.handle, tokens, cols, Wg.handle, wg_scales.handle,
                                         Wu.handle, wu_scales.handle, ff, codes.handle, scales.handle, workspace.handle,
                                         workspace.nbytes))
+
+    # -------------------------------- attention over a 4-bit cache
+    # include/strata_mi355x.h has the cache's layout. A view is (stride, head,
+    # offset) in values, None: rows of heads of dim values without gaps.
+    @staticmethod
+    def _view(view):
+        return None if view is None else (ctypes.c_int64 * 3)(*view)
+
+    def qk_norm_rope(self, Q, K, tokens, heads, kv_heads, dim, q_gamma, k_gamma, eps, Cos, Sin, rotary, context, positions,
+                     Yq, Yk, q_view=None, k_view=None, type="f32"):
+        """Each head of Q and K normed, then turned by its row's position."""
+        self._check(lib().sm_qk_norm_rope(self._ctx, Q.handle, self._view(q_view), K.handle, self._view(k_view),
+                                          self._f8_type(type), tokens, heads, kv_heads, dim, q_gamma.handle, k_gamma.handle,
+                                          eps, Cos.handle, Sin.handle, rotary, context, positions.handle, Yq.handle,
+                                          Yk.handle))
+
+    @staticmethod
+    def kv4_bytes(pages, kv_heads, dim):
+        """Bytes of a pool of pages."""
+        n = ctypes.c_uint64()
+        rc = lib().sm_kv4_bytes(pages, kv_heads, dim, ctypes.byref(n))
+        if rc != SM_OK:
+            raise ArgumentError(rc, "invalid kv4 pool")
+        return n.value
+
+    def kv4_write(self, K, V, sequences, pool, pages, kv_heads, dim, k_view=None, v_view=None, type="f32"):
+        """The rows' keys and values into the last positions of their sequences."""
+        q = sequences
+        self._check(lib().sm_kv4_write(self._ctx, K.handle, self._view(k_view), V.handle, self._view(v_view),
+                                       self._f8_type(type), q.tokens, q.count, q.longest, q.starts.handle, q.lengths.handle,
+                                       q.table.handle, q.table_pages, kv_heads, dim, pool.handle, pages))
+
+    def kv4_read(self, pool, pages, kv_heads, dim, sequences, K, V, k_view=None, v_view=None, type="f32"):
+        """The last positions of the sequences, as many as they have rows, as numbers."""
+        q = sequences
+        self._check(lib().sm_kv4_read(self._ctx, pool.handle, pages, kv_heads, dim, q.tokens, q.count, q.longest,
+                                      q.starts.handle, q.lengths.handle, q.table.handle, q.table_pages, K.handle,
+                                      self._view(k_view), V.handle, self._view(v_view), self._f8_type(type)))
+
+    @staticmethod
+    def kv4_attention_workspace_bytes(sequences, heads, kv_heads, dim):
+        """Bytes of the workspace; 0: none is needed."""
+        q, n = sequences, ctypes.c_uint64()
+        rc = lib().sm_kv4_attention_workspace(q.tokens, q.count, q.longest, q.table_pages, heads, kv_heads, dim,
+                                              ctypes.byref(n))
+        if rc != SM_OK:
+            raise ArgumentError(rc, "invalid kv4 attention geometry")
+        return n.value
+
+    def kv4_attention(self, Q, sequences, pool, pages, heads, kv_heads, dim, scale, Y, workspace=None, window=0, gate=None,
+                      q_view=None, gate_view=None, type="f32"):
+        """Y = softmax(scale * Q . keys) . values over each row's positions, times sigmoid(gate)."""
+        q = sequences
+        self._check(lib().sm_kv4_attention(self._ctx, Q.handle, self._view(q_view), self._f8_type(type), q.tokens, q.count,
+                                           q.longest, q.starts.handle, q.lengths.handle, q.table.handle, q.table_pages,
+                                           pool.handle, pages, heads, kv_heads, dim, scale, window,
+                                           gate.handle if gate else 0, self._view(gate_view if gate else None), Y.handle,
+                                           workspace.handle if workspace else 0, workspace.nbytes if workspace else 0))
 
     # ------------------------------------------------------------ timing
     STAGES = ["decode_route", "decode_gate_up", "decode_down_combine", "prefill_route", "prefill_dispatch",

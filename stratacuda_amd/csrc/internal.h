@@ -282,6 +282,44 @@ uint64_t f8_gate_up_workspace(int tokens, int ff);
 int f8_gate_up_launch(sm_ctx *ctx, const F8Operand &X, int tokens, int cols, const F8Operand &Wg, const F8Operand &Wu, int ff,
                       uint8_t *codes, uint8_t *scales, void *workspace);
 
+// ------------------------------------------- attention over a 4-bit cache
+// Where row t, head h, dimension d of a tensor lies: t * stride + h * head +
+// offset + d, in values.
+struct Kv4View {
+    int64_t stride, head, offset;
+    bool multiple_of(int n) const { return stride % n == 0 && head % n == 0 && offset % n == 0; }
+};
+struct Kv4Sequences {
+    int count, tokens, longest, table_pages;
+    const int *starts, *lengths, *table;
+};
+inline int kv4_pitch(int dim) { return (dim + 63) / 64 * 64; }
+inline uint64_t kv4_page_bytes(int heads, int dim) { return (uint64_t)heads * 68 * kv4_pitch(dim); }
+struct QkNormRope {
+    int tokens, heads, kv_heads, dim, rotary, context;
+    float eps;
+    const float *q_gamma, *k_gamma, *cos, *sin;
+    const int *positions;
+    Kv4View q_view, k_view;
+};
+struct Kv4Attention {
+    Kv4Sequences q;
+    int pages, heads, kv_heads, dim, window;  // window 0: none
+    float scale_log2;                         // the scores' scale for powers of two
+    Kv4View q_view, g_view;
+    bool vec;           // queries lie aligned to 16 bytes
+    int pieces, least;  // the launcher's: how many pieces of the context, of how many pages at least
+};
+// Unchecked launchers on raw device pointers (kv4_cache.hip, kv4_attention.hip).
+int qk_norm_rope_launch(sm_ctx *ctx, const QkNormRope &a, const void *Q, const void *K, void *Yq, void *Yk, bool bf16);
+int kv4_write_launch(sm_ctx *ctx, const void *K, const Kv4View &kv, const void *V, const Kv4View &vv, bool bf16,
+                     const Kv4Sequences &q, int heads, int dim, uint8_t *pool, int pages);
+int kv4_read_launch(sm_ctx *ctx, const uint8_t *pool, int pages, int heads, int dim, const Kv4Sequences &q, void *K,
+                    const Kv4View &kv, void *V, const Kv4View &vv, bool bf16);
+uint64_t kv4_attention_workspace(const Kv4Sequences &q, int heads, int kv_heads, int dim);
+int kv4_attention_launch(sm_ctx *ctx, const Kv4Attention &a, const void *Q, const uint8_t *pool, const void *G, void *Y, bool bf16,
+                         void *workspace);
+
 // ------------------------------------------------ kernels by name (sm_run)
 // One 64-bit slot per reference parameter: a buffer handle, or the int32 /
 // float32 bit pattern in the low 32 bits.

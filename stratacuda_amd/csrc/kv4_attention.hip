@@ -1,0 +1,527 @@
+// Attention over a key-value cache held in 4 bits.
+//
+// For a query q of the sequence's position p and the positions t in
+// (p - window, p]: s_t = scale q . k_t, y = sum_t e^(s_t - m) v_t / sum_t
+// e^(s_t - m), one pass with the running maximum m; y * sigmoid(gate) where
+// there is a gate. A row with no position gives 0.
+//
+// What a code and its scale stand for has two significant bits, so it is exact
+// in bf16: keys and values go to the bf16 matrix units without a rounding.
+// Queries of bf16 do too; those of f32 and their probabilities are taken as
+// the sum of three bf16 numbers (8 significant bits each, so all 24) and cost
+// three matrix instructions. For bf16 the probabilities are rounded to bf16,
+// half a step of 2^-8 relative, like the result; sums are f32's.
+#include "kv4_device.h"
+
+namespace {
+using namespace smi;
+using kv4::bf16x2;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+constexpr float kNone = -INFINITY;
+
+__device__ __forceinline__ bf16x8 as_bf16(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
+__device__ __forceinline__ uint32_t bits(bf16x2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+// Three bf16 numbers whose sum is v: each the rounding of what is left, which
+// the subtraction gives exactly.
+__device__ __forceinline__ void three_parts(float a, float b, uint32_t part[3]) {
+    part[0] = kv4::bf16_pair(a, b);
+    const float a1 = a - __uint_as_float(part[0] << 16), b1 = b - __uint_as_float(part[0] & 0xffff0000u);
+    part[1] = kv4::bf16_pair(a1, b1);
+    part[2] = kv4::bf16_pair(a1 - __uint_as_float(part[1] << 16), b1 - __uint_as_float(part[1] & 0xffff0000u));
+}
+
+// The larger of a lane's value and those of the lanes 16, 32 and 48 away.
+__device__ __forceinline__ float max_of_quarters(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_of_quarters(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// ---------------------------------------------------------------- the shares
+// A sequence's pages are cut into pieces of equally many pages; piece number
+// `slot` of all sequences' is a workgroup's. A sequence with rows has one
+// piece at least.
+struct Piece {
+    int s, first, end;  // the sequence and the pages; s = -1: there is no such piece
+    int number, count;  // which of the sequence's pieces it is
+};
+// The pages that the sequence's rows reach.
+__device__ __forceinline__ int2 pages_of(const kv4::Span &a, int window) {
+    const int first = a.length - a.n;
+    const int lo = window > 0 ? max(first - window + 1, 0) / 64 : 0;
+    return make_int2(lo, max((a.length + 63) / 64, lo));
+}
+__device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int least, int slot) {
+    const int lane = threadIdx.x % 64;
+    int total = 0;
+    for (int at = 0; at < q.count; at += 64) {
+        int n = 0;
+        if (at + lane < q.count) {
+            const kv4::Span a = kv4::span(q, at + lane);
+            const int2 p = pages_of(a, window);
+            n = a.n > 0 ? p.y - p.x : 0;
+        }
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) n += __shfl_xor(n, i, 64);
+        total += n;
+    }
+    const int each = max(least, (total + pieces - 1) / pieces);
+    int before = 0;
+    for (int at = 0; at < q.count; at += 64) {
+        int n = 0;
+        int2 p = make_int2(0, 0);
+        if (at + lane < q.count) {
+            const kv4::Span a = kv4::span(q, at + lane);
+            p = pages_of(a, window);
+            n = a.n > 0 ? max((p.y - p.x + each - 1) / each, 1) : 0;
+        }
+        int upto = n;  // with this lane's
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) {
+            const int other = __shfl_up(upto, i, 64);
+            if (lane >= i) upto += other;
+        }
+        const uint64_t past = __ballot(before + upto > slot);
+        if (past) {
+            const int who = __ffsll((unsigned long long)past) - 1;
+            const int count = __shfl(n, who, 64), number = slot - before - (__shfl(upto, who, 64) - count);
+            const int first = __shfl(p.x, who, 64), end = __shfl(p.y, who, 64);
+            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count};
+        }
+        before += __shfl(upto, 63, 64);
+    }
+    return {-1, 0, 0, 0, 0};
+}
+
+// ------------------------------------------------------------------ 16 rows
+// One workgroup: 16 rows (a token's heads of one key-value head, then the next
+// token's) over one piece of the sequence, whose pages its four waves take in
+// turn. Both products are transposed, S^T = K Q^T and O^T = V^T P^T: a lane
+// holds one row's scores of 4 positions out of 16, which is what it brings to
+// the second product, and every row's maximum and sum lie in its own lanes.
+// Codes go from memory into registers: 16 bytes a lane are 32 dimensions of
+// one key (its block: one scale), or two dimensions of 16 positions' values.
+// The next page's keys are on their way while this one's probabilities are
+// made, its values during the products.
+template <int NC, bool F32>
+struct Rows16 {
+    static constexpr int kPitch = 64 * NC, kBlocks = 2 * NC;
+    static constexpr bool kWide = NC % 2 == 0;            // 16 bytes of a key a load; else 8
+    static constexpr int kChunks = kWide ? NC / 2 : NC;   // loads of a key
+    static constexpr int kSteps = kWide ? 4 : 2;          // matrix steps of 32 dimensions of each
+    static constexpr int kParts = F32 ? 3 : 1;
+
+    struct Keys {
+        uint32_t codes[4][kChunks][kSteps];  // of positions 16 g + lane % 16
+        uint32_t scales[kChunks];            // a byte for each g
+    };
+    struct Values {
+        u32x4 codes[kBlocks], scales[kBlocks];
+    };
+    static __device__ __forceinline__ void load(Keys &k, const uint8_t *tile, int lane) {
+        const int n = lane % 16, kq = lane / 16;
+#pragma unroll
+        for (int c = 0; c < kChunks; c++) {
+            const int block = kWide ? 4 * c + kq : 2 * c + kq / 2;
+            k.scales[c] = *(const uint32_t *)(tile + kv4::key_scales(kPitch) + block * 64 + n * 4);
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const uint8_t *p = tile + (16 * g + n) * (kPitch / 2) + (4 * kSteps) * (4 * c + kq);
+                if constexpr (kWide) {
+                    const u32x4 v = *(const u32x4 *)p;
+                    k.codes[g][c][0] = v[0], k.codes[g][c][1] = v[1], k.codes[g][c][2] = v[2], k.codes[g][c][3] = v[3];
+                } else {
+                    const uint2 v = *(const uint2 *)p;
+                    k.codes[g][c][0] = v.x, k.codes[g][c][1] = v.y;
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ void load(Values &v, const uint8_t *tile, int lane) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; b++) {
+            v.codes[b] = *(const u32x4 *)(tile + kv4::value_codes(kPitch) + b * 1024 + lane * 16);
+            v.scales[b] = *(const u32x4 *)(tile + kv4::value_scales(kPitch) + b * 64 + lane / 16 * 16);
+        }
+    }
+    // The query's part of step (c, s): dimensions as the keys' loads have them.
+    static __device__ __forceinline__ int dimension(int c, int s, int kq) { return 8 * kSteps * (4 * c + kq) + 8 * s; }
+};
+
+// The byte i of w as a scale operand: the conversions take the exponent field
+// alone, so what else the word brings along does not count.
+__device__ __forceinline__ float scale_at(uint32_t w, int i) {
+    return __uint_as_float(i == 0 ? w << 23 : i == 1 ? w << 15 : i == 2 ? w << 7 : w >> 1);
+}
+// Eight codes, of dimension 2 j and 2 j + 1 in byte j, as bf16.
+__device__ __forceinline__ u32x4 eight(uint32_t w, float scale) {
+    return u32x4{bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)), bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                 bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)), bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+}
+// Four positions of two dimensions (a byte each, with its scale) as two
+// registers of the lower dimension and two of the upper one.
+__device__ __forceinline__ void four(uint32_t w, uint32_t scales, uint32_t low[2], uint32_t high[2]) {
+    const uint32_t a = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale_at(scales, 0), 0));
+    const uint32_t b = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale_at(scales, 1), 1));
+    const uint32_t c = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale_at(scales, 2), 2));
+    const uint32_t d = bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale_at(scales, 3), 3));
+    low[0] = __builtin_amdgcn_perm(b, a, 0x05040100u), low[1] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    high[0] = __builtin_amdgcn_perm(b, a, 0x07060302u), high[1] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
+template <int NC, typename T>
+__global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, const uint8_t *pool, const T *G, T *Y, float *parts,
+                                                  float2 *stats, int tiles) {
+    constexpr bool F32 = sizeof(T) == 4;
+    using R = Rows16<NC, F32>;
+    constexpr int kPitch = R::kPitch, kTiles = kPitch / 16, kLine = kPitch + 4;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n16 = lane % 16, kq = lane / 16;
+    const Piece piece = piece_of(a.q, a.window, a.pieces, a.least, blockIdx.y);
+    if (piece.s < 0) return;
+    const kv4::Span span = kv4::span(a.q, piece.s);
+    const int head = blockIdx.x / tiles, tile = blockIdx.x % tiles, group = a.heads / a.kv_heads;
+    const int rows = span.n * group - 16 * tile;  // of the sequence, from this tile's first on
+    if (rows <= 0) return;
+    const int first = span.length - span.n;       // the first new token's position
+
+    // this lane's row, the last one's once more past it; its positions lo .. hi
+    const int row = 16 * tile + min(n16, rows - 1), token = row / group, hq = head * group + row % group;
+    const int hi = first + token, lo = a.window > 0 ? max(hi - a.window + 1, 0) : 0;
+    // the tile's: those that any row has, and that all rows have
+    const int last = first + (16 * tile + min(15, rows - 1)) / group, early = first + 16 * tile / group;
+    const int any_lo = a.window > 0 ? max(early - a.window + 1, 0) : 0, all_lo = a.window > 0 ? max(last - a.window + 1, 0) : 0;
+    const int begin = max(piece.first, any_lo / 64), end = min(piece.end, (last >> 6) + 1);
+
+    // queries
+    uint32_t q[R::kParts][R::kChunks][R::kSteps][4];
+    {
+        const T *x = Q + (int64_t)(span.row + token) * a.q_view.stride + hq * a.q_view.head + a.q_view.offset;
+#pragma unroll
+        for (int c = 0; c < R::kChunks; c++)
+#pragma unroll
+            for (int s = 0; s < R::kSteps; s++) {
+                const int d = R::dimension(c, s, kq);
+                float v[8] = {};
+                if (d < a.dim) kv4::load8(x + d, a.vec, v);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (F32) {
+                        uint32_t part[3];
+                        three_parts(v[2 * j], v[2 * j + 1], part);
+#pragma unroll
+                        for (int t = 0; t < 3; t++) q[t][c][s][j] = part[t];
+                    } else {
+                        q[0][c][s][j] = kv4::bf16_pair(v[2 * j], v[2 * j + 1]);
+                    }
+                }
+            }
+    }
+
+    f32x4 o[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; t++) o[t] = f32x4{0, 0, 0, 0};
+    float m = kNone, sum = 0.0f;  // the row's maximum (times scale_log2); this lane's share of its sum
+
+    typename R::Keys keys;
+    typename R::Values values;
+    const int64_t step = (int64_t)a.kv_heads * (68 * kPitch);
+    const uint8_t *base = pool + (int64_t)head * (68 * kPitch);
+    int at = begin + wave, page = at < end ? kv4::page_of(a.q, piece.s, at, a.pages) : -1;
+    if (at < end) {
+        R::load(keys, base + max(page, 0) * step, lane);
+        R::load(values, base + max(page, 0) * step, lane);
+    }
+    for (; at < end; at += 4) {
+        // S^T: positions 16 g + 4 kq + i of row n16
+        f32x4 s[4];
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            s[g] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < R::kChunks; c++) {
+                const float scale = scale_at(keys.scales[c], g);
+#pragma unroll
+                for (int t = 0; t < R::kSteps; t++) {
+                    const bf16x8 k = as_bf16(eight(keys.codes[g][c][t], scale));
+#pragma unroll
+                    for (int p = R::kParts - 1; p >= 0; p--)
+                        s[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            k, as_bf16(u32x4{q[p][c][t][0], q[p][c][t][1], q[p][c][t][2], q[p][c][t][3]}), s[g], 0, 0, 0);
+                }
+            }
+        }
+        const int now = page, next = at + 4;
+        if (next < end) {
+            page = kv4::page_of(a.q, piece.s, next, a.pages);
+            R::load(keys, base + max(page, 0) * step, lane);
+        }
+        const int p0 = 64 * at;
+        const bool edge = now < 0 || p0 < all_lo || p0 + 63 > early;  // a position that some row does not have
+        bool poisoned = false;
+        if (edge) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                uint32_t kept = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = p0 + 16 * g + 4 * kq + i;
+                    if (now < 0 || t < lo || t > hi) s[g][i] = kNone;
+                    if (now >= 0 && t >= any_lo && t <= last) kept |= 255u << (8 * i);
+                }
+                // values that no row has may be anything: their scales count as 1, and 0 times their codes is 0
+#pragma unroll
+                for (int b = 0; b < R::kBlocks; b++) values.scales[b][g] = (values.scales[b][g] & kept) | (0x7f7f7f7fu & ~kept);
+            }
+            // a block of NaN that some rows have and others do not
+#pragma unroll
+            for (int b = 0; b < R::kBlocks; b++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) poisoned |= (values.scales[b][g] >> (8 * i) & 255u) == 255u;
+            poisoned = __any(poisoned);
+        }
+        float top = kNone;
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) top = fmaxf(top, s[g][i]);
+        top = max_of_quarters(top) * a.scale_log2;
+        // the maximum is raised once scores pass it by 2^8: any number near it does
+        if (__any(top > m + 8.0f || (m == kNone && top > kNone))) {
+            const float to = fmaxf(m, top), by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            sum *= by;
+#pragma unroll
+            for (int t = 0; t < kTiles; t++) o[t] *= by;
+        }
+        const float from = m == kNone ? 0.0f : -m;
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], a.scale_log2, from));
+                sum += s[g][i];
+            }
+        uint32_t poison = 0;  // bit b: a block b of NaN at a position that the row has
+        if (poisoned) {
+#pragma unroll
+            for (int b = 0; b < R::kBlocks; b++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int t = p0 + 16 * g + 4 * kq + i;
+                        uint32_t any = (values.scales[b][g] >> (8 * i) & 255u) == 255u;
+                        if (!any) continue;
+                        values.scales[b][g] ^= 0x80u << (8 * i);
+                        // the scales are those of this quarter's positions, the same in its 16 lanes: each its own row
+                        if (t >= lo && t <= hi) poison |= 1u << b;
+                    }
+            poison |= __shfl_xor(poison, 16, 64);
+            poison |= __shfl_xor(poison, 32, 64);
+        }
+        // O^T: dimensions 16 t + 4 kq + i of row n16
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+            u32x4 p[R::kParts];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float x = s[2 * ks + j / 2][2 * (j % 2)], y = s[2 * ks + j / 2][2 * (j % 2) + 1];
+                if constexpr (F32) {
+                    uint32_t part[3];
+                    three_parts(x, y, part);
+#pragma unroll
+                    for (int t = 0; t < 3; t++) p[t][j] = part[t];
+                } else {
+                    p[0][j] = kv4::bf16_pair(x, y);
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < R::kBlocks; b++) {
+                uint32_t low[4], high[4];
+                four(values.codes[b][2 * ks], values.scales[b][2 * ks], low, high);
+                four(values.codes[b][2 * ks + 1], values.scales[b][2 * ks + 1], low + 2, high + 2);
+                const bf16x8 vl = as_bf16(u32x4{low[0], low[1], low[2], low[3]}),
+                             vh = as_bf16(u32x4{high[0], high[1], high[2], high[3]});
+#pragma unroll
+                for (int t = R::kParts - 1; t >= 0; t--) {
+                    o[2 * b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vl, as_bf16(p[t]), o[2 * b], 0, 0, 0);
+                    o[2 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vh, as_bf16(p[t]), o[2 * b + 1], 0, 0, 0);
+                }
+            }
+        }
+        if (poison) {
+#pragma unroll
+            for (int b = 0; b < R::kBlocks; b++)
+                if (poison >> b & 1) o[2 * b] = o[2 * b + 1] = f32x4{NAN, NAN, NAN, NAN};
+        }
+        if (next < end) R::load(values, base + max(page, 0) * step, lane);
+    }
+
+    // the four waves' sums meet
+    __shared__ float s_o[4][16][kLine], s_m[4][16], s_sum[4][16];
+    sum = sum_of_quarters(sum);
+#pragma unroll
+    for (int t = 0; t < kTiles; t++) *(f32x4 *)&s_o[wave][n16][16 * t + 4 * kq] = o[t];
+    if (kq == 0) s_m[wave][n16] = m, s_sum[wave][n16] = sum;
+    __syncthreads();
+    const int r = threadIdx.x / 16, d0 = threadIdx.x % 16 * 4;
+    if (r >= rows) return;
+    float by[4], top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r])), all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        by[w] = s_m[w][r] == kNone ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][r] - top);
+        // a sum that is not a number, of scores that are none, stays one
+        all += s_m[w][r] == kNone ? (s_sum[w][r] == 0.0f ? 0.0f : NAN) : s_sum[w][r] * by[w];
+    }
+    const int64_t part = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16 + r;
+    const int tok = (16 * tile + r) / group, h = head * group + (16 * tile + r) % group;
+    const int64_t out = ((int64_t)(span.row + tok) * a.heads + h) * a.dim;
+    const T *g = G ? G + (int64_t)(span.row + tok) * a.g_view.stride + h * a.g_view.head + a.g_view.offset : nullptr;
+#pragma unroll
+    for (int d = d0; d < kPitch; d += 64) {
+        f32x4 v = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; w++) v += *(f32x4 *)&s_o[w][r][d] * by[w];
+        if (piece.count > 1) {
+            *(f32x4 *)(parts + part * kPitch + d) = v;
+        } else {
+            const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (d + i < a.dim) {
+                    float y = all == 0.0f ? 0.0f : v[i] * inv;
+                    if (g) y = y / (1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * kv4::value(g[d + i])));
+                    kv4::store1(Y + out + d + i, y);
+                }
+        }
+    }
+    if (piece.count > 1 && d0 == 0) stats[part] = make_float2(top, all);
+}
+
+// The pieces of one row joined: its sequence's partial sums, each brought to
+// the largest of their maxima.
+template <typename T>
+__global__ void __launch_bounds__(256) k_kv4_join(Kv4Attention a, const T *G, T *Y, const float *parts, const float2 *stats,
+                                                  int tiles, int pitch) {
+    const int s = blockIdx.y, group = a.heads / a.kv_heads;
+    const kv4::Span span = kv4::span(a.q, s);
+    const int token = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
+    if (token >= span.n) return;
+    // this sequence's first piece: as the rows' kernel counts them
+    const int lane = threadIdx.x % 64;
+    int total = 0, before = 0, count = 0;
+    for (int at = 0; at < a.q.count; at += 64) {
+        int n = 0;
+        if (at + lane < a.q.count) {
+            const kv4::Span o = kv4::span(a.q, at + lane);
+            const int2 p = pages_of(o, a.window);
+            n = o.n > 0 ? p.y - p.x : 0;
+        }
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) n += __shfl_xor(n, i, 64);
+        total += n;
+    }
+    const int each = max(a.least, (total + a.pieces - 1) / a.pieces);
+    for (int at = 0; at <= s; at += 64) {
+        int n = 0;
+        if (at + lane <= s) {
+            const kv4::Span o = kv4::span(a.q, at + lane);
+            const int2 p = pages_of(o, a.window);
+            n = o.n > 0 ? max((p.y - p.x + each - 1) / each, 1) : 0;
+        }
+        if (s - at < 64) count = __shfl(n, s - at, 64);
+        if (at + lane == s) n = 0;
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) n += __shfl_xor(n, i, 64);
+        before += n;
+    }
+    if (count <= 1) return;
+    const int head = h / group, row = token * group + h % group;
+    const int64_t base = ((int64_t)head * tiles + row / 16) * 16 + row % 16, step = (int64_t)a.kv_heads * tiles * 16;
+    float top = kNone, all = 0.0f;
+    for (int c = 0; c < count; c++) top = fmaxf(top, stats[base + (before + c) * step].x);
+    const int64_t out = ((int64_t)(span.row + token) * a.heads + h) * a.dim;
+    const T *g = G ? G + (int64_t)(span.row + token) * a.g_view.stride + h * a.g_view.head + a.g_view.offset : nullptr;
+    float v = 0.0f;
+    const int d = threadIdx.x;
+    if (d >= pitch) return;
+    for (int c = 0; c < count; c++) {
+        const float2 st = stats[base + (before + c) * step];
+        const float by = st.x == kNone ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
+        all += st.x == kNone ? (st.y == 0.0f ? 0.0f : NAN) : st.y * by;
+        v += parts[(base + (before + c) * step) * pitch + d] * by;
+    }
+    if (d >= a.dim) return;
+    float y = all == 0.0f ? 0.0f : v / all;
+    if (g) y = y / (1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * kv4::value(g[d])));
+    kv4::store1(Y + out + d, y);
+}
+
+// Workgroups that fill the GPU, and the least pages that are worth a piece.
+constexpr int kWorkgroups = 512, kLeast = 4;
+
+struct Shape {
+    int tiles, pieces;
+    uint64_t slots, part_bytes, bytes;
+};
+Shape shape_of(const Kv4Sequences &q, int heads, int kv_heads, int dim) {
+    Shape s;
+    s.tiles = (int)(((int64_t)q.longest * (heads / kv_heads) + 15) / 16);
+    const int64_t each = (int64_t)kv_heads * s.tiles, most = (int64_t)q.count * ((q.table_pages + kLeast - 1) / kLeast);
+    int64_t pieces = (kWorkgroups + each - 1) / each;
+    if (pieces > most) pieces = most;
+    s.pieces = pieces < 1 ? 1 : (int)pieces;
+    s.slots = (uint64_t)(s.pieces > 1 ? s.pieces + q.count : q.count);
+    s.part_bytes = s.pieces > 1 ? s.slots * each * 16 * kv4_pitch(dim) * 4 : 0;
+    s.bytes = s.pieces > 1 ? s.part_bytes + s.slots * each * 16 * 8 : 0;
+    return s;
+}
+
+template <typename T>
+void launch(sm_ctx *ctx, Kv4Attention a, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
+    const Shape s = shape_of(a.q, a.heads, a.kv_heads, a.dim);
+    const int pitch = kv4_pitch(a.dim);
+    // one piece a sequence: as large as any
+    a.pieces = s.pieces, a.least = s.pieces > 1 ? kLeast : a.q.table_pages + 1;
+    float *parts = (float *)workspace;
+    float2 *stats = (float2 *)((char *)workspace + s.part_bytes);
+    const dim3 grid((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots);
+    switch (pitch / 64) {
+        case 1: k_kv4_rows<1, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles); break;
+        case 2: k_kv4_rows<2, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles); break;
+        case 3: k_kv4_rows<3, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles); break;
+        default: k_kv4_rows<4, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles); break;
+    }
+    if (s.pieces > 1)
+        k_kv4_join<T><<<dim3((uint32_t)a.q.longest * a.heads, a.q.count), 256, 0, ctx->stream>>>(a, G, Y, parts, stats, s.tiles, pitch);
+}
+
+}  // namespace
+
+namespace smi {
+
+uint64_t kv4_attention_workspace(const Kv4Sequences &q, int heads, int kv_heads, int dim) {
+    return shape_of(q, heads, kv_heads, dim).bytes;
+}
+
+int kv4_attention_launch(sm_ctx *ctx, const Kv4Attention &a, const void *Q, const uint8_t *pool, const void *G, void *Y, bool bf16,
+                         void *workspace) {
+    if (bf16) launch(ctx, a, (const uint16_t *)Q, pool, (const uint16_t *)G, (uint16_t *)Y, workspace);
+    else launch(ctx, a, (const float *)Q, pool, (const float *)G, (float *)Y, workspace);
+    return launched(ctx);
+}
+
+}  // namespace smi
