@@ -308,7 +308,10 @@ struct Kv4Attention {
     float scale_log2;                         // the scores' scale for powers of two
     Kv4View q_view, g_view;
     bool vec;           // queries lie aligned to 16 bytes
-    int pieces, least;  // the launcher's: how many pieces of the context, of how many pages at least
+    // the launcher's: how many pieces of the context, of how many pages at least, and where their kernel leaves for
+    // each sequence which is its first and how many they are
+    int pieces, least;
+    int2 *info;
 };
 // Unchecked launchers on raw device pointers (kv4_cache.hip, kv4_attention.hip).
 int qk_norm_rope_launch(sm_ctx *ctx, const QkNormRope &a, const void *Q, const void *K, void *Yq, void *Yk, bool bf16);

@@ -18,6 +18,7 @@ using namespace smi;
 using kv4::bf16x2;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 constexpr float kNone = -INFINITY;
@@ -34,6 +35,14 @@ __device__ __forceinline__ void three_parts(float a, float b, uint32_t part[3]) 
     part[2] = kv4::bf16_pair(a1 - __uint_as_float(part[1] << 16), b1 - __uint_as_float(part[1] & 0xffff0000u));
 }
 
+__device__ __forceinline__ float gated(float y, float g) { return y / (1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)); }
+
+// v, of which nothing is known: what a loop makes of it is made in each turn instead of being held in registers.
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // The larger of a lane's value and those of the lanes 16, 32 and 48 away.
 __device__ __forceinline__ float max_of_quarters(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -44,6 +53,15 @@ __device__ __forceinline__ float max_of_quarters(float v) {
 __device__ __forceinline__ float sum_of_quarters(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ float max_of_halves(float v) {
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
@@ -189,8 +207,9 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n16 = lane % 16, kq = lane / 16;
     const Piece piece = piece_of(a.q, a.window, a.pieces, a.least, blockIdx.y);
     if (piece.s < 0) return;
+    if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
     const kv4::Span span = kv4::span(a.q, piece.s);
-    const int head = blockIdx.x / tiles, tile = blockIdx.x % tiles, group = a.heads / a.kv_heads;
+    const int head = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
     const int rows = span.n * group - 16 * tile;  // of the sequence, from this tile's first on
     if (rows <= 0) return;
     const int first = span.length - span.n;       // the first new token's position
@@ -403,7 +422,7 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
             for (int i = 0; i < 4; i++)
                 if (d + i < a.dim) {
                     float y = all == 0.0f ? 0.0f : v[i] * inv;
-                    if (g) y = y / (1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * kv4::value(g[d + i])));
+                    if (g) y = gated(y, kv4::value(g[d + i]));
                     kv4::store1(Y + out + d + i, y);
                 }
         }
@@ -411,110 +430,410 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
     if (piece.count > 1 && d0 == 0) stats[part] = make_float2(top, all);
 }
 
-// The pieces of one row joined: its sequence's partial sums, each brought to
-// the largest of their maxima.
-template <typename T>
-__global__ void __launch_bounds__(256) k_kv4_join(Kv4Attention a, const T *G, T *Y, const float *parts, const float2 *stats,
-                                                  int tiles, int pitch) {
+// ------------------------------------------------------------------ prompts
+// One workgroup: 32 rows a wave, all of one key-value head, over one piece.
+// The products are transposed as above, on 32 x 32 tiles: a lane holds one
+// row's scores of 32 of a page's 64 positions, and brings them to the second
+// product as they are. A page's keys are staged in LDS as codes, which every
+// wave converts for itself, its values as bf16, converted once; both double,
+// the page after next on its way in registers.
+template <int NC, typename T>
+struct Prompt {
+    static constexpr bool kF32 = sizeof(T) == 4;
+    static constexpr int kPitch = 64 * NC, kBlocks = 2 * NC, kParts = kF32 ? 3 : 1;
+    // f32 queries of 192 dimensions and more take most of a SIMD's registers: one wave on each
+    static constexpr int kWaves = kF32 && NC > 2 ? 4 : 8, kThreads = 64 * kWaves, kRows = 32 * kWaves;
+    static constexpr int kPieces = 2 * NC;                           // of 16 bytes, of a key's codes
+    static constexpr int kKeys = (64 * kPieces + kThreads - 1) / kThreads;  // a thread's
+    static constexpr int kValues = kBlocks * 256 / kThreads;         // words of four positions' values, a thread's
+    static constexpr int kHalves = NC > 2 ? 1 : 2;                   // of a page at a time: what registers hold
+    // Where piece `p` of position t lies: any eight neighbouring positions' same piece in other banks.
+    static __device__ __forceinline__ int slot(int t, int p) {
+        const int turned = NC == 1 ? p ^ (t >> 2 & 1) : NC == 2 ? p ^ (t >> 1 & 3) : NC == 4 ? p ^ (t & 7) : (p + (t >> 2 & 1)) % kPieces;
+        return (t * kPieces + turned) * 16;
+    }
+};
+
+template <int NC, typename T>
+__global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Attention a, const T *Q, const uint8_t *pool, const T *G,
+                                                                        T *Y, float *parts, float2 *stats, int tiles) {
+    using R = Prompt<NC, T>;
+    constexpr int kPitch = R::kPitch, kBlocks = R::kBlocks;
+    __shared__ __attribute__((aligned(16))) uint8_t s_keys[2][64 * R::kPieces * 16];
+    __shared__ __attribute__((aligned(16))) uint8_t s_values[2][kBlocks * 4096];
+    __shared__ uint32_t s_scales[2][kBlocks][16];  // of the keys: a byte for each 16 positions
+    __shared__ uint32_t s_nan[3][kBlocks][2];
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n32 = lane % 32, kq = lane / 32;
+    const Piece piece = piece_of(a.q, a.window, a.pieces, a.least, blockIdx.y);
+    if (piece.s < 0) return;
+    if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
+    const kv4::Span span = kv4::span(a.q, piece.s);
+    // the longest rows first
+    const int head = blockIdx.x % a.kv_heads, tile = tiles - 1 - blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
+    const int rows = span.n * group - R::kRows * tile;
+    if (rows <= 0) return;
+    const int first = span.length - span.n;
+    const auto token_of = [&](int r) { return (R::kRows * tile + min(r, rows - 1)) / group; };
+
+    const int row = R::kRows * tile + min(32 * wave + n32, rows - 1), token = row / group, hq = head * group + row % group;
+    const int hi = first + token, lo = a.window > 0 ? max(hi - a.window + 1, 0) : 0;
+    const auto low = [&](int position) { return a.window > 0 ? max(position - a.window + 1, 0) : 0; };
+    // the workgroup's rows and the wave's: the first and last one's position, the lowest position of any, of all
+    const int last = first + token_of(R::kRows - 1), early = first + token_of(0), any_lo = low(early), all_lo = low(last);
+    const int w_last = first + token_of(32 * wave + 31), w_early = first + token_of(32 * wave), w_any = low(w_early), w_all = low(w_last);
+    const bool works = 32 * wave < rows;
+    const int begin = max(piece.first, any_lo / 64), end = min(piece.end, (last >> 6) + 1);
+
+    uint32_t q[R::kParts][NC][4][4];  // step (c, s): dimensions 64 c + 32 kq + 8 s
+    {
+        const T *x = Q + (int64_t)(span.row + token) * a.q_view.stride + hq * a.q_view.head + a.q_view.offset;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const int d = 64 * c + 32 * kq + 8 * s;
+                float v[8] = {};
+                if (d < a.dim) kv4::load8(x + d, a.vec, v);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (R::kF32) {
+                        uint32_t part[3];
+                        three_parts(v[2 * j], v[2 * j + 1], part);
+#pragma unroll
+                        for (int t = 0; t < 3; t++) q[t][c][s][j] = part[t];
+                    } else {
+                        q[0][c][s][j] = kv4::bf16_pair(v[2 * j], v[2 * j + 1]);
+                    }
+                }
+            }
+    }
+
+    f32x16 o[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++) o[b] = f32x16{};
+    float m = kNone, sum = 0.0f;
+
+    const int64_t step = (int64_t)a.kv_heads * (68 * kPitch);
+    const uint8_t *base = pool + (int64_t)head * (68 * kPitch);
+    u32x4 key[R::kKeys];
+    uint32_t value[R::kValues], scale[R::kValues], key_scale = 0;
+    const auto fetch = [&](int at, int &page) {
+        const int tid = here(threadIdx.x);
+        page = kv4::page_of(a.q, piece.s, at, a.pages);
+        const uint8_t *t = base + max(page, 0) * step;
+#pragma unroll
+        for (int j = 0; j < R::kKeys; j++)
+            if (64 * R::kPieces % R::kThreads == 0 || tid + j * R::kThreads < 64 * R::kPieces)
+                key[j] = *(const u32x4 *)(t + (tid + j * R::kThreads) * 16);
+#pragma unroll
+        for (int j = 0; j < R::kValues; j++) {
+            const int u = tid * R::kValues + j;
+            value[j] = *(const uint32_t *)(t + kv4::value_codes(kPitch) + u * 4);
+            scale[j] = *(const uint32_t *)(t + kv4::value_scales(kPitch) + u / 256 * 64 + u / 64 % 4 * 16 + u % 4 * 4);
+        }
+        if (tid < 16 * kBlocks) key_scale = *(const uint32_t *)(t + kv4::key_scales(kPitch) + tid * 4);
+    };
+    const auto is_edge = [&](int at, int page) { return page < 0 || 64 * at < all_lo || 64 * at + 63 > early; };
+    const auto stage = [&](int at, int page) {
+        const int tid = here(threadIdx.x);
+        const int buffer = (at - begin) & 1;
+#pragma unroll
+        for (int j = 0; j < R::kKeys; j++) {
+            const int u = tid + j * R::kThreads;
+            if (64 * R::kPieces % R::kThreads == 0 || u < 64 * R::kPieces)
+                *(u32x4 *)(s_keys[buffer] + R::slot(u / R::kPieces, u % R::kPieces)) = key[j];
+        }
+        const bool edge = is_edge(at, page);
+#pragma unroll
+        for (int j = 0; j < R::kValues; j++) {
+            const int u = tid * R::kValues + j, b = u / 256, r = u / 4 % 16, k = u / 64 % 4, g = u % 4;
+            if (edge) {
+                // values that no row has may be anything: their scales count as 1, and 0 times their codes is 0;
+                // NaN that some rows have and others do not is told apart afterwards
+                const int t0 = 16 * g + 4 * k;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = 64 * at + t0 + i;
+                    const bool has = page >= 0 && t >= any_lo && t <= last, nan = (scale[j] >> (8 * i) & 255u) == 255u;
+                    if (has && nan) atomicOr(&s_nan[(at - begin) % 3][b][t0 / 32], 1u << ((t0 + i) % 32));
+                    if (!has || nan) scale[j] = (scale[j] & ~(255u << (8 * i))) | 127u << (8 * i);
+                }
+            }
+            uint32_t v[2][2];
+            four(value[j], scale[j], v[0], v[1]);
+            uint8_t *to = s_values[buffer] + ((b * 4 + g) * 2 + (k & 1)) * 512 + r * 16 + (k >> 1) * 8;
+            *(uint2 *)to = make_uint2(v[0][0], v[0][1]);
+            *(uint2 *)(to + 256) = make_uint2(v[1][0], v[1][1]);
+        }
+        if (tid < 16 * kBlocks) s_scales[buffer][tid / 16][tid % 16] = key_scale;
+    };
+
+    if (tid < 3 * kBlocks * 2) (&s_nan[0][0][0])[tid] = 0;
+    int page = -1, next_page = -1;
+    if (begin < end) {
+        fetch(begin, next_page);
+        __syncthreads();
+        stage(begin, next_page);
+    }
+    for (int at = begin; at < end; at++) {
+        page = next_page;
+        __syncthreads();
+        if (tid < kBlocks * 2) s_nan[(at - begin + 2) % 3][tid / 2][tid % 2] = 0;
+        if (at + 1 < end) fetch(at + 1, next_page);
+        const int p0 = 64 * at, buffer = (at - begin) & 1, n32 = here(lane % 32), kq = here(lane / 32);
+        if (works && p0 <= w_last && p0 + 63 >= w_any) {
+#pragma unroll
+            for (int h0 = 0; h0 < 2; h0 += R::kHalves) {
+                // S^T: positions 32 h + 8 (i / 4) + 4 kq + i % 4 of row n32
+                f32x16 s[R::kHalves];
+#pragma unroll
+                for (int h = 0; h < R::kHalves; h++) {
+                    s[h] = f32x16{};
+#pragma unroll
+                    for (int c = 0; c < NC; c++) {
+                        const u32x4 w = *(const u32x4 *)(s_keys[buffer] + R::slot(32 * (h0 + h) + n32, 2 * c + kq));
+                        // byte 0 or 1 for the lower half of the page, 2 or 3 for the upper one
+                        const float by = scale_at(s_scales[buffer][2 * c + kq][n32 % 16] >> (n32 / 16 * 8), 2 * (h0 + h));
+#pragma unroll
+                        for (int t = 0; t < 4; t++) {
+                            const bf16x8 k = as_bf16(eight(w[t], by));
+#pragma unroll
+                            for (int p = R::kParts - 1; p >= 0; p--)
+                                s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                                    k, as_bf16(u32x4{q[p][c][t][0], q[p][c][t][1], q[p][c][t][2], q[p][c][t][3]}), s[h], 0, 0, 0);
+                        }
+                    }
+                }
+                if (page < 0 || p0 < w_all || p0 + 63 > w_early) {
+                    const int from_t = page < 0 ? 64 : lo - p0 - 4 * kq, to_t = hi - p0 - 4 * kq;
+#pragma unroll
+                    for (int h = 0; h < R::kHalves; h++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int t = 32 * (h0 + h) + i / 4 * 8 + i % 4;
+                            if (t < from_t || t > to_t) s[h][i] = kNone;
+                        }
+                }
+                float top = kNone;
+#pragma unroll
+                for (int h = 0; h < R::kHalves; h++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) top = fmaxf(top, s[h][i]);
+                top = max_of_halves(top) * a.scale_log2;
+                if (__any(top > m + 8.0f || (m == kNone && top > kNone))) {
+                    const float to = fmaxf(m, top), by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+                    m = to;
+                    sum *= by;
+#pragma unroll
+                    for (int b = 0; b < kBlocks; b++) o[b] *= by;
+                }
+                const float from = m == kNone ? 0.0f : -m;
+#pragma unroll
+                for (int h = 0; h < R::kHalves; h++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        s[h][i] = __builtin_amdgcn_exp2f(fmaf(s[h][i], a.scale_log2, from));
+                        sum += s[h][i];
+                    }
+                // O^T: dimensions 32 b + 8 (i / 4) + 4 kq + i % 4 of row n32
+#pragma unroll
+                for (int g = 0; g < 2 * R::kHalves; g++) {
+                    u32x4 p[R::kParts];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float x = s[g / 2][8 * (g % 2) + 2 * j], y = s[g / 2][8 * (g % 2) + 2 * j + 1];
+                        if constexpr (R::kF32) {
+                            uint32_t part[3];
+                            three_parts(x, y, part);
+#pragma unroll
+                            for (int t = 0; t < 3; t++) p[t][j] = part[t];
+                        } else {
+                            p[0][j] = kv4::bf16_pair(x, y);
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < kBlocks; b++) {
+                        const bf16x8 v =
+                            as_bf16(*(const u32x4 *)(s_values[buffer] + ((b * 4 + 2 * h0 + g) * 2 + kq) * 512 + n32 * 16));
+#pragma unroll
+                        for (int t = R::kParts - 1; t >= 0; t--)
+                            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, as_bf16(p[t]), o[b], 0, 0, 0);
+                    }
+                }
+            }
+            if (is_edge(at, page)) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; b++) {
+                    const uint64_t nan = (uint64_t)s_nan[(at - begin) % 3][b][1] << 32 | s_nan[(at - begin) % 3][b][0];
+                    if (nan == 0) continue;
+                    // the row's positions of this page: bits from lo to hi
+                    const int from_bit = min(max(lo - p0, 0), 64), to_bit = min(max(hi + 1 - p0, 0), 64);
+                    const uint64_t below = to_bit == 64 ? ~0ull : (1ull << to_bit) - 1, above = from_bit == 64 ? 0ull : ~0ull << from_bit;
+                    if (nan & below & above)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[b][i] = NAN;
+                }
+            }
+        }
+        if (at + 1 < end) stage(at + 1, next_page);
+    }
+    if (32 * wave + n32 >= rows) return;
+    sum = sum_of_halves(sum);
+    const int64_t part = ((int64_t)blockIdx.y * gridDim.x + tile * a.kv_heads + head) * R::kRows + 32 * wave + n32;
+    const int64_t out = ((int64_t)(span.row + token) * a.heads + hq) * a.dim;
+    const T *g = G ? G + (int64_t)(span.row + token) * a.g_view.stride + hq * a.g_view.head + a.g_view.offset : nullptr;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int b = 0; b < kBlocks; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 32 * b + 2 * i + 4 * kq;
+            if (piece.count > 1) {
+                *(f32x4 *)(parts + part * kPitch + d) = f32x4{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
+            } else if (d < a.dim) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    y[j] = sum == 0.0f ? 0.0f : o[b][i + j] * inv;
+                    if (g) y[j] = gated(y[j], kv4::value(g[d + j]));
+                }
+                if constexpr (R::kF32) *(f32x4 *)(Y + out + d) = f32x4{y[0], y[1], y[2], y[3]};
+                else *(uint2 *)(Y + out + d) = make_uint2(kv4::bf16_pair(y[0], y[1]), kv4::bf16_pair(y[2], y[3]));
+            }
+        }
+    if (piece.count > 1 && kq == 0) stats[part] = make_float2(m, sum);
+}
+
+// ------------------------------------------------------------ pieces joined
+// The pieces of one row: its sequence's partial sums, each brought to the
+// largest of their maxima. Eight waves a row take the pieces in turn.
+constexpr int kJoinWaves = 8;
+template <int NC, typename T>
+__global__ void __launch_bounds__(64 * kJoinWaves) k_kv4_join(Kv4Attention a, const T *G, T *Y, const float *parts,
+                                                              const float2 *stats, const int2 *info, int tiles, int tile_rows) {
+    constexpr int kPitch = 64 * NC;
     const int s = blockIdx.y, group = a.heads / a.kv_heads;
     const kv4::Span span = kv4::span(a.q, s);
     const int token = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
     if (token >= span.n) return;
-    // this sequence's first piece: as the rows' kernel counts them
-    const int lane = threadIdx.x % 64;
-    int total = 0, before = 0, count = 0;
-    for (int at = 0; at < a.q.count; at += 64) {
-        int n = 0;
-        if (at + lane < a.q.count) {
-            const kv4::Span o = kv4::span(a.q, at + lane);
-            const int2 p = pages_of(o, a.window);
-            n = o.n > 0 ? p.y - p.x : 0;
-        }
-#pragma unroll
-        for (int i = 1; i < 64; i *= 2) n += __shfl_xor(n, i, 64);
-        total += n;
-    }
-    const int each = max(a.least, (total + a.pieces - 1) / a.pieces);
-    for (int at = 0; at <= s; at += 64) {
-        int n = 0;
-        if (at + lane <= s) {
-            const kv4::Span o = kv4::span(a.q, at + lane);
-            const int2 p = pages_of(o, a.window);
-            n = o.n > 0 ? max((p.y - p.x + each - 1) / each, 1) : 0;
-        }
-        if (s - at < 64) count = __shfl(n, s - at, 64);
-        if (at + lane == s) n = 0;
-#pragma unroll
-        for (int i = 1; i < 64; i *= 2) n += __shfl_xor(n, i, 64);
-        before += n;
-    }
-    if (count <= 1) return;
+    const int2 pieces = info[s];  // the first, how many
+    if (pieces.y <= 1) return;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int head = h / group, row = token * group + h % group;
-    const int64_t base = ((int64_t)head * tiles + row / 16) * 16 + row % 16, step = (int64_t)a.kv_heads * tiles * 16;
-    float top = kNone, all = 0.0f;
-    for (int c = 0; c < count; c++) top = fmaxf(top, stats[base + (before + c) * step].x);
-    const int64_t out = ((int64_t)(span.row + token) * a.heads + h) * a.dim;
-    const T *g = G ? G + (int64_t)(span.row + token) * a.g_view.stride + h * a.g_view.head + a.g_view.offset : nullptr;
-    float v = 0.0f;
-    const int d = threadIdx.x;
-    if (d >= pitch) return;
-    for (int c = 0; c < count; c++) {
-        const float2 st = stats[base + (before + c) * step];
-        const float by = st.x == kNone ? 0.0f : __builtin_amdgcn_exp2f(st.x - top);
-        all += st.x == kNone ? (st.y == 0.0f ? 0.0f : NAN) : st.y * by;
-        v += parts[(base + (before + c) * step) * pitch + d] * by;
+    const int64_t step = (int64_t)a.kv_heads * tiles * tile_rows;
+    const int64_t base = ((int64_t)row / tile_rows * a.kv_heads + head) * tile_rows + row % tile_rows + pieces.x * step;
+    float top = kNone, all = 0.0f, v[NC] = {};
+    for (int c0 = 4 * wave; c0 < pieces.y; c0 += 4 * kJoinWaves) {
+        float2 st[4];
+        float x[4][NC];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int64_t at = base + min(c0 + j, pieces.y - 1) * step;
+            st[j] = stats[at];
+#pragma unroll
+            for (int n = 0; n < NC; n++) x[j][n] = parts[at * kPitch + 64 * n + lane];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (c0 + j >= pieces.y) break;
+            const float to = fmaxf(top, st[j].x);
+            const float was = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(top - to);
+            const float by = st[j].x == kNone ? 0.0f : __builtin_amdgcn_exp2f(st[j].x - to);
+            // a sum that is not a number, of scores that are none, stays one
+            all = all * was + (st[j].x == kNone ? (st[j].y == 0.0f ? 0.0f : NAN) : st[j].y * by);
+#pragma unroll
+            for (int n = 0; n < NC; n++) v[n] = v[n] * was + x[j][n] * by;
+            top = to;
+        }
     }
+    __shared__ float s_v[kJoinWaves][kPitch], s_top[kJoinWaves], s_all[kJoinWaves];
+#pragma unroll
+    for (int n = 0; n < NC; n++) s_v[wave][64 * n + lane] = v[n];
+    if (lane == 0) s_top[wave] = top, s_all[wave] = all;
+    __syncthreads();
+    const int d = threadIdx.x;
     if (d >= a.dim) return;
-    float y = all == 0.0f ? 0.0f : v / all;
-    if (g) y = y / (1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * kv4::value(g[d])));
-    kv4::store1(Y + out + d, y);
+    top = s_top[0], all = 0.0f;
+#pragma unroll
+    for (int w = 1; w < kJoinWaves; w++) top = fmaxf(top, s_top[w]);
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; w++) {
+        const float by = s_top[w] == kNone ? 0.0f : __builtin_amdgcn_exp2f(s_top[w] - top);
+        all += s_top[w] == kNone ? s_all[w] : s_all[w] * by;
+        y += s_v[w][d] * by;
+    }
+    y = all == 0.0f ? 0.0f : y / all;
+    if (G) y = gated(y, kv4::value(G[(int64_t)(span.row + token) * a.g_view.stride + h * a.g_view.head + a.g_view.offset + d]));
+    kv4::store1(Y + ((int64_t)(span.row + token) * a.heads + h) * a.dim + d, y);
 }
 
 // Workgroups that fill the GPU, and the least pages that are worth a piece.
 constexpr int kWorkgroups = 512, kLeast = 4;
+// From so many rows of a key-value head on a workgroup of prompts.
+constexpr int kPromptRows = 64;
 
 struct Shape {
-    int tiles, pieces;
-    uint64_t slots, part_bytes, bytes;
+    bool prompt;
+    int tile_rows, tiles, pieces, least;
+    uint64_t slots, part_bytes, stat_bytes, bytes;
 };
-Shape shape_of(const Kv4Sequences &q, int heads, int kv_heads, int dim) {
+template <typename T>
+int prompt_rows(int pitch) {
+    return pitch <= 64 ? Prompt<1, T>::kRows : pitch <= 128 ? Prompt<2, T>::kRows : pitch <= 192 ? Prompt<3, T>::kRows : Prompt<4, T>::kRows;
+}
+Shape shape_of(const Kv4Sequences &q, int heads, int kv_heads, int dim, bool bf16) {
     Shape s;
-    s.tiles = (int)(((int64_t)q.longest * (heads / kv_heads) + 15) / 16);
-    const int64_t each = (int64_t)kv_heads * s.tiles, most = (int64_t)q.count * ((q.table_pages + kLeast - 1) / kLeast);
-    int64_t pieces = (kWorkgroups + each - 1) / each;
+    const int64_t rows = (int64_t)q.longest * (heads / kv_heads);
+    const int pitch = kv4_pitch(dim);
+    s.prompt = rows >= kPromptRows;
+    s.tile_rows = !s.prompt ? 16 : bf16 ? prompt_rows<uint16_t>(pitch) : prompt_rows<float>(pitch);
+    s.tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
+    s.least = kLeast;
+    const int64_t each = (int64_t)kv_heads * s.tiles, most = (int64_t)q.count * ((q.table_pages + s.least - 1) / s.least);
+    int64_t pieces = s.prompt ? 256 / (each * q.count) : (kWorkgroups + each - 1) / each;
     if (pieces > most) pieces = most;
     s.pieces = pieces < 1 ? 1 : (int)pieces;
     s.slots = (uint64_t)(s.pieces > 1 ? s.pieces + q.count : q.count);
-    s.part_bytes = s.pieces > 1 ? s.slots * each * 16 * kv4_pitch(dim) * 4 : 0;
-    s.bytes = s.pieces > 1 ? s.part_bytes + s.slots * each * 16 * 8 : 0;
+    s.part_bytes = s.pieces > 1 ? s.slots * each * s.tile_rows * pitch * 4 : 0;
+    s.stat_bytes = s.pieces > 1 ? s.slots * each * s.tile_rows * 8 : 0;
+    s.bytes = s.part_bytes + s.stat_bytes + (s.pieces > 1 ? (uint64_t)q.count * 8 : 0);
+    if (s.pieces == 1) s.least = q.table_pages + 1;  // one piece a sequence: as large as any
     return s;
 }
 
-template <typename T>
-void launch(sm_ctx *ctx, Kv4Attention a, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
-    const Shape s = shape_of(a.q, a.heads, a.kv_heads, a.dim);
-    const int pitch = kv4_pitch(a.dim);
-    // one piece a sequence: as large as any
-    a.pieces = s.pieces, a.least = s.pieces > 1 ? kLeast : a.q.table_pages + 1;
+template <int NC, typename T>
+void launch(sm_ctx *ctx, Kv4Attention a, const Shape &s, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
+    a.pieces = s.pieces, a.least = s.least;
     float *parts = (float *)workspace;
     float2 *stats = (float2 *)((char *)workspace + s.part_bytes);
+    a.info = s.pieces > 1 ? (int2 *)((char *)workspace + s.part_bytes + s.stat_bytes) : nullptr;
     const dim3 grid((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots);
-    switch (pitch / 64) {
-        case 1: k_kv4_rows<1, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles); break;
-        case 2: k_kv4_rows<2, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles); break;
-        case 3: k_kv4_rows<3, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles); break;
-        default: k_kv4_rows<4, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles); break;
-    }
+    if (s.prompt) k_kv4_prompt<NC, T><<<grid, Prompt<NC, T>::kThreads, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
+    else k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
     if (s.pieces > 1)
-        k_kv4_join<T><<<dim3((uint32_t)a.q.longest * a.heads, a.q.count), 256, 0, ctx->stream>>>(a, G, Y, parts, stats, s.tiles, pitch);
+        k_kv4_join<NC, T><<<dim3((uint32_t)a.q.longest * a.heads, a.q.count), 64 * kJoinWaves, 0, ctx->stream>>>(
+            a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
+}
+template <typename T>
+void launch(sm_ctx *ctx, const Kv4Attention &a, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
+    const Shape s = shape_of(a.q, a.heads, a.kv_heads, a.dim, sizeof(T) == 2);
+    switch (kv4_pitch(a.dim) / 64) {
+        case 1: return launch<1, T>(ctx, a, s, Q, pool, G, Y, workspace);
+        case 2: return launch<2, T>(ctx, a, s, Q, pool, G, Y, workspace);
+        case 3: return launch<3, T>(ctx, a, s, Q, pool, G, Y, workspace);
+        default: return launch<4, T>(ctx, a, s, Q, pool, G, Y, workspace);
+    }
 }
 
 }  // namespace
 
 namespace smi {
 
+// Enough for either type.
 uint64_t kv4_attention_workspace(const Kv4Sequences &q, int heads, int kv_heads, int dim) {
-    return shape_of(q, heads, kv_heads, dim).bytes;
+    const uint64_t f = shape_of(q, heads, kv_heads, dim, false).bytes, b = shape_of(q, heads, kv_heads, dim, true).bytes;
+    return f > b ? f : b;
 }
 
 int kv4_attention_launch(sm_ctx *ctx, const Kv4Attention &a, const void *Q, const uint8_t *pool, const void *G, void *Y, bool bf16,
