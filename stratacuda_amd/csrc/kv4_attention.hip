@@ -11,7 +11,10 @@
 // the sum of three bf16 numbers (8 significant bits each, so all 24) and cost
 // three matrix instructions. For bf16 the probabilities are rounded to bf16,
 // half a step of 2^-8 relative, like the result; sums are f32's.
+#include <type_traits>
+
 #include "kv4_device.h"
+#include "strata_device.h"
 
 namespace {
 using namespace smi;
@@ -19,6 +22,7 @@ using kv4::bf16x2;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f32x16 = __attribute__((ext_vector_type(16))) float;
+using i32x8 = __attribute__((ext_vector_type(8))) int;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 constexpr float kNone = -INFINITY;
@@ -38,7 +42,7 @@ __device__ __forceinline__ void three_parts(float a, float b, uint32_t part[3]) 
 __device__ __forceinline__ float gated(float y, float g) { return y / (1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * g)); }
 
 // v, of which nothing is known: what a loop makes of it is made in each turn instead of being held in registers.
-__device__ __forceinline__ int here(int v) {
+__device__ __forceinline__ uint32_t here(uint32_t v) {
     asm volatile("" : "+v"(v));
     return v;
 }
@@ -115,7 +119,9 @@ __device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int lea
             const int who = __ffsll((unsigned long long)past) - 1;
             const int count = __shfl(n, who, 64), number = slot - before - (__shfl(upto, who, 64) - count);
             const int first = __shfl(p.x, who, 64), end = __shfl(p.y, who, 64);
-            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count};
+            // the same in all lanes: kept, and what it leads to, in scalar registers
+            const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+            return {one(at + who), one(first + number * each), one(min(first + (number + 1) * each, end)), one(number), one(count)};
         }
         before += __shfl(upto, 63, 64);
     }
@@ -431,22 +437,37 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
 }
 
 // ------------------------------------------------------------------ prompts
-// One workgroup: 32 rows a wave, all of one key-value head, over one piece.
-// The products are transposed as above, on 32 x 32 tiles: a lane holds one
-// row's scores of 32 of a page's 64 positions, and brings them to the second
-// product as they are. A page's keys are staged in LDS as codes, which every
-// wave converts for itself, its values as bf16, converted once; both double,
-// the page after next on its way in registers.
+// One workgroup: 32 rows a wave, all of one key-value head, over one piece of
+// the sequence, in units of 32 or 64 positions. The products are transposed as
+// above, on 32 x 32 tiles: a lane holds one row's scores of half of a unit's
+// positions, and brings them to the second product as they are.
+//
+// A wave alternates between the matrix unit (a unit's scores, the unit
+// before's values) and vector instructions (its softmax, its share of the
+// units that are staged next); of the two waves of a SIMD one is half a turn
+// ahead, so that both are busy. Turns end at barriers. Keys are staged in LDS
+// as codes, values as bf16, converted once; both twice, the next unit's on
+// their way in registers.
+//
+// Scores of bf16 queries: codes go into the matrix unit as they are, with
+// their scales. The query is the sum of two e4m3 numbers of 4 significant bits
+// each, with one power of two for the row: all 8 bits of a bf16 number from
+// 2^-13 of the row's largest up, 2^-22 of that largest otherwise. That unit
+// cuts products 2^13 below the largest of eight neighbours: at most 7 * 2^-13
+// of a score's products' magnitudes are lost, 1e-5 for ordinary ones, where
+// probabilities are rounded by 2^-8. Queries of f32 take bf16's unit.
 template <int NC, typename T>
 struct Prompt {
     static constexpr bool kF32 = sizeof(T) == 4;
     static constexpr int kPitch = 64 * NC, kBlocks = 2 * NC, kParts = kF32 ? 3 : 1;
     // f32 queries of 192 dimensions and more take most of a SIMD's registers: one wave on each
     static constexpr int kWaves = kF32 && NC > 2 ? 4 : 8, kThreads = 64 * kWaves, kRows = 32 * kWaves;
-    static constexpr int kPieces = 2 * NC;                           // of 16 bytes, of a key's codes
-    static constexpr int kKeys = (64 * kPieces + kThreads - 1) / kThreads;  // a thread's
-    static constexpr int kValues = kBlocks * 256 / kThreads;         // words of four positions' values, a thread's
-    static constexpr int kHalves = NC > 2 ? 1 : 2;                   // of a page at a time: what registers hold
+    static constexpr int kHalves = NC > 2 || (kF32 && NC > 1) ? 1 : 2;  // of a page in a unit: what registers hold
+    static constexpr int kUnit = 32 * kHalves, kTurns = 64 / kUnit;
+    static constexpr int kPieces = 2 * NC;  // of 16 bytes, of a key's codes
+    // words of codes that are staged in a turn, and a thread's
+    static constexpr int kKeyWords = kUnit * 4 * kPieces, kKeys = (kKeyWords + kThreads - 1) / kThreads;
+    static constexpr int kValueWords = kBlocks * 128 * kHalves, kValues = (kValueWords + kThreads - 1) / kThreads;
     // Where piece `p` of position t lies: any eight neighbouring positions' same piece in other banks.
     static __device__ __forceinline__ int slot(int t, int p) {
         const int turned = NC == 1 ? p ^ (t >> 2 & 1) : NC == 2 ? p ^ (t >> 1 & 3) : NC == 4 ? p ^ (t & 7) : (p + (t >> 2 & 1)) % kPieces;
@@ -456,14 +477,16 @@ struct Prompt {
 
 template <int NC, typename T>
 __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Attention a, const T *Q, const uint8_t *pool, const T *G,
-                                                                        T *Y, float *parts, float2 *stats, int tiles) {
+                                                                          T *Y, float *parts, float2 *stats, int tiles) {
     using R = Prompt<NC, T>;
-    constexpr int kPitch = R::kPitch, kBlocks = R::kBlocks;
-    __shared__ __attribute__((aligned(16))) uint8_t s_keys[2][64 * R::kPieces * 16];
-    __shared__ __attribute__((aligned(16))) uint8_t s_values[2][kBlocks * 4096];
-    __shared__ uint32_t s_scales[2][kBlocks][16];  // of the keys: a byte for each 16 positions
-    __shared__ uint32_t s_nan[3][kBlocks][2];
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64, n32 = lane % 32, kq = lane / 32;
+    constexpr int kPitch = R::kPitch, kBlocks = R::kBlocks, kUnit = R::kUnit, kHalves = R::kHalves, kTurns = R::kTurns;
+    constexpr int kGroups = kUnit / 16;  // of 16 positions
+    __shared__ __attribute__((aligned(16))) uint8_t s_keys[2][kUnit * R::kPieces * 16];
+    __shared__ __attribute__((aligned(16))) uint8_t s_values[2][kBlocks * kGroups * 1024];
+    __shared__ uint32_t s_scales[2][kBlocks][16];  // of the keys: a byte for each 16 positions of the page
+    __shared__ uint64_t s_nan[4][kBlocks];         // values that are NaN for some rows and not there for others
+    const uint32_t lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const Piece piece = piece_of(a.q, a.window, a.pieces, a.least, blockIdx.y);
     if (piece.s < 0) return;
     if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
@@ -475,37 +498,89 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
     const int first = span.length - span.n;
     const auto token_of = [&](int r) { return (R::kRows * tile + min(r, rows - 1)) / group; };
 
-    const int row = R::kRows * tile + min(32 * wave + n32, rows - 1), token = row / group, hq = head * group + row % group;
+    const int row = R::kRows * tile + min(32 * wave + (int)(lane % 32), rows - 1), token = row / group, hq = head * group + row % group;
     const int hi = first + token, lo = a.window > 0 ? max(hi - a.window + 1, 0) : 0;
     const auto low = [&](int position) { return a.window > 0 ? max(position - a.window + 1, 0) : 0; };
     // the workgroup's rows and the wave's: the first and last one's position, the lowest position of any, of all
     const int last = first + token_of(R::kRows - 1), early = first + token_of(0), any_lo = low(early), all_lo = low(last);
     const int w_last = first + token_of(32 * wave + 31), w_early = first + token_of(32 * wave), w_any = low(w_early), w_all = low(w_last);
     const bool works = 32 * wave < rows;
-    const int begin = max(piece.first, any_lo / 64), end = min(piece.end, (last >> 6) + 1);
+    const int begin = max(piece.first, any_lo / 64), end = min(piece.end, (last >> 6) + 1), units = max(end - begin, 0) * kTurns;
+    const auto position_of = [&](int u) { return 64 * begin + kUnit * u; };
+    // page numbers, a lane's each, of 64 pages; asked for in order
+    int ids = -1;
+    bool holes = false;  // a page that is none was among them
+    const auto id_of = [&](int u) {
+        const int at = u / kTurns;
+        if (at >= end - begin) return -1;
+        if (u % (64 * kTurns) == 0) {
+            ids = kv4::page_of(a.q, piece.s, min(begin + at + (int)lane, end - 1), a.pages);
+            holes = holes || __any(ids < 0);
+        }
+        return __builtin_amdgcn_readlane(ids, at % 64);
+    };
+    const auto is_edge = [&](int p0, int id) { return id < 0 || p0 < all_lo || p0 + kUnit - 1 > early; };
+    // units all of whose positions every row of the workgroup has
+    const int whole_from = (max(all_lo - 64 * begin, 0) + kUnit - 1) / kUnit, whole_to = min(max(early + 1 - 64 * begin, 0) / kUnit, units);
+    const auto is_live = [&](int p0) { return works && p0 <= w_last && p0 + kUnit - 1 >= w_any; };
 
-    uint32_t q[R::kParts][NC][4][4];  // step (c, s): dimensions 64 c + 32 kq + 8 s
+    // queries: for f32 three bf16 numbers, dimensions 64 c + 32 kq + 8 s of step (c, s) a lane; else two e4m3 ones,
+    // 64 c + 32 i + 16 kq of half i of step c
+    uint32_t q[R::kParts][NC][16];
+    int q_scale = 0;
     {
         const T *x = Q + (int64_t)(span.row + token) * a.q_view.stride + hq * a.q_view.head + a.q_view.offset;
+        const int kq = lane / 32;
+        if constexpr (R::kF32) {
 #pragma unroll
-        for (int c = 0; c < NC; c++)
+            for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int s = 0; s < 4; s++) {
-                const int d = 64 * c + 32 * kq + 8 * s;
-                float v[8] = {};
-                if (d < a.dim) kv4::load8(x + d, a.vec, v);
+                for (int s = 0; s < 4; s++) {
+                    const int d = 64 * c + 32 * kq + 8 * s;
+                    float v[8] = {};
+                    if (d < a.dim) kv4::load8(x + d, a.vec, v);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if constexpr (R::kF32) {
+                    for (int j = 0; j < 4; j++) {
                         uint32_t part[3];
                         three_parts(v[2 * j], v[2 * j + 1], part);
 #pragma unroll
-                        for (int t = 0; t < 3; t++) q[t][c][s][j] = part[t];
-                    } else {
-                        q[0][c][s][j] = kv4::bf16_pair(v[2 * j], v[2 * j + 1]);
+                        for (int t = 0; t < 3; t++) q[t][c][4 * s + j] = part[t];
                     }
                 }
+        } else {
+            float amax = 0.0f;
+#pragma unroll
+            for (int turn = 0; turn < 2; turn++) {  // the row's largest magnitude, then its parts
+                float by = 0.0f;
+                if (turn == 1) {
+                    // at least 2^-123, so that the lower part's scale is one
+                    const int byte = max((int)f8::scale_byte(max_of_halves(amax)), 4);
+                    q_scale = byte, by = f8::inverse_scale(byte);
+                }
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int s = 0; s < 4; s++) {
+                        const int d = 64 * c + 32 * (s / 2) + 16 * kq + 8 * (s % 2);
+                        float v[8] = {};
+                        if (d < a.dim) kv4::load8(x + d, a.vec, v);
+                        if (turn == 0) {
+#pragma unroll
+                            for (int j = 0; j < 8; j++) amax = fmaxf(amax, f8::finite_magnitude(v[j]));
+                            continue;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const float *w = v + 4 * j;
+                            const uint32_t high = f8::codes4((float4){w[0], w[1], w[2], w[3]}, by);
+                            const kv4::f32x2 h0 = __builtin_amdgcn_cvt_pk_f32_fp8(high, false), h1 = __builtin_amdgcn_cvt_pk_f32_fp8(high, true);
+                            const float4 rest = {w[0] * by - h0[0], w[1] * by - h0[1], w[2] * by - h1[0], w[3] * by - h1[1]};
+                            q[0][c][2 * s + j] = high;
+                            q[0][c][8 + 2 * s + j] = f8::codes4(rest, 16.0f);  // at most 16, half a step of 448
+                        }
+                    }
             }
+        }
     }
 
     f32x16 o[kBlocks];
@@ -513,173 +588,293 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
     for (int b = 0; b < kBlocks; b++) o[b] = f32x16{};
     float m = kNone, sum = 0.0f;
 
+    // ------------------------------------------------------------- staging
     const int64_t step = (int64_t)a.kv_heads * (68 * kPitch);
     const uint8_t *base = pool + (int64_t)head * (68 * kPitch);
-    u32x4 key[R::kKeys];
-    uint32_t value[R::kValues], scale[R::kValues], key_scale = 0;
-    const auto fetch = [&](int at, int &page) {
-        const int tid = here(threadIdx.x);
-        page = kv4::page_of(a.q, piece.s, at, a.pages);
-        const uint8_t *t = base + max(page, 0) * step;
-#pragma unroll
-        for (int j = 0; j < R::kKeys; j++)
-            if (64 * R::kPieces % R::kThreads == 0 || tid + j * R::kThreads < 64 * R::kPieces)
-                key[j] = *(const u32x4 *)(t + (tid + j * R::kThreads) * 16);
-#pragma unroll
-        for (int j = 0; j < R::kValues; j++) {
-            const int u = tid * R::kValues + j;
-            value[j] = *(const uint32_t *)(t + kv4::value_codes(kPitch) + u * 4);
-            scale[j] = *(const uint32_t *)(t + kv4::value_scales(kPitch) + u / 256 * 64 + u / 64 % 4 * 16 + u % 4 * 4);
-        }
-        if (tid < 16 * kBlocks) key_scale = *(const uint32_t *)(t + kv4::key_scales(kPitch) + tid * 4);
+    uint32_t key[R::kKeys], key_scale = 0, value[R::kValues], scale[R::kValues];
+    // word w of a unit's values: block, quarter of the positions, dimension, group of 16 positions
+    struct Word {
+        uint32_t b, k, r, g;
     };
-    const auto is_edge = [&](int at, int page) { return page < 0 || 64 * at < all_lo || 64 * at + 63 > early; };
-    const auto stage = [&](int at, int page) {
-        const int tid = here(threadIdx.x);
-        const int buffer = (at - begin) & 1;
+    const auto word_of = [&](uint32_t w) { return Word{w / kGroups / 64, w / kGroups / 16 % 4, w / kGroups % 16, w % kGroups}; };
+    const auto codes_of = [](const Word &w) { return kv4::value_codes(kPitch) + ((w.b * 4 + w.k) * 16 + w.r) * 16 + w.g * 4; };
+    const auto scales_of = [](const Word &w) { return kv4::value_scales(kPitch) + (w.b * 4 + w.k) * 16 + w.g * 4; };
+    constexpr int kRun = R::kValues % 2 == 0 ? 2 : 1;  // a thread's words that lie together
+    // Every load is sent, also those that nothing follows (threads and units past the last take one that is there): so
+    // the ones under way are known where others are waited for. Offsets in 32 bits, opened in each turn: beside a
+    // scalar base they need no registers of their own.
+    const bool has_keys = R::kKeyWords % R::kThreads == 0 || threadIdx.x * R::kKeys < R::kKeyWords;
+    const bool has_values = R::kValueWords % R::kThreads == 0 || threadIdx.x * R::kValues < R::kValueWords;
+    const uint32_t key_at = has_keys ? threadIdx.x * (4 * R::kKeys) : 0, key_scale_at = min(threadIdx.x, 16u * kBlocks - 1) * 4;
+    const uint32_t value_word = has_values ? threadIdx.x * R::kValues : 0;
+    uint32_t value_at[R::kValues / kRun], scale_at_[R::kValues / kRun];
 #pragma unroll
-        for (int j = 0; j < R::kKeys; j++) {
-            const int u = tid + j * R::kThreads;
-            if (64 * R::kPieces % R::kThreads == 0 || u < 64 * R::kPieces)
-                *(u32x4 *)(s_keys[buffer] + R::slot(u / R::kPieces, u % R::kPieces)) = key[j];
+    for (int j = 0; j < R::kValues; j += kRun)
+        value_at[j / kRun] = codes_of(word_of(value_word + j)), scale_at_[j / kRun] = scales_of(word_of(value_word + j));
+    const auto tile_of = [&](int id) { return base + max(id, 0) * step; };
+    const auto fetch_keys = [&](int u, const uint8_t *t) {
+        const uint8_t *from = t + u % kTurns * (4 * R::kKeyWords);
+        const uint32_t at = here(key_at);
+        if constexpr (R::kKeys == 4) {
+            const u32x4 v = *(const u32x4 *)(from + at);
+            key[0] = v[0], key[1] = v[1], key[2] = v[2], key[3] = v[3];
+        } else if constexpr (R::kKeys == 2) {
+            const uint2 v = *(const uint2 *)(from + at);
+            key[0] = v.x, key[1] = v.y;
+        } else {
+#pragma unroll
+            for (int j = 0; j < R::kKeys; j++) key[j] = *(const uint32_t *)(from + at + 4 * j);
         }
-        const bool edge = is_edge(at, page);
+        key_scale = *(const uint32_t *)(t + kv4::key_scales(kPitch) + here(key_scale_at));
+    };
+    const auto fetch_values = [&](int u, const uint8_t *t) {
+        t += u % kTurns * 8;
 #pragma unroll
-        for (int j = 0; j < R::kValues; j++) {
-            const int u = tid * R::kValues + j, b = u / 256, r = u / 4 % 16, k = u / 64 % 4, g = u % 4;
-            if (edge) {
-                // values that no row has may be anything: their scales count as 1, and 0 times their codes is 0;
-                // NaN that some rows have and others do not is told apart afterwards
-                const int t0 = 16 * g + 4 * k;
+        for (int j = 0; j < R::kValues; j += kRun) {
+            const uint8_t *v = t + here(value_at[j / kRun]), *f = t + here(scale_at_[j / kRun]);
+            if constexpr (kRun == 2) {
+                const uint2 x = *(const uint2 *)v, y = *(const uint2 *)f;
+                value[j] = x.x, value[j + 1] = x.y, scale[j] = y.x, scale[j + 1] = y.y;
+            } else {
+                value[j] = *(const uint32_t *)v, scale[j] = *(const uint32_t *)f;
+            }
+        }
+    };
+    const auto stage_keys = [&](int u) {
+        const uint32_t tid = threadIdx.x, word = tid * R::kKeys;
+        const int buffer = u & 1;
+        if (has_keys) {
+            const auto place = [&](uint32_t w) { return s_keys[buffer] + R::slot(w / (4 * R::kPieces), w / 4 % R::kPieces) + w % 4 * 4; };
+            if constexpr (R::kKeys == 4) {
+                *(u32x4 *)place(word) = u32x4{key[0], key[1], key[2], key[3]};
+            } else if constexpr (R::kKeys == 2) {
+                *(uint2 *)place(word) = make_uint2(key[0], key[1]);
+            } else {
 #pragma unroll
+                for (int j = 0; j < R::kKeys; j++) *(uint32_t *)place(word + j) = key[j];
+            }
+        }
+        if (tid < 16 * kBlocks) (&s_scales[buffer][0][0])[tid] = key_scale;
+    };
+    const auto stage_values = [&](int u, int id, auto whole) {
+        const int p0 = position_of(u);
+        if (!has_values) return;
+        if (!whole && u < units && is_edge(p0, id)) {
+            // values that no row has may be anything: their scales count as 1, and 0 times their codes is 0;
+            // NaN that some rows have and others do not is told apart afterwards
+            const uint32_t tid = here(threadIdx.x);
+#pragma unroll
+            for (int j = 0; j < R::kValues; j++) {
+                const Word w = word_of(tid * R::kValues + j);
+                const int t0 = 16 * w.g + 4 * w.k;
                 for (int i = 0; i < 4; i++) {
-                    const int t = 64 * at + t0 + i;
-                    const bool has = page >= 0 && t >= any_lo && t <= last, nan = (scale[j] >> (8 * i) & 255u) == 255u;
-                    if (has && nan) atomicOr(&s_nan[(at - begin) % 3][b][t0 / 32], 1u << ((t0 + i) % 32));
+                    const int t = p0 + t0 + i;
+                    const bool has = id >= 0 && t >= any_lo && t <= last, nan = (scale[j] >> (8 * i) & 255u) == 255u;
+                    if (has && nan) atomicOr((unsigned long long *)&s_nan[u & 3][w.b], 1ull << (t0 + i));
                     if (!has || nan) scale[j] = (scale[j] & ~(255u << (8 * i))) | 127u << (8 * i);
                 }
             }
+        }
+#pragma unroll
+        for (int j = 0; j < R::kValues; j++) {
+            const Word w = word_of(threadIdx.x * R::kValues + j);
             uint32_t v[2][2];
             four(value[j], scale[j], v[0], v[1]);
-            uint8_t *to = s_values[buffer] + ((b * 4 + g) * 2 + (k & 1)) * 512 + r * 16 + (k >> 1) * 8;
+            uint8_t *to = s_values[u & 1] + ((w.b * kGroups + w.g) * 2 + (w.k & 1)) * 512 + w.r * 16 + (w.k >> 1) * 8;
             *(uint2 *)to = make_uint2(v[0][0], v[0][1]);
             *(uint2 *)(to + 256) = make_uint2(v[1][0], v[1][1]);
         }
-        if (tid < 16 * kBlocks) s_scales[buffer][tid / 16][tid % 16] = key_scale;
     };
-
-    if (tid < 3 * kBlocks * 2) (&s_nan[0][0][0])[tid] = 0;
-    int page = -1, next_page = -1;
-    if (begin < end) {
-        fetch(begin, next_page);
-        __syncthreads();
-        stage(begin, next_page);
+    // turn j brings in unit j + 1's keys and unit j's values, and sends for the next ones; past the last unit it writes
+    // where nobody reads any more
+    int id_keys = id_of(0), id_values = id_keys, id_old = -1, id_next = id_of(1);
+    const uint8_t *tile_keys = tile_of(id_keys), *tile_values = tile_keys;
+    const auto stage = [&](int j, auto whole) {
+        stage_keys(j + 1);
+        stage_values(j, id_values, whole);
+        if (threadIdx.x < kBlocks) s_nan[(j + 2) & 3][threadIdx.x] = 0;  // read last in turn j - 1 of the later waves
+        id_old = id_values, id_values = id_keys, id_keys = id_next, id_next = id_of(j + 3);
+        tile_values = tile_keys, tile_keys = tile_of(id_keys);
+        fetch_keys(j + 2, tile_keys);
+        fetch_values(j + 1, tile_values);
+    };
+    if (threadIdx.x < 4 * kBlocks) s_nan[threadIdx.x / kBlocks][threadIdx.x % kBlocks] = 0;
+    if (units > 0) {
+        fetch_keys(0, tile_keys);
+        fetch_values(0, tile_values);
+        stage_keys(0);
+        id_keys = id_next, id_next = id_of(2);
+        tile_keys = tile_of(id_keys);
+        fetch_keys(1, tile_keys);
     }
-    for (int at = begin; at < end; at++) {
-        page = next_page;
-        __syncthreads();
-        if (tid < kBlocks * 2) s_nan[(at - begin + 2) % 3][tid / 2][tid % 2] = 0;
-        if (at + 1 < end) fetch(at + 1, next_page);
-        const int p0 = 64 * at, buffer = (at - begin) & 1, n32 = here(lane % 32), kq = here(lane / 32);
-        if (works && p0 <= w_last && p0 + 63 >= w_any) {
+    sm::lds_barrier();
+
+    // ----------------------------------------------------------------- turns
+    f32x16 s[kHalves];                         // S^T: positions 32 h + 8 (i / 4) + 4 kq + i % 4 of row n32
+    uint32_t p[R::kParts][kHalves][2][4] = {};  // the same positions' probabilities, as the second product takes them
+    const auto scores = [&](int u) {
+        const uint32_t l = here(lane);
+        const int n32 = l % 32, kq = l / 32, buffer = u & 1;
+        const int shift = n32 / 16 * 8 + (kTurns == 2 ? u % 2 * 16 : 0);
 #pragma unroll
-            for (int h0 = 0; h0 < 2; h0 += R::kHalves) {
-                // S^T: positions 32 h + 8 (i / 4) + 4 kq + i % 4 of row n32
-                f32x16 s[R::kHalves];
+        for (int h = 0; h < kHalves; h++) {
+            s[h] = f32x16{};
 #pragma unroll
-                for (int h = 0; h < R::kHalves; h++) {
-                    s[h] = f32x16{};
+            for (int c = 0; c < NC; c++) {
+                const u32x4 w = *(const u32x4 *)(s_keys[buffer] + R::slot(32 * h + n32, 2 * c + kq));
+                // byte 0 for the unit's lower half, 2 for its upper one
+                const uint32_t by = s_scales[buffer][2 * c + kq][n32 % 16] >> shift;
+                if constexpr (R::kF32) {
+                    const float f = scale_at(by, 2 * h);
 #pragma unroll
-                    for (int c = 0; c < NC; c++) {
-                        const u32x4 w = *(const u32x4 *)(s_keys[buffer] + R::slot(32 * (h0 + h) + n32, 2 * c + kq));
-                        // byte 0 or 1 for the lower half of the page, 2 or 3 for the upper one
-                        const float by = scale_at(s_scales[buffer][2 * c + kq][n32 % 16] >> (n32 / 16 * 8), 2 * (h0 + h));
+                    for (int t = 0; t < 4; t++) {
+                        const bf16x8 k = as_bf16(eight(w[t], f));
 #pragma unroll
-                        for (int t = 0; t < 4; t++) {
-                            const bf16x8 k = as_bf16(eight(w[t], by));
-#pragma unroll
-                            for (int p = R::kParts - 1; p >= 0; p--)
-                                s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                                    k, as_bf16(u32x4{q[p][c][t][0], q[p][c][t][1], q[p][c][t][2], q[p][c][t][3]}), s[h], 0, 0, 0);
-                        }
+                        for (int part = 2; part >= 0; part--)
+                            s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                                k, as_bf16(u32x4{q[part][c][4 * t], q[part][c][4 * t + 1], q[part][c][4 * t + 2], q[part][c][4 * t + 3]}),
+                                s[h], 0, 0, 0);
                     }
-                }
-                if (page < 0 || p0 < w_all || p0 + 63 > w_early) {
-                    const int from_t = page < 0 ? 64 : lo - p0 - 4 * kq, to_t = hi - p0 - 4 * kq;
+                } else {
+                    const i32x8 k = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
 #pragma unroll
-                    for (int h = 0; h < R::kHalves; h++)
+                    for (int part = 1; part >= 0; part--) {
+                        i32x8 x;
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int t = 32 * (h0 + h) + i / 4 * 8 + i % 4;
-                            if (t < from_t || t > to_t) s[h][i] = kNone;
-                        }
-                }
-                float top = kNone;
-#pragma unroll
-                for (int h = 0; h < R::kHalves; h++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) top = fmaxf(top, s[h][i]);
-                top = max_of_halves(top) * a.scale_log2;
-                if (__any(top > m + 8.0f || (m == kNone && top > kNone))) {
-                    const float to = fmaxf(m, top), by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
-                    m = to;
-                    sum *= by;
-#pragma unroll
-                    for (int b = 0; b < kBlocks; b++) o[b] *= by;
-                }
-                const float from = m == kNone ? 0.0f : -m;
-#pragma unroll
-                for (int h = 0; h < R::kHalves; h++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        s[h][i] = __builtin_amdgcn_exp2f(fmaf(s[h][i], a.scale_log2, from));
-                        sum += s[h][i];
+                        for (int j = 0; j < 8; j++) x[j] = (int)q[0][c][8 * part + j];
+                        // fp4 times e4m3
+                        if (h == 0) s[h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, x, s[h], 4, 0, 0, by, 0, q_scale - 4 * part);
+                        else s[h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, x, s[h], 4, 0, 2, by, 0, q_scale - 4 * part);
                     }
-                // O^T: dimensions 32 b + 8 (i / 4) + 4 kq + i % 4 of row n32
-#pragma unroll
-                for (int g = 0; g < 2 * R::kHalves; g++) {
-                    u32x4 p[R::kParts];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float x = s[g / 2][8 * (g % 2) + 2 * j], y = s[g / 2][8 * (g % 2) + 2 * j + 1];
-                        if constexpr (R::kF32) {
-                            uint32_t part[3];
-                            three_parts(x, y, part);
-#pragma unroll
-                            for (int t = 0; t < 3; t++) p[t][j] = part[t];
-                        } else {
-                            p[0][j] = kv4::bf16_pair(x, y);
-                        }
-                    }
-#pragma unroll
-                    for (int b = 0; b < kBlocks; b++) {
-                        const bf16x8 v =
-                            as_bf16(*(const u32x4 *)(s_values[buffer] + ((b * 4 + 2 * h0 + g) * 2 + kq) * 512 + n32 * 16));
-#pragma unroll
-                        for (int t = R::kParts - 1; t >= 0; t--)
-                            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, as_bf16(p[t]), o[b], 0, 0, 0);
-                    }
-                }
-            }
-            if (is_edge(at, page)) {
-#pragma unroll
-                for (int b = 0; b < kBlocks; b++) {
-                    const uint64_t nan = (uint64_t)s_nan[(at - begin) % 3][b][1] << 32 | s_nan[(at - begin) % 3][b][0];
-                    if (nan == 0) continue;
-                    // the row's positions of this page: bits from lo to hi
-                    const int from_bit = min(max(lo - p0, 0), 64), to_bit = min(max(hi + 1 - p0, 0), 64);
-                    const uint64_t below = to_bit == 64 ? ~0ull : (1ull << to_bit) - 1, above = from_bit == 64 ? 0ull : ~0ull << from_bit;
-                    if (nan & below & above)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[b][i] = NAN;
                 }
             }
         }
-        if (at + 1 < end) stage(at + 1, next_page);
+    };
+    const auto softmax = [&](int u, int id, auto whole) {
+        const int kq = here(lane / 32), p0 = position_of(u);
+        if (!whole && (id < 0 || p0 < w_all || p0 + kUnit - 1 > w_early)) {
+            const int from_t = id < 0 ? 64 : lo - p0 - 4 * kq, to_t = hi - p0 - 4 * kq;
+#pragma unroll
+            for (int h = 0; h < kHalves; h++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int t = 32 * h + i / 4 * 8 + i % 4;
+                    if (t < from_t || t > to_t) s[h][i] = kNone;
+                }
+        }
+        float top = kNone;
+#pragma unroll
+        for (int h = 0; h < kHalves; h++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, s[h][i]);
+        top = max_of_halves(top) * a.scale_log2;
+        // the maximum is raised once scores pass it by 2^8: any number near it does
+        if (__any(top > m + 8.0f || (m == kNone && top > kNone))) {
+            const float to = fmaxf(m, top), by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            sum *= by;
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++) o[b] *= by;
+        }
+        const float from = m == kNone ? 0.0f : -m;
+#pragma unroll
+        for (int h = 0; h < kHalves; h++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[h][2 * j], a.scale_log2, from));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[h][2 * j + 1], a.scale_log2, from));
+                if constexpr (R::kF32) {
+                    sum += x;
+                    sum += y;
+                    uint32_t part[3];
+                    three_parts(x, y, part);
+#pragma unroll
+                    for (int t = 0; t < 3; t++) p[t][h][j / 4][j % 4] = part[t];
+                } else {  // the sum of what the second product takes
+                    p[0][h][j / 4][j % 4] = kv4::bf16_pair(x, y);
+                    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p[0][h][j / 4][j % 4]), bf16x2{1.0f, 1.0f}, sum, false);
+                }
+            }
+    };
+    // O^T: dimensions 32 b + 8 (i / 4) + 4 kq + i % 4 of row n32
+    const auto products = [&](int u, auto whole) {
+        const uint32_t l = here(lane);
+        const int n32 = l % 32, kq = l / 32, p0 = position_of(u);
+        // a few blocks' values ahead of the products
+        constexpr int kSome = NC > 2 ? 2 : kBlocks, kSteps = kGroups * kBlocks / kSome;
+        u32x4 v[2][kSome];
+        const auto read = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < kSome; j++) {
+                const int g = i * kSome / kBlocks, b = i * kSome % kBlocks + j;
+                v[i & 1][j] = *(const u32x4 *)(s_values[u & 1] + ((b * kGroups + g) * 2 + kq) * 512 + n32 * 16);
+            }
+        };
+        read(0);
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) {
+            if (i + 1 < kSteps) read(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < kSome; j++) {
+                const int g = i * kSome / kBlocks, b = i * kSome % kBlocks + j;
+#pragma unroll
+                for (int t = R::kParts - 1; t >= 0; t--) {
+                    const uint32_t *x = p[t][g / 2][g % 2];
+                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(v[i & 1][j]), as_bf16(u32x4{x[0], x[1], x[2], x[3]}), o[b], 0, 0, 0);
+                }
+            }
+        }
+        if (!whole && (p0 < all_lo || p0 + kUnit - 1 > early)) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; b++) {
+                const uint64_t nan = s_nan[u & 3][b];
+                if (!__any(nan != 0)) continue;
+                // the row's positions of this unit: bits from lo to hi
+                const int from_bit = min(max(lo - p0, 0), 64), to_bit = min(max(hi + 1 - p0, 0), 64);
+                const uint64_t below = to_bit == 64 ? ~0ull : (1ull << to_bit) - 1, above = from_bit == 64 ? 0ull : ~0ull << from_bit;
+                const float poison = nan & below & above ? NAN : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[b][i] += poison;
+            }
+        }
+    };
+
+    const bool later = R::kWaves > 4 && wave >= 4;  // half a turn behind
+    const int behind = later ? 1 : 0;
+    const std::true_type whole;
+    const std::false_type any;
+    if (later && units > 0) {
+        stage(0, any);
+        sm::lds_barrier();
     }
-    if (32 * wave + n32 >= rows) return;
+    // units that are whole, and so are those beside them, go without questions
+    int u = 0, from = works ? min(whole_from + 1, units) : units, to = works ? whole_to - 1 : 0;
+    while (u < units) {
+        for (; u < from; u++) {
+            if (is_live(position_of(u))) scores(u);
+            if (u > 0 && is_live(position_of(u - 1))) products(u - 1, any);
+            sm::lds_barrier();
+            if (is_live(position_of(u))) softmax(u, later ? id_old : id_values, any);
+            stage(u + behind, any);
+            if (!later || u + 1 < units) sm::lds_barrier();
+        }
+        from = units;
+        for (; u < to && !holes; u++) {
+            scores(u);
+            products(u - 1, whole);
+            sm::lds_barrier();
+            softmax(u, 0, whole);
+            stage(u + behind, whole);
+            sm::lds_barrier();
+        }
+    }
+    if (units > 0 && is_live(position_of(units - 1))) products(units - 1, any);
+
+    if (32 * wave + (int)(lane % 32) >= rows) return;
+    const int kq = lane / 32;
     sum = sum_of_halves(sum);
-    const int64_t part = ((int64_t)blockIdx.y * gridDim.x + tile * a.kv_heads + head) * R::kRows + 32 * wave + n32;
+    const int64_t part = ((int64_t)blockIdx.y * gridDim.x + tile * a.kv_heads + head) * R::kRows + 32 * wave + lane % 32;
     const int64_t out = ((int64_t)(span.row + token) * a.heads + hq) * a.dim;
     const T *g = G ? G + (int64_t)(span.row + token) * a.g_view.stride + hq * a.g_view.head + a.g_view.offset : nullptr;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
