@@ -465,6 +465,7 @@ struct Prompt {
     static constexpr int kHalves = NC > 2 || (kF32 && NC > 1) ? 1 : 2;  // of a page in a unit: what registers hold
     static constexpr int kUnit = 32 * kHalves, kTurns = 64 / kUnit;
     static constexpr int kPieces = 2 * NC;  // of 16 bytes, of a key's codes
+    static constexpr bool kScoresFirst = NC < 3;
     // words of codes that are staged in a turn, and a thread's
     static constexpr int kKeyWords = kUnit * 4 * kPieces, kKeys = (kKeyWords + kThreads - 1) / kThreads;
     static constexpr int kValueWords = kBlocks * 128 * kHalves, kValues = (kValueWords + kThreads - 1) / kThreads;
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
                 if (turn == 1) {
                     // at least 2^-123, so that the lower part's scale is one
                     const int byte = max((int)f8::scale_byte(max_of_halves(amax)), 4);
-                    q_scale = byte, by = f8::inverse_scale(byte);
+                    q_scale = byte | (byte - 4) << 8, by = f8::inverse_scale(byte);  // byte 0 for the higher part, 1 for the lower
                 }
 #pragma unroll
                 for (int c = 0; c < NC; c++)
@@ -654,7 +655,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
                 for (int j = 0; j < R::kKeys; j++) *(uint32_t *)place(word + j) = key[j];
             }
         }
-        if (tid < 16 * kBlocks) (&s_scales[buffer][0][0])[tid] = key_scale;
+        *(uint32_t *)((uint8_t *)s_scales[buffer] + key_scale_at) = key_scale;  // threads past the last write the same
     };
     const auto stage_values = [&](int u, int id, auto whole) {
         const int p0 = position_of(u);
@@ -685,29 +686,27 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
             *(uint2 *)(to + 256) = make_uint2(v[1][0], v[1][1]);
         }
     };
-    // turn j brings in unit j + 1's keys and unit j's values, and sends for the next ones; past the last unit it writes
-    // where nobody reads any more
-    int id_keys = id_of(0), id_values = id_keys, id_old = -1, id_next = id_of(1);
-    const uint8_t *tile_keys = tile_of(id_keys), *tile_values = tile_keys;
-    const auto stage = [&](int j, auto whole) {
-        stage_keys(j + 1);
-        stage_values(j, id_values, whole);
-        if (threadIdx.x < kBlocks) s_nan[(j + 2) & 3][threadIdx.x] = 0;  // read last in turn j - 1 of the later waves
-        id_old = id_values, id_values = id_keys, id_keys = id_next, id_next = id_of(j + 3);
-        tile_values = tile_keys, tile_keys = tile_of(id_keys);
-        fetch_keys(j + 2, tile_keys);
-        fetch_values(j + 1, tile_values);
+    // unit u's turn brings in unit u + 1's keys and its own values, and sends for the next ones; past the last unit it
+    // writes where nobody reads any more
+    int id_now = -1, id_0 = id_of(0), id_1 = id_of(1), id_2 = id_of(2);  // pages of the unit at hand and of the next ones
+    const uint8_t *tile_values = tile_of(id_1), *tile_keys = tile_of(id_2);
+    const auto stage = [&](int u, auto whole) {
+        stage_keys(u + 1);
+        stage_values(u, id_0, whole);
+        fetch_keys(u + 2, tile_keys);
+        fetch_values(u + 1, tile_values);
+    };
+    const auto advance = [&](int u) {  // to the turn after unit u's
+        id_now = id_0, id_0 = id_1, id_1 = id_2, id_2 = id_of(u + 3);
+        tile_values = tile_keys, tile_keys = tile_of(id_2);
     };
     if (threadIdx.x < 4 * kBlocks) s_nan[threadIdx.x / kBlocks][threadIdx.x % kBlocks] = 0;
     if (units > 0) {
-        fetch_keys(0, tile_keys);
-        fetch_values(0, tile_values);
+        fetch_keys(0, tile_of(id_0));
+        fetch_values(0, tile_of(id_0));
         stage_keys(0);
-        id_keys = id_next, id_next = id_of(2);
-        tile_keys = tile_of(id_keys);
-        fetch_keys(1, tile_keys);
+        fetch_keys(1, tile_of(id_1));
     }
-    sm::lds_barrier();
 
     // ----------------------------------------------------------------- turns
     f32x16 s[kHalves];                         // S^T: positions 32 h + 8 (i / 4) + 4 kq + i % 4 of row n32
@@ -743,8 +742,16 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
 #pragma unroll
                         for (int j = 0; j < 8; j++) x[j] = (int)q[0][c][8 * part + j];
                         // fp4 times e4m3
-                        if (h == 0) s[h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, x, s[h], 4, 0, 0, by, 0, q_scale - 4 * part);
-                        else s[h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, x, s[h], 4, 0, 2, by, 0, q_scale - 4 * part);
+                        const auto product = [&](auto k_byte, auto q_byte) {
+                            s[h] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k, x, s[h], 4, 0, k_byte, by, q_byte, q_scale);
+                        };
+                        const std::integral_constant<int, 0> b0;
+                        const std::integral_constant<int, 1> b1;
+                        const std::integral_constant<int, 2> b2;
+                        if (h == 0 && part == 0) product(b0, b0);
+                        if (h == 0 && part == 1) product(b0, b1);
+                        if (h == 1 && part == 0) product(b2, b0);
+                        if (h == 1 && part == 1) product(b2, b1);
                     }
                 }
             }
@@ -777,52 +784,47 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
             for (int b = 0; b < kBlocks; b++) o[b] *= by;
         }
         const float from = m == kNone ? 0.0f : -m;
+        float sums[2] = {sum, 0.0f};
 #pragma unroll
         for (int h = 0; h < kHalves; h++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(s[h][2 * j], a.scale_log2, from));
                 const float y = __builtin_amdgcn_exp2f(fmaf(s[h][2 * j + 1], a.scale_log2, from));
+                sums[j % 2] += x;
+                sums[j % 2] += y;
                 if constexpr (R::kF32) {
-                    sum += x;
-                    sum += y;
                     uint32_t part[3];
                     three_parts(x, y, part);
 #pragma unroll
                     for (int t = 0; t < 3; t++) p[t][h][j / 4][j % 4] = part[t];
-                } else {  // the sum of what the second product takes
+                } else {
                     p[0][h][j / 4][j % 4] = kv4::bf16_pair(x, y);
-                    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p[0][h][j / 4][j % 4]), bf16x2{1.0f, 1.0f}, sum, false);
                 }
             }
+        sum = sums[0] + sums[1];
     };
     // O^T: dimensions 32 b + 8 (i / 4) + 4 kq + i % 4 of row n32
     const auto products = [&](int u, auto whole) {
         const uint32_t l = here(lane);
         const int n32 = l % 32, kq = l / 32, p0 = position_of(u);
-        // a few blocks' values ahead of the products
-        constexpr int kSome = NC > 2 ? 2 : kBlocks, kSteps = kGroups * kBlocks / kSome;
-        u32x4 v[2][kSome];
+        // a block's values are read some products ahead: longer than LDS takes to answer
+        constexpr int kAhead = 4, kSteps = kGroups * kBlocks;
+        u32x4 v[kAhead];
         const auto read = [&](int i) {
-#pragma unroll
-            for (int j = 0; j < kSome; j++) {
-                const int g = i * kSome / kBlocks, b = i * kSome % kBlocks + j;
-                v[i & 1][j] = *(const u32x4 *)(s_values[u & 1] + ((b * kGroups + g) * 2 + kq) * 512 + n32 * 16);
-            }
+            v[i % kAhead] = *(const u32x4 *)(s_values[u & 1] + ((i % kBlocks * kGroups + i / kBlocks) * 2 + kq) * 512 + n32 * 16);
         };
-        read(0);
+#pragma unroll
+        for (int i = 0; i < kAhead - 1; i++) read(i);
 #pragma unroll
         for (int i = 0; i < kSteps; i++) {
-            if (i + 1 < kSteps) read(i + 1);
-            __builtin_amdgcn_sched_barrier(0);
+            if (i + kAhead - 1 < kSteps) read(i + kAhead - 1);
+            if (NC < 3) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < kSome; j++) {
-                const int g = i * kSome / kBlocks, b = i * kSome % kBlocks + j;
-#pragma unroll
-                for (int t = R::kParts - 1; t >= 0; t--) {
-                    const uint32_t *x = p[t][g / 2][g % 2];
-                    o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(v[i & 1][j]), as_bf16(u32x4{x[0], x[1], x[2], x[3]}), o[b], 0, 0, 0);
-                }
+            for (int t = R::kParts - 1; t >= 0; t--) {
+                const uint32_t *x = p[t][i / kBlocks / 2][i / kBlocks % 2];
+                o[i % kBlocks] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16(v[i % kAhead]), as_bf16(u32x4{x[0], x[1], x[2], x[3]}),
+                                                                         o[i % kBlocks], 0, 0, 0);
             }
         }
         if (!whole && (p0 < all_lo || p0 + kUnit - 1 > early)) {
@@ -840,32 +842,36 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
         }
     };
 
-    const bool later = R::kWaves > 4 && wave >= 4;  // half a turn behind
-    const int behind = later ? 1 : 0;
     const std::true_type whole;
     const std::false_type any;
-    if (later && units > 0) {
-        stage(0, any);
+    const bool later = R::kWaves > 4 && wave >= 4;  // half a turn behind
+    if (units > 0) {
         sm::lds_barrier();
+        if (later) sm::lds_barrier();
     }
     // units that are whole, and so are those beside them, go without questions
     int u = 0, from = works ? min(whole_from + 1, units) : units, to = works ? whole_to - 1 : 0;
     while (u < units) {
         for (; u < from; u++) {
-            if (is_live(position_of(u))) scores(u);
+            if (threadIdx.x < kBlocks) s_nan[(u + 1) & 3][threadIdx.x] = 0;  // the next unit's
+            stage(u, any);
+            if (R::kScoresFirst && is_live(position_of(u))) scores(u);
             if (u > 0 && is_live(position_of(u - 1))) products(u - 1, any);
+            if (!R::kScoresFirst && is_live(position_of(u))) scores(u);
             sm::lds_barrier();
-            if (is_live(position_of(u))) softmax(u, later ? id_old : id_values, any);
-            stage(u + behind, any);
+            advance(u);
+            if (is_live(position_of(u))) softmax(u, id_now, any);
             if (!later || u + 1 < units) sm::lds_barrier();
         }
         from = units;
         for (; u < to && !holes; u++) {
-            scores(u);
+            if (R::kScoresFirst) scores(u);
+            stage(u, whole);
             products(u - 1, whole);
+            if (!R::kScoresFirst) scores(u);
             sm::lds_barrier();
+            advance(u);
             softmax(u, 0, whole);
-            stage(u + behind, whole);
             sm::lds_barrier();
         }
     }
