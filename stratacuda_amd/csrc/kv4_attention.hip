@@ -84,46 +84,49 @@ __device__ __forceinline__ int2 pages_of(const kv4::Span &a, int window) {
     const int lo = window > 0 ? max(first - window + 1, 0) / 64 : 0;
     return make_int2(lo, max((a.length + 63) / 64, lo));
 }
+__device__ __forceinline__ int pieces_in(const int2 &p, int n, int each) { return n > 0 ? max((p.y - p.x + each - 1) / each, 1) : 0; }
 __device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int least, int slot) {
     const int lane = threadIdx.x % 64;
-    int total = 0;
+    const auto sequence = [&](int s, int &n) {
+        n = 0;
+        if (s >= q.count) return make_int2(0, 0);
+        const kv4::Span a = kv4::span(q, s);
+        n = a.n;
+        return pages_of(a, window);
+    };
+    int n, n0, total = 0;
+    int2 p, p0 = sequence(lane, n0);
     for (int at = 0; at < q.count; at += 64) {
-        int n = 0;
-        if (at + lane < q.count) {
-            const kv4::Span a = kv4::span(q, at + lane);
-            const int2 p = pages_of(a, window);
-            n = a.n > 0 ? p.y - p.x : 0;
-        }
+        p = at == 0 ? p0 : sequence(at + lane, n);
+        if (at == 0) n = n0;
+        int some = n > 0 ? p.y - p.x : 0;
+        if (q.count > 1)
 #pragma unroll
-        for (int i = 1; i < 64; i *= 2) n += __shfl_xor(n, i, 64);
-        total += n;
+            for (int i = 1; i < 64; i *= 2) some += __shfl_xor(some, i, 64);
+        total += __builtin_amdgcn_readfirstlane(some);
     }
     const int each = max(least, (total + pieces - 1) / pieces);
     int before = 0;
     for (int at = 0; at < q.count; at += 64) {
-        int n = 0;
-        int2 p = make_int2(0, 0);
-        if (at + lane < q.count) {
-            const kv4::Span a = kv4::span(q, at + lane);
-            p = pages_of(a, window);
-            n = a.n > 0 ? max((p.y - p.x + each - 1) / each, 1) : 0;
-        }
-        int upto = n;  // with this lane's
+        p = at == 0 ? p0 : sequence(at + lane, n);
+        if (at == 0) n = n0;
+        const int mine = pieces_in(p, n, each);
+        int upto = mine;  // with this lane's
+        if (q.count > 1)
 #pragma unroll
-        for (int i = 1; i < 64; i *= 2) {
-            const int other = __shfl_up(upto, i, 64);
-            if (lane >= i) upto += other;
-        }
-        const uint64_t past = __ballot(before + upto > slot);
+            for (int i = 1; i < 64; i *= 2) {
+                const int other = __shfl_up(upto, i, 64);
+                if (lane >= i) upto += other;
+            }
+        const uint64_t past = __ballot(before + upto > slot && mine > 0);
         if (past) {
             const int who = __ffsll((unsigned long long)past) - 1;
-            const int count = __shfl(n, who, 64), number = slot - before - (__shfl(upto, who, 64) - count);
-            const int first = __shfl(p.x, who, 64), end = __shfl(p.y, who, 64);
             // the same in all lanes: kept, and what it leads to, in scalar registers
-            const auto one = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-            return {one(at + who), one(first + number * each), one(min(first + (number + 1) * each, end)), one(number), one(count)};
+            const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
+            const int count = of(mine), number = slot - before - (of(upto) - count), first = of(p.x), end = of(p.y);
+            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count};
         }
-        before += __shfl(upto, 63, 64);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return {-1, 0, 0, 0, 0};
 }
