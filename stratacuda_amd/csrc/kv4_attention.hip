@@ -148,6 +148,7 @@ struct Rows16 {
     static constexpr int kChunks = kWide ? NC / 2 : NC;   // loads of a key
     static constexpr int kSteps = kWide ? 4 : 2;          // matrix steps of 32 dimensions of each
     static constexpr int kParts = F32 ? 3 : 1;
+    static constexpr int kWavesOfSimd = F32 && NC > 2 ? 1 : 2;  // at least: what their registers leave
 
     struct Keys {
         uint32_t codes[4][kChunks][kSteps];  // of positions 16 g + lane % 16
@@ -208,12 +209,14 @@ __device__ __forceinline__ void four(uint32_t w, uint32_t scales, uint32_t low[2
 }
 
 template <int NC, typename T>
-__global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, const uint8_t *pool, const T *G, T *Y, float *parts,
-                                                  float2 *stats, int tiles) {
+__global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd)) k_kv4_rows(Kv4Attention a, const T *Q, const uint8_t *pool,
+                                                                                            const T *G, T *Y, float *parts, float2 *stats,
+                                                                                            int tiles) {
     constexpr bool F32 = sizeof(T) == 4;
     using R = Rows16<NC, F32>;
     constexpr int kPitch = R::kPitch, kTiles = kPitch / 16, kLine = kPitch + 4;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, n16 = lane % 16, kq = lane / 16;
+    const uint32_t lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const Piece piece = piece_of(a.q, a.window, a.pieces, a.least, blockIdx.y);
     if (piece.s < 0) return;
     if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
@@ -223,15 +226,25 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
     if (rows <= 0) return;
     const int first = span.length - span.n;       // the first new token's position
 
-    // this lane's row, the last one's once more past it; its positions lo .. hi
-    const int row = 16 * tile + min(n16, rows - 1), token = row / group, hq = head * group + row % group;
-    const int hi = first + token, lo = a.window > 0 ? max(hi - a.window + 1, 0) : 0;
-    // the tile's: those that any row has, and that all rows have
+    // the tile's rows: the first and last one's position, the lowest position of any, of all
     const int last = first + (16 * tile + min(15, rows - 1)) / group, early = first + 16 * tile / group;
     const int any_lo = a.window > 0 ? max(early - a.window + 1, 0) : 0, all_lo = a.window > 0 ? max(last - a.window + 1, 0) : 0;
     const int begin = max(piece.first, any_lo / 64), end = min(piece.end, (last >> 6) + 1);
+    // this wave's pages: begin + wave + 4 i; their numbers, a lane's each, of 64
+    const int mine = (end - begin - wave + 3) / 4, start = begin + wave;
+    int ids = -1;
+    const auto id_of = [&](int i) {
+        if (i % 64 == 0) {
+            const int at = start + 4 * (i + (int)lane);
+            ids = at < end ? kv4::page_of(a.q, piece.s, at, a.pages) : -1;
+        }
+        return __builtin_amdgcn_readlane(ids, i % 64);
+    };
+    int page = mine > 0 ? id_of(0) : -1;
 
-    // queries
+    // this lane's row, the last one's once more past it; its positions lo .. hi
+    const int row = 16 * tile + min((int)(lane % 16), rows - 1), token = row / group, hq = head * group + row % group;
+    const int hi = first + token, lo = a.window > 0 ? max(hi - a.window + 1, 0) : 0;
     uint32_t q[R::kParts][R::kChunks][R::kSteps][4];
     {
         const T *x = Q + (int64_t)(span.row + token) * a.q_view.stride + hq * a.q_view.head + a.q_view.offset;
@@ -239,7 +252,7 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
         for (int c = 0; c < R::kChunks; c++)
 #pragma unroll
             for (int s = 0; s < R::kSteps; s++) {
-                const int d = R::dimension(c, s, kq);
+                const int d = R::dimension(c, s, lane / 16);
                 float v[8] = {};
                 if (d < a.dim) kv4::load8(x + d, a.vec, v);
 #pragma unroll
@@ -265,13 +278,10 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
     typename R::Values values;
     const int64_t step = (int64_t)a.kv_heads * (68 * kPitch);
     const uint8_t *base = pool + (int64_t)head * (68 * kPitch);
-    int at = begin + wave, page = at < end ? kv4::page_of(a.q, piece.s, at, a.pages) : -1;
-    if (at < end) {
-        R::load(keys, base + max(page, 0) * step, lane);
-        R::load(values, base + max(page, 0) * step, lane);
-    }
-    for (; at < end; at += 4) {
-        // S^T: positions 16 g + 4 kq + i of row n16
+    const auto tile_of = [&](int id) { return base + max(id, 0) * step; };
+    // page i of the wave; `whole`: every row has all its positions, and another page follows
+    const auto turn = [&](int i, auto whole) {
+        // S^T: positions 16 g + 4 kq + i of row lane % 16
         f32x4 s[4];
 #pragma unroll
         for (int g = 0; g < 4; g++) {
@@ -289,15 +299,16 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
                 }
             }
         }
-        const int now = page, next = at + 4;
-        if (next < end) {
-            page = kv4::page_of(a.q, piece.s, next, a.pages);
-            R::load(keys, base + max(page, 0) * step, lane);
+        const int now = page, p0 = 64 * (start + 4 * i);
+        const bool more = whole || i + 1 < mine;
+        if (more) {
+            page = id_of(i + 1);
+            R::load(keys, tile_of(page), here(lane));
         }
-        const int p0 = 64 * at;
-        const bool edge = now < 0 || p0 < all_lo || p0 + 63 > early;  // a position that some row does not have
+        const bool edge = !whole && (now < 0 || p0 < all_lo || p0 + 63 > early);  // a position that some row does not have
         bool poisoned = false;
         if (edge) {
+            const int kq = here(lane) / 16;
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 uint32_t kept = 0;
@@ -344,6 +355,7 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
             }
         uint32_t poison = 0;  // bit b: a block b of NaN at a position that the row has
         if (poisoned) {
+            const int kq = here(lane) / 16;
 #pragma unroll
             for (int b = 0; b < R::kBlocks; b++)
 #pragma unroll
@@ -351,8 +363,7 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int t = p0 + 16 * g + 4 * kq + i;
-                        uint32_t any = (values.scales[b][g] >> (8 * i) & 255u) == 255u;
-                        if (!any) continue;
+                        if ((values.scales[b][g] >> (8 * i) & 255u) != 255u) continue;
                         values.scales[b][g] ^= 0x80u << (8 * i);
                         // the scales are those of this quarter's positions, the same in its 16 lanes: each its own row
                         if (t >= lo && t <= hi) poison |= 1u << b;
@@ -360,7 +371,7 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
             poison |= __shfl_xor(poison, 16, 64);
             poison |= __shfl_xor(poison, 32, 64);
         }
-        // O^T: dimensions 16 t + 4 kq + i of row n16
+        // O^T: dimensions 16 t + 4 kq + i of row lane % 16
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
             u32x4 p[R::kParts];
@@ -390,20 +401,32 @@ __global__ void __launch_bounds__(256) k_kv4_rows(Kv4Attention a, const T *Q, co
                 }
             }
         }
-        if (poison) {
+        if (!whole && poison) {
 #pragma unroll
             for (int b = 0; b < R::kBlocks; b++)
                 if (poison >> b & 1) o[2 * b] = o[2 * b + 1] = f32x4{NAN, NAN, NAN, NAN};
         }
-        if (next < end) R::load(values, base + max(page, 0) * step, lane);
+        if (more) R::load(values, tile_of(page), here(lane));
+    };
+    if (mine > 0) {
+        R::load(keys, tile_of(page), lane);
+        R::load(values, tile_of(page), lane);
+    }
+    // the wave's pages that are whole: from the first at or past all_lo to the last that ends at or before `early`, and not its last
+    const int whole_from = max((all_lo + 63) / 64 - start + 3, 0) / 4, whole_to = min(((early + 1) / 64 - start + 3) / 4, mine - 1);
+    int i = 0, from = whole_from < whole_to ? whole_from : mine;
+    while (i < mine) {
+        for (; i < from; i++) turn(i, std::false_type());
+        from = mine;
+        for (; i < whole_to && page >= 0; i++) turn(i, std::true_type());
     }
 
     // the four waves' sums meet
     __shared__ float s_o[4][16][kLine], s_m[4][16], s_sum[4][16];
     sum = sum_of_quarters(sum);
 #pragma unroll
-    for (int t = 0; t < kTiles; t++) *(f32x4 *)&s_o[wave][n16][16 * t + 4 * kq] = o[t];
-    if (kq == 0) s_m[wave][n16] = m, s_sum[wave][n16] = sum;
+    for (int t = 0; t < kTiles; t++) *(f32x4 *)&s_o[wave][lane % 16][16 * t + lane / 16 * 4] = o[t];
+    if (lane < 16) s_m[wave][lane] = m, s_sum[wave][lane] = sum;
     __syncthreads();
     const int r = threadIdx.x / 16, d0 = threadIdx.x % 16 * 4;
     if (r >= rows) return;
@@ -910,35 +933,37 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
 
 // ------------------------------------------------------------ pieces joined
 // The pieces of one row: its sequence's partial sums, each brought to the
-// largest of their maxima. Eight waves a row take the pieces in turn.
-constexpr int kJoinWaves = 8;
-template <int NC, typename T>
-__global__ void __launch_bounds__(64 * kJoinWaves) k_kv4_join(Kv4Attention a, const T *G, T *Y, const float *parts,
-                                                              const float2 *stats, const int2 *info, int tiles, int tile_rows) {
-    constexpr int kPitch = 64 * NC;
+// largest of their maxima. kWaves waves a row take some pieces in turn; with
+// one, four rows a workgroup.
+template <int NC, typename T, int kWaves>
+__global__ void __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) k_kv4_join(Kv4Attention a, const T *G, T *Y, const float *parts,
+                                                                              const float2 *stats, const int2 *info, int tiles,
+                                                                              int tile_rows) {
+    constexpr int kPitch = 64 * NC, kSome = kWaves == 1 ? 4 : 8;
     const int s = blockIdx.y, group = a.heads / a.kv_heads;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int number = kWaves == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    const int token = number / a.heads, h = number % a.heads;
     const kv4::Span span = kv4::span(a.q, s);
-    const int token = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
     if (token >= span.n) return;
     const int2 pieces = info[s];  // the first, how many
     if (pieces.y <= 1) return;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int head = h / group, row = token * group + h % group;
     const int64_t step = (int64_t)a.kv_heads * tiles * tile_rows;
     const int64_t base = ((int64_t)row / tile_rows * a.kv_heads + head) * tile_rows + row % tile_rows + pieces.x * step;
     float top = kNone, all = 0.0f, v[NC] = {};
-    for (int c0 = 4 * wave; c0 < pieces.y; c0 += 4 * kJoinWaves) {
-        float2 st[4];
-        float x[4][NC];
+    for (int c0 = kWaves == 1 ? 0 : kSome * wave; c0 < pieces.y; c0 += kSome * kWaves) {
+        float2 st[kSome];
+        float x[kSome][NC];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < kSome; j++) {
             const int64_t at = base + min(c0 + j, pieces.y - 1) * step;
             st[j] = stats[at];
 #pragma unroll
-            for (int n = 0; n < NC; n++) x[j][n] = parts[at * kPitch + 64 * n + lane];
+            for (int n = 0; n < NC; n++) x[j][n] = parts[at * kPitch + NC * lane + n];
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < kSome; j++) {
             if (c0 + j >= pieces.y) break;
             const float to = fmaxf(top, st[j].x);
             const float was = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(top - to);
@@ -950,32 +975,45 @@ __global__ void __launch_bounds__(64 * kJoinWaves) k_kv4_join(Kv4Attention a, co
             top = to;
         }
     }
-    __shared__ float s_v[kJoinWaves][kPitch], s_top[kJoinWaves], s_all[kJoinWaves];
+    if constexpr (kWaves > 1) {
+        __shared__ float s_v[kWaves][kPitch], s_top[kWaves], s_all[kWaves];
 #pragma unroll
-    for (int n = 0; n < NC; n++) s_v[wave][64 * n + lane] = v[n];
-    if (lane == 0) s_top[wave] = top, s_all[wave] = all;
-    __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= a.dim) return;
-    top = s_top[0], all = 0.0f;
+        for (int n = 0; n < NC; n++) s_v[wave][NC * lane + n] = v[n];
+        if (lane == 0) s_top[wave] = top, s_all[wave] = all;
+        __syncthreads();
+        if (wave > 0) return;
+        top = s_top[0];
 #pragma unroll
-    for (int w = 1; w < kJoinWaves; w++) top = fmaxf(top, s_top[w]);
-    float y = 0.0f;
+        for (int w = 1; w < kWaves; w++) top = fmaxf(top, s_top[w]);
+        all = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kJoinWaves; w++) {
-        const float by = s_top[w] == kNone ? 0.0f : __builtin_amdgcn_exp2f(s_top[w] - top);
-        all += s_top[w] == kNone ? s_all[w] : s_all[w] * by;
-        y += s_v[w][d] * by;
+        for (int n = 0; n < NC; n++) v[n] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float by = s_top[w] == kNone ? 0.0f : __builtin_amdgcn_exp2f(s_top[w] - top);
+            all += s_top[w] == kNone ? s_all[w] : s_all[w] * by;
+#pragma unroll
+            for (int n = 0; n < NC; n++) v[n] += s_v[w][NC * lane + n] * by;
+        }
     }
-    y = all == 0.0f ? 0.0f : y / all;
-    if (G) y = gated(y, kv4::value(G[(int64_t)(span.row + token) * a.g_view.stride + h * a.g_view.head + a.g_view.offset + d]));
-    kv4::store1(Y + ((int64_t)(span.row + token) * a.heads + h) * a.dim + d, y);
+    const T *g = G ? G + (int64_t)(span.row + token) * a.g_view.stride + h * a.g_view.head + a.g_view.offset : nullptr;
+    T *y = Y + ((int64_t)(span.row + token) * a.heads + h) * a.dim;
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        const int d = NC * lane + n;
+        if (d >= a.dim) break;
+        const float out = all == 0.0f ? 0.0f : v[n] / all;
+        kv4::store1(y + d, g ? gated(out, kv4::value(g[d])) : out);
+    }
 }
 
 // Workgroups that fill the GPU, and the least pages that are worth a piece.
-constexpr int kWorkgroups = 512, kLeast = 4;
+constexpr int kWorkgroups = 256, kLeast = 4;
 // From so many rows of a key-value head on a workgroup of prompts.
 constexpr int kPromptRows = 64;
+
+// Up to so many pieces one wave joins a row's.
+constexpr int kJoinAlone = 12;
 
 struct Shape {
     bool prompt;
@@ -1015,9 +1053,12 @@ void launch(sm_ctx *ctx, Kv4Attention a, const Shape &s, const T *Q, const uint8
     const dim3 grid((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots);
     if (s.prompt) k_kv4_prompt<NC, T><<<grid, Prompt<NC, T>::kThreads, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
     else k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
-    if (s.pieces > 1)
-        k_kv4_join<NC, T><<<dim3((uint32_t)a.q.longest * a.heads, a.q.count), 64 * kJoinWaves, 0, ctx->stream>>>(
-            a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
+    if (s.pieces == 1) return;
+    const uint32_t all = (uint32_t)a.q.longest * a.heads;
+    if (s.pieces > kJoinAlone)
+        k_kv4_join<NC, T, 16><<<dim3(all, a.q.count), 1024, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
+    else
+        k_kv4_join<NC, T, 1><<<dim3((all + 3) / 4, a.q.count), 256, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
 }
 template <typename T>
 void launch(sm_ctx *ctx, const Kv4Attention &a, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
