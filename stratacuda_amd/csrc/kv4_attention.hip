@@ -11,6 +11,7 @@
 // the sum of three bf16 numbers (8 significant bits each, so all 24) and cost
 // three matrix instructions. For bf16 the probabilities are rounded to bf16,
 // half a step of 2^-8 relative, like the result; sums are f32's.
+#include <algorithm>
 #include <type_traits>
 
 #include "kv4_device.h"
@@ -77,6 +78,7 @@ __device__ __forceinline__ float sum_of_halves(float v) {
 struct Piece {
     int s, first, end;  // the sequence and the pages; s = -1: there is no such piece
     int number, count;  // which of the sequence's pieces it is
+    kv4::Span span;
 };
 // The pages that the sequence's rows reach.
 __device__ __forceinline__ int2 pages_of(const kv4::Span &a, int window) {
@@ -87,19 +89,13 @@ __device__ __forceinline__ int2 pages_of(const kv4::Span &a, int window) {
 __device__ __forceinline__ int pieces_in(const int2 &p, int n, int each) { return n > 0 ? max((p.y - p.x + each - 1) / each, 1) : 0; }
 __device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int least, int slot) {
     const int lane = threadIdx.x % 64;
-    const auto sequence = [&](int s, int &n) {
-        n = 0;
-        if (s >= q.count) return make_int2(0, 0);
-        const kv4::Span a = kv4::span(q, s);
-        n = a.n;
-        return pages_of(a, window);
-    };
-    int n, n0, total = 0;
-    int2 p, p0 = sequence(lane, n0);
+    const auto sequence = [&](int s) { return s < q.count ? kv4::span(q, s) : kv4::Span{0, 0, 0}; };
+    int total = 0;
+    const kv4::Span a0 = sequence(lane);
     for (int at = 0; at < q.count; at += 64) {
-        p = at == 0 ? p0 : sequence(at + lane, n);
-        if (at == 0) n = n0;
-        int some = n > 0 ? p.y - p.x : 0;
+        const kv4::Span a = at == 0 ? a0 : sequence(at + lane);
+        const int2 p = pages_of(a, window);
+        int some = a.n > 0 ? p.y - p.x : 0;
         if (q.count > 1)
 #pragma unroll
             for (int i = 1; i < 64; i *= 2) some += __shfl_xor(some, i, 64);
@@ -108,9 +104,9 @@ __device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int lea
     const int each = max(least, (total + pieces - 1) / pieces);
     int before = 0;
     for (int at = 0; at < q.count; at += 64) {
-        p = at == 0 ? p0 : sequence(at + lane, n);
-        if (at == 0) n = n0;
-        const int mine = pieces_in(p, n, each);
+        const kv4::Span a = at == 0 ? a0 : sequence(at + lane);
+        const int2 p = pages_of(a, window);
+        const int mine = pieces_in(p, a.n, each);
         int upto = mine;  // with this lane's
         if (q.count > 1)
 #pragma unroll
@@ -124,11 +120,12 @@ __device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int lea
             // the same in all lanes: kept, and what it leads to, in scalar registers
             const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
             const int count = of(mine), number = slot - before - (of(upto) - count), first = of(p.x), end = of(p.y);
-            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count};
+            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count,
+                    {of(a.row), of(a.n), of(a.length)}};
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
-    return {-1, 0, 0, 0, 0};
+    return {-1, 0, 0, 0, 0, {0, 0, 0}};
 }
 
 // ------------------------------------------------------------------ 16 rows
@@ -220,7 +217,7 @@ __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd
     const Piece piece = piece_of(a.q, a.window, a.pieces, a.least, blockIdx.y);
     if (piece.s < 0) return;
     if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
-    const kv4::Span span = kv4::span(a.q, piece.s);
+    const kv4::Span span = piece.span;
     const int head = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
     const int rows = span.n * group - 16 * tile;  // of the sequence, from this tile's first on
     if (rows <= 0) return;
@@ -486,8 +483,9 @@ template <int NC, typename T>
 struct Prompt {
     static constexpr bool kF32 = sizeof(T) == 4;
     static constexpr int kPitch = 64 * NC, kBlocks = 2 * NC, kParts = kF32 ? 3 : 1;
-    // f32 queries of 192 dimensions and more take most of a SIMD's registers: one wave on each
-    static constexpr int kWaves = kF32 && NC > 2 ? 4 : 8, kThreads = 64 * kWaves, kRows = 32 * kWaves;
+    // f32 queries of more than 128 dimensions would take more registers than two waves of a SIMD have
+    static constexpr bool kThere = !kF32 || NC < 3;
+    static constexpr int kWaves = 8, kThreads = 64 * kWaves, kRows = 32 * kWaves;
     static constexpr int kHalves = NC > 2 || (kF32 && NC > 1) ? 1 : 2;  // of a page in a unit: what registers hold
     static constexpr int kUnit = 32 * kHalves, kTurns = 64 / kUnit;
     static constexpr int kPieces = 2 * NC;  // of 16 bytes, of a key's codes
@@ -517,7 +515,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
     const Piece piece = piece_of(a.q, a.window, a.pieces, a.least, blockIdx.y);
     if (piece.s < 0) return;
     if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
-    const kv4::Span span = kv4::span(a.q, piece.s);
+    const kv4::Span span = piece.span;
     // the longest rows first
     const int head = blockIdx.x % a.kv_heads, tile = tiles - 1 - blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
     const int rows = span.n * group - R::kRows * tile;
@@ -870,7 +868,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
 
     const std::true_type whole;
     const std::false_type any;
-    const bool later = R::kWaves > 4 && wave >= 4;  // half a turn behind
+    const bool later = wave >= 4;  // half a turn behind
     if (units > 0) {
         sm::lds_barrier();
         if (later) sm::lds_barrier();
@@ -916,7 +914,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
         for (int i = 0; i < 16; i += 4) {
             const int d = 32 * b + 2 * i + 4 * kq;
             if (piece.count > 1) {
-                *(f32x4 *)(parts + part * kPitch + d) = f32x4{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
+                if (units > 0) *(f32x4 *)(parts + part * kPitch + d) = f32x4{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
             } else if (d < a.dim) {
                 float y[4];
 #pragma unroll
@@ -933,13 +931,13 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
 
 // ------------------------------------------------------------ pieces joined
 // The pieces of one row: its sequence's partial sums, each brought to the
-// largest of their maxima. kWaves waves a row take some pieces in turn; with
-// one, four rows a workgroup.
+// largest of their maxima. kWaves waves a row share out the pieces; with one,
+// four rows a workgroup.
 template <int NC, typename T, int kWaves>
 __global__ void __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) k_kv4_join(Kv4Attention a, const T *G, T *Y, const float *parts,
                                                                               const float2 *stats, const int2 *info, int tiles,
                                                                               int tile_rows) {
-    constexpr int kPitch = 64 * NC, kSome = kWaves == 1 ? 4 : 8;
+    constexpr int kPitch = 64 * NC, kSome = 8;
     const int s = blockIdx.y, group = a.heads / a.kv_heads;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int number = kWaves == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
@@ -952,28 +950,38 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) k_kv4_join(Kv
     const int64_t step = (int64_t)a.kv_heads * tiles * tile_rows;
     const int64_t base = ((int64_t)row / tile_rows * a.kv_heads + head) * tile_rows + row % tile_rows + pieces.x * step;
     float top = kNone, all = 0.0f, v[NC] = {};
-    for (int c0 = kWaves == 1 ? 0 : kSome * wave; c0 < pieces.y; c0 += kSome * kWaves) {
+    const int share = (pieces.y + kWaves - 1) / kWaves, from = kWaves == 1 ? 0 : wave * share, end = min(from + share, pieces.y);
+    for (int c0 = from; c0 < end; c0 += kSome) {
         float2 st[kSome];
         float x[kSome][NC];
 #pragma unroll
         for (int j = 0; j < kSome; j++) {
-            const int64_t at = base + min(c0 + j, pieces.y - 1) * step;
+            const int64_t at = base + min(c0 + j, end - 1) * step;
             st[j] = stats[at];
 #pragma unroll
             for (int n = 0; n < NC; n++) x[j][n] = parts[at * kPitch + NC * lane + n];
         }
+        float to = top;
+#pragma unroll
+        for (int j = 0; j < kSome; j++) to = fmaxf(to, st[j].x);  // those past the end repeat the last one
+        const float was = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(top - to);
+        all *= was;
+#pragma unroll
+        for (int n = 0; n < NC; n++) v[n] *= was;
 #pragma unroll
         for (int j = 0; j < kSome; j++) {
-            if (c0 + j >= pieces.y) break;
-            const float to = fmaxf(top, st[j].x);
-            const float was = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(top - to);
-            const float by = st[j].x == kNone ? 0.0f : __builtin_amdgcn_exp2f(st[j].x - to);
-            // a sum that is not a number, of scores that are none, stays one
-            all = all * was + (st[j].x == kNone ? (st[j].y == 0.0f ? 0.0f : NAN) : st[j].y * by);
+            if (c0 + j >= end) break;
+            // a sum that is not a number, of scores that are none, stays one; else such a piece has left no values
+            if (st[j].x == kNone) {
+                all += st[j].y == 0.0f ? 0.0f : NAN;
+                continue;
+            }
+            const float by = __builtin_amdgcn_exp2f(st[j].x - to);
+            all += st[j].y * by;
 #pragma unroll
-            for (int n = 0; n < NC; n++) v[n] = v[n] * was + x[j][n] * by;
-            top = to;
+            for (int n = 0; n < NC; n++) v[n] += x[j][n] * by;
         }
+        top = to;
     }
     if constexpr (kWaves > 1) {
         __shared__ float s_v[kWaves][kPitch], s_top[kWaves], s_all[kWaves];
@@ -1007,33 +1015,47 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) k_kv4_join(Kv
     }
 }
 
-// Workgroups that fill the GPU, and the least pages that are worth a piece.
-constexpr int kWorkgroups = 256, kLeast = 4;
-// From so many rows of a key-value head on a workgroup of prompts.
-constexpr int kPromptRows = 64;
+// The least pages that are worth a piece: one a wave.
+constexpr int kLeast = 4;
+// From so many rows a wave joins a row's pieces: they fill the GPU.
+constexpr int kJoinRows = 512;
+constexpr int kPromptRows = 256;
 
-// Up to so many pieces one wave joins a row's.
-constexpr int kJoinAlone = 12;
+// Sixteen rows a workgroup, or 256. The first takes W (17 + p) of its turns, W workgroups of p pages on average (17 pages
+// are what a workgroup costs besides); the second half as many of theirs and 14 us more to begin and end with, but only
+// where several workgroups read the same pages, so from 1024 rows of a key-value head. Measured, in us, sixteen rows
+// against 256, 32 heads on 8 of dimension 128, bf16: 1024 tokens 32 and 45, 2048 tokens 81 and 66, 512 tokens over 4096
+// positions 60 and 52, 8 prompts of 512 tokens 95 and 62, 8 times 64 tokens over 4096 positions 67 and 114. Dimensions
+// up to 64 (16 heads, 4096 tokens 86 and 89, 512 over 32768 152 and 95) and f32 (512 over 8192 173 and 165, 8 of 512 tokens
+// 164 and 104) gain later; f32 of more than 128 dimensions has no second kind.
+constexpr int kPromptLeast = 1024;
+constexpr int64_t kPromptTurns = 53 << 10, kPromptTurnsF32 = 140 << 10, kPromptTurns64 = 220 << 10;
 
 struct Shape {
     bool prompt;
     int tile_rows, tiles, pieces, least;
     uint64_t slots, part_bytes, stat_bytes, bytes;
 };
-template <typename T>
-int prompt_rows(int pitch) {
-    return pitch <= 64 ? Prompt<1, T>::kRows : pitch <= 128 ? Prompt<2, T>::kRows : pitch <= 192 ? Prompt<3, T>::kRows : Prompt<4, T>::kRows;
-}
-Shape shape_of(const Kv4Sequences &q, int heads, int kv_heads, int dim, bool bf16) {
+Shape shape_of(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16) {
     Shape s;
     const int64_t rows = (int64_t)q.longest * (heads / kv_heads);
     const int pitch = kv4_pitch(dim);
-    s.prompt = rows >= kPromptRows;
-    s.tile_rows = !s.prompt ? 16 : bf16 ? prompt_rows<uint16_t>(pitch) : prompt_rows<float>(pitch);
+    const int64_t pages = window > 0 ? std::min<int64_t>(q.table_pages, ((int64_t)window + q.longest) / 64 + 2) : q.table_pages;
+    const int64_t reached = std::max<int64_t>(pages - q.longest / 128, 1);  // a row's on average, of the longest sequence's
+    const int64_t turns = (int64_t)q.count * kv_heads * ((rows + 15) / 16) * (17 + reached);
+    s.prompt = (bf16 || pitch <= 128) && rows >= kPromptLeast &&
+               turns >= (pitch == 64 ? kPromptTurns64 : bf16 ? kPromptTurns : kPromptTurnsF32);
+    s.tile_rows = s.prompt ? kPromptRows : 16;
     s.tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
     s.least = kLeast;
     const int64_t each = (int64_t)kv_heads * s.tiles, most = (int64_t)q.count * ((q.table_pages + s.least - 1) / s.least);
-    int64_t pieces = s.prompt ? 256 / (each * q.count) : (kWorkgroups + each - 1) / each;
+    // Sixteen rows: a workgroup for each CU, or three for two CUs where registers leave room for three on each (32 sequences
+    // of dimension 128: 51 us with one for each, 42 with these). Prompts that leave CUs idle: what one round holds, two
+    // where most of the context is the prompt itself, whose first rows reach little of it (4096 tokens, 12 heads on 4 of
+    // dimension 192: 179 us whole, 128 in pieces).
+    const int64_t whole = each * q.count;
+    int64_t pieces = !s.prompt ? ((pitch > 128 || !bf16 ? 256 : 384) + each - 1) / each
+                     : whole >= 256 ? 1 : (64 * (int64_t)q.table_pages <= 2 * (int64_t)q.longest ? 512 : 256) / whole;
     if (pieces > most) pieces = most;
     s.pieces = pieces < 1 ? 1 : (int)pieces;
     s.slots = (uint64_t)(s.pieces > 1 ? s.pieces + q.count : q.count);
@@ -1051,18 +1073,19 @@ void launch(sm_ctx *ctx, Kv4Attention a, const Shape &s, const T *Q, const uint8
     float2 *stats = (float2 *)((char *)workspace + s.part_bytes);
     a.info = s.pieces > 1 ? (int2 *)((char *)workspace + s.part_bytes + s.stat_bytes) : nullptr;
     const dim3 grid((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots);
-    if (s.prompt) k_kv4_prompt<NC, T><<<grid, Prompt<NC, T>::kThreads, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
-    else k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
+    if constexpr (Prompt<NC, T>::kThere)
+        if (s.prompt) k_kv4_prompt<NC, T><<<grid, Prompt<NC, T>::kThreads, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
+    if (!s.prompt) k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
     if (s.pieces == 1) return;
     const uint32_t all = (uint32_t)a.q.longest * a.heads;
-    if (s.pieces > kJoinAlone)
+    if ((int64_t)all * a.q.count < kJoinRows)
         k_kv4_join<NC, T, 16><<<dim3(all, a.q.count), 1024, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
     else
         k_kv4_join<NC, T, 1><<<dim3((all + 3) / 4, a.q.count), 256, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
 }
 template <typename T>
 void launch(sm_ctx *ctx, const Kv4Attention &a, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
-    const Shape s = shape_of(a.q, a.heads, a.kv_heads, a.dim, sizeof(T) == 2);
+    const Shape s = shape_of(a.q, a.heads, a.kv_heads, a.dim, a.window, sizeof(T) == 2);
     switch (kv4_pitch(a.dim) / 64) {
         case 1: return launch<1, T>(ctx, a, s, Q, pool, G, Y, workspace);
         case 2: return launch<2, T>(ctx, a, s, Q, pool, G, Y, workspace);
@@ -1075,10 +1098,12 @@ void launch(sm_ctx *ctx, const Kv4Attention &a, const T *Q, const uint8_t *pool,
 
 namespace smi {
 
-// Enough for either type.
 uint64_t kv4_attention_workspace(const Kv4Sequences &q, int heads, int kv_heads, int dim) {
-    const uint64_t f = shape_of(q, heads, kv_heads, dim, false).bytes, b = shape_of(q, heads, kv_heads, dim, true).bytes;
-    return f > b ? f : b;
+    // enough for either type, with a window and without one
+    uint64_t most = 0;
+    for (int bf16 = 0; bf16 < 2; bf16++)
+        for (int window = 0; window < 2; window++) most = std::max(most, shape_of(q, heads, kv_heads, dim, window, bf16).bytes);
+    return most;
 }
 
 int kv4_attention_launch(sm_ctx *ctx, const Kv4Attention &a, const void *Q, const uint8_t *pool, const void *G, void *Y, bool bf16,
