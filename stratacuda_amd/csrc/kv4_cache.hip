@@ -7,193 +7,180 @@
 namespace {
 using namespace smi;
 
-// ------------------------------------------------------------------- write
-// One workgroup a page and head. Keys: eight neighbouring dimensions a thread,
-// so that four threads hold a block of 32 and a position's codes are stored in
-// one piece. Values: a wave takes a block of 32 dimensions of all 64
-// positions, a thread two dimensions (one byte of codes) of 16 of them, whose
-// bytes lie together: 16 bytes a store where all are written.
+// Write and read: a workgroup takes 64 dimensions of a page and head, of its
+// keys or of its values; a thread eight neighbouring dimensions of a position,
+// four threads a block of 32. Keys' codes lie in memory as the threads have
+// them; values' (whose bytes are two dimensions of a position, 16 positions
+// together) pass through LDS on their way, so that both sides are read and
+// written in pieces of 16 bytes.
+struct Share {
+    int head, part, page;  // `part`: which 64 dimensions; page -1: none
+    int lo, hi;            // the page's positions that have rows; none: lo = hi
+    int64_t row;           // position 0's
+};
+__device__ __forceinline__ Share share_of(const Kv4Sequences &q, int run, int heads, int pages) {
+    const int s = blockIdx.y, h = blockIdx.x / run, parts = gridDim.z / 2;
+    const kv4::Span a = kv4::span(q, s);
+    const int first = a.length - a.n, at = (first >> 6) + (int)(blockIdx.x % run);  // first may lie before 0
+    if (a.n == 0 || at * 64 >= a.length) return {h, 0, -1, 0, 0, 0};
+    return {h, (int)blockIdx.z % parts, kv4::page_of(q, s, at, pages), max(first - at * 64, 0), min(a.length - at * 64, 64),
+            (int64_t)a.row + at * 64 - first};
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) k_kv4_write(const T *K, Kv4View kv, const T *V, Kv4View vv, Kv4Sequences q, int run,
-                                                   int dim, int pitch, uint8_t *pool, int pages, int heads, bool vec) {
-    const int s = blockIdx.y, h = blockIdx.x / run, tid = threadIdx.x;
-    const kv4::Span a = kv4::span(q, s);
-    if (a.n == 0) return;
-    const int first = a.length - a.n, at = (first >> 6) + (int)(blockIdx.x % run);  // first may lie before 0
-    if (at * 64 >= a.length) return;
-    const int page = kv4::page_of(q, s, at, pages);
-    if (page < 0) return;
-    // positions lo .. hi - 1 of the page are written; position p is row `base` + p
-    const int lo = max(first - at * 64, 0), hi = min(a.length - at * 64, 64);
-    const int64_t base = (int64_t)a.row + at * 64 - first;
-    uint8_t *tile = pool + ((int64_t)page * heads + h) * (68 * pitch);
-    const int nb = pitch / 32, wide = pitch / 8;
-    for (int e = tid + lo * wide; e < hi * wide; e += 256) {
-        const int p = e / wide, d = e % wide * 8;
-        float v[8] = {};
-        if (d < dim) kv4::load8(K + (base + p) * kv.stride + h * kv.head + kv.offset + d, vec, v);
+                                                   int dim, int pitch, uint8_t *pool, int pages, int heads, bool k_vec, bool v_vec) {
+    __shared__ __attribute__((aligned(16))) uint8_t s_codes[2048], s_scales[128];
+    const Share a = share_of(q, run, heads, pages);
+    if (a.page < 0) return;
+    const bool values = blockIdx.z >= gridDim.z / 2;
+    const int tid = threadIdx.x, d = 64 * a.part + tid % 8 * 8, b = tid / 4 % 2, sub = tid % 4;
+    uint8_t *tile = pool + ((int64_t)a.page * heads + a.head) * (68 * pitch);
+    const T *x = values ? V : K;
+    const Kv4View view = values ? vv : kv;
+    float v[2][8] = {};
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int p = tid / 8 + 32 * j;
+        if (p >= a.lo && p < a.hi && d < dim)
+            kv4::load8(x + (a.row + p) * view.stride + a.head * view.head + view.offset + d, values ? v_vec : k_vec, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int p = tid / 8 + 32 * j;
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) m = max(m, kv4::magnitude_bits(v[i]));
+        for (int i = 0; i < 8; i++) m = max(m, kv4::magnitude_bits(v[j][i]));
         m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, f8::kSwap1, 0xf, 0xf, true));
         m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, f8::kSwap2, 0xf, 0xf, true));
         const uint32_t byte = kv4::scale_byte(m);
         const float scale = kv4::code_scale(byte);
-        uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = kv4::code_value(v[i], byte);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], scale, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], scale, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], scale, 2);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], scale, 3);
-        *(uint32_t *)(tile + p * (pitch / 2) + d / 2) = w;
-        if (d % 32 == 0) tile[kv4::key_scales(pitch) + d / 32 * 64 + p % 16 * 4 + p / 16] = (uint8_t)byte;
-    }
-    const int lane = tid % 64, r = lane % 16, k = lane / 16;
-    for (int b = tid / 64; b < nb; b += 4) {
-        uint32_t w[4] = {}, scales[4] = {};
-#pragma unroll
-        for (int g = 0; g < 4; g++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int p = 16 * g + 4 * k + i, d = 32 * b + r;
-                float x = 0.0f, y = 0.0f;
-                if (p >= lo && p < hi) {
-                    const T *row = V + (base + p) * vv.stride + h * vv.head + vv.offset;
-                    if (d < dim) x = kv4::value(row[d]);
-                    if (d + 16 < dim) y = kv4::value(row[d + 16]);
-                }
-                uint32_t m = max(kv4::magnitude_bits(x), kv4::magnitude_bits(y));
-                m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, f8::kSwap1, 0xf, 0xf, true));
-                m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, f8::kSwap2, 0xf, 0xf, true));
-                m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, f8::kMirror8, 0xf, 0xf, true));
-                m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, f8::kMirror16, 0xf, 0xf, true));
-                const uint32_t byte = kv4::scale_byte(m);
-                const float scale = kv4::code_scale(byte);
-                x = kv4::code_value(x, byte), y = kv4::code_value(y, byte);
-                if (i == 0) w[g] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[g], x, y, scale, 0);
-                if (i == 1) w[g] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[g], x, y, scale, 1);
-                if (i == 2) w[g] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[g], x, y, scale, 2);
-                if (i == 3) w[g] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w[g], x, y, scale, 3);
-                scales[g] |= byte << (8 * i);
-            }
-        uint8_t *codes = tile + kv4::value_codes(pitch) + b * 1024 + lane * 16;
-        uint8_t *bytes = tile + kv4::value_scales(pitch) + b * 64 + k * 16;
-        if (lo == 0 && hi == 64) {
-            *(uint4 *)codes = make_uint4(w[0], w[1], w[2], w[3]);
-            if (r == 0) *(uint4 *)bytes = make_uint4(scales[0], scales[1], scales[2], scales[3]);
+        for (int i = 0; i < 8; i++) v[j][i] = kv4::code_value(v[j][i], byte);
+        uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0, v[j][0], v[j][1], scale, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][2], v[j][3], scale, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][4], v[j][5], scale, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[j][6], v[j][7], scale, 3);
+        if (!values) {
+            if (p < a.lo || p >= a.hi) continue;
+            *(uint32_t *)(tile + p * (pitch / 2) + d / 2) = w;
+            if (sub == 0) tile[kv4::key_scales(pitch) + d / 32 * 64 + p % 16 * 4 + p / 16] = (uint8_t)byte;
         } else {
+            // dimensions r and r + 16 in a byte: the thread two further has the other eight; four bytes each
+            const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, f8::kSwap2, 0xf, 0xf, true);
+            const uint32_t low = sub < 2 ? w : other >> 16, high = sub < 2 ? other : w >> 16;
+            const int r = sub % 2 * 8 + sub / 2 * 4, place = 16 * ((b * 4 + p / 4 % 4) * 16 + r) + p / 16 * 4 + p % 4;
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int p = 16 * g + 4 * k + i;
-                    if (p < lo || p >= hi) continue;
-                    codes[4 * g + i] = (uint8_t)(w[g] >> (8 * i));
-                    if (r == 0) bytes[4 * g + i] = (uint8_t)(scales[g] >> (8 * i));
-                }
+            for (int i = 0; i < 4; i++) s_codes[place + 16 * i] = (uint8_t)((low >> (4 * i) & 15u) | (high >> (4 * i) & 15u) << 4);
+            if (sub == 0) s_scales[b * 64 + p / 4 % 4 * 16 + p / 16 * 4 + p % 4] = (uint8_t)byte;
         }
     }
+    if (!values) return;
+    __syncthreads();
+    // 16 bytes each: block, quarter k and (codes) dimension; byte 4 g + i is position 16 g + 4 k + i
+    if (tid >= 136) return;
+    const bool codes = tid < 128;
+    const int u = codes ? tid : tid - 128, k = codes ? u / 16 % 4 : u % 4;
+    const uint4 w4 = codes ? ((const uint4 *)s_codes)[u] : ((const uint4 *)s_scales)[u];
+    uint8_t *to = codes ? tile + kv4::value_codes(pitch) + 2048 * a.part + 16 * u : tile + kv4::value_scales(pitch) + 128 * a.part + 16 * u;
+    if (a.lo == 0 && a.hi == 64) {
+        *(uint4 *)to = w4;
+        return;
+    }
+    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+    for (int g = 0; g < 4; g++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (16 * g + 4 * k + i >= a.lo && 16 * g + 4 * k + i < a.hi) to[4 * g + i] = (uint8_t)(w[g] >> (8 * i));
 }
 
-// -------------------------------------------------------------------- read
-// The same shares. What a code stands for is exact in bf16.
-__device__ __forceinline__ void values_of(uint32_t w, float scale, float v[8]) {
-    const kv4::f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1),
-                     c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
-    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
-}
-
+// What a code stands for is exact in bf16.
 template <typename T>
 __global__ void __launch_bounds__(256) k_kv4_read(const uint8_t *pool, int pages, int heads, int dim, int pitch, Kv4Sequences q,
-                                                  int run, T *K, Kv4View kv, T *V, Kv4View vv, bool vec) {
-    const int s = blockIdx.y, h = blockIdx.x / run, tid = threadIdx.x;
-    const kv4::Span a = kv4::span(q, s);
-    if (a.n == 0) return;
-    const int first = a.length - a.n, at = (first >> 6) + (int)(blockIdx.x % run);
-    if (at * 64 >= a.length) return;
-    const int page = kv4::page_of(q, s, at, pages);
-    // positions lo .. hi - 1 of the page have rows; those of no page are zeros
-    const int lo = max(first - at * 64, 0), hi = min(a.length - at * 64, 64);
-    const int64_t base = (int64_t)a.row + at * 64 - first;
-    const uint8_t *tile = pool + ((int64_t)max(page, 0) * heads + h) * (68 * pitch);
-    const int nb = pitch / 32, wide = pitch / 8;
-    for (int e = tid + lo * wide; e < hi * wide; e += 256) {
-        const int p = e / wide, d = e % wide * 8;
-        if (d >= dim) continue;
-        float v[8] = {};
-        if (page >= 0) {
-            const uint32_t byte = tile[kv4::key_scales(pitch) + d / 32 * 64 + p % 16 * 4 + p / 16];
-            values_of(*(const uint32_t *)(tile + p * (pitch / 2) + d / 2), kv4::scale_value(byte), v);
-        }
-        kv4::store8(K + (base + p) * kv.stride + h * kv.head + kv.offset + d, vec, v);
+                                                  int run, T *K, Kv4View kv, T *V, Kv4View vv, bool k_vec, bool v_vec) {
+    __shared__ __attribute__((aligned(8))) uint8_t s_codes[64][40];  // of a position: bytes 16 b + r; rows of 8 more for the banks
+    const Share a = share_of(q, run, heads, pages);
+    if (a.lo == a.hi) return;
+    const bool values = blockIdx.z >= gridDim.z / 2;
+    const int tid = threadIdx.x, d = 64 * a.part + tid % 8 * 8, b = tid / 4 % 2, sub = tid % 4;
+    // positions of no page are zeros
+    const uint8_t *tile = pool + ((int64_t)max(a.page, 0) * heads + a.head) * (68 * pitch);
+    uint32_t bytes[2], w[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int p = tid / 8 + 32 * j;
+        bytes[j] = values ? tile[kv4::value_scales(pitch) + d / 32 * 64 + p / 4 % 4 * 16 + p / 16 * 4 + p % 4]
+                          : tile[kv4::key_scales(pitch) + d / 32 * 64 + p % 16 * 4 + p / 16];
+        if (!values) w[j] = *(const uint32_t *)(tile + p * (pitch / 2) + d / 2);
     }
-    const int lane = tid % 64, r = lane % 16, k = lane / 16;
-    for (int b = tid / 64; b < nb; b += 4) {
-        const uint4 w4 = *(const uint4 *)(tile + kv4::value_codes(pitch) + b * 1024 + lane * 16);
-        const uint4 s4 = *(const uint4 *)(tile + kv4::value_scales(pitch) + b * 64 + k * 16);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w}, scales[4] = {s4.x, s4.y, s4.z, s4.w};
+    if (values) {
+        // half of 16 bytes each: block, quarter k, dimension; byte 4 g + i is position 16 g + 4 k + i
+        const int u = tid / 2, k = u / 16 % 4, g0 = tid % 2 * 2;
+        const uint2 two = *(const uint2 *)(tile + kv4::value_codes(pitch) + 2048 * a.part + 8 * tid);
 #pragma unroll
-        for (int g = 0; g < 4; g++)
+        for (int g = 0; g < 2; g++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int p = 16 * g + 4 * k + i, d = 32 * b + r;
-                if (p < lo || p >= hi) continue;
-                kv4::f32x2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[g] >> (8 * i),
-                                                                        kv4::scale_value(scales[g] >> (8 * i) & 255u), 0);
-                if (page < 0) v[0] = v[1] = 0.0f;
-                T *row = V + (base + p) * vv.stride + h * vv.head + vv.offset;
-                if (d < dim) kv4::store1(row + d, v[0]);
-                if (d + 16 < dim) kv4::store1(row + d + 16, v[1]);
+            for (int i = 0; i < 4; i++)
+                s_codes[16 * (g0 + g) + 4 * k + i][u / 64 * 16 + u % 16] = (uint8_t)((g == 0 ? two.x : two.y) >> (8 * i));
+        __syncthreads();
+    }
+    const Kv4View view = values ? vv : kv;
+    T *x = values ? V : K;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const int p = tid / 8 + 32 * j;
+        if (p < a.lo || p >= a.hi || d >= dim) continue;
+        const float scale = kv4::scale_value(bytes[j]);
+        float v[8];
+        if (values) {
+            const uint2 eight = *(const uint2 *)&s_codes[p][16 * b + 8 * (sub % 2)];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const kv4::f32x2 f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((i < 4 ? eight.x : eight.y) >> (8 * (i % 4)), scale, 0);
+                v[i] = sub < 2 ? f[0] : f[1];
             }
+        } else {
+            const kv4::f32x2 f0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], scale, 0), f1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], scale, 1),
+                             f2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], scale, 2), f3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[j], scale, 3);
+            v[0] = f0[0], v[1] = f0[1], v[2] = f1[0], v[3] = f1[1], v[4] = f2[0], v[5] = f2[1], v[6] = f3[0], v[7] = f3[1];
+        }
+        if (a.page < 0)
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = 0.0f;
+        kv4::store8(x + (a.row + p) * view.stride + a.head * view.head + view.offset + d, values ? v_vec : k_vec, v);
     }
 }
 
 // ----------------------------------------------------------- norm and rotate
-// `lanes` lanes (a power of two, 32 at most) a head, eight dimensions each.
+// kLanes lanes (a power of two, 32 at most) a head, eight dimensions each.
 // The dimension that another is turned with lies half the rotated ones away:
-// its value is read again (from the caches) rather than exchanged. The squares
-// are summed in f64 and the power of two of 1 / sqrt(mean) is applied apart: a
-// row of large values does not overflow, one of subnormal ones does not pass
-// f32's range.
-template <typename T>
-__global__ void __launch_bounds__(256) k_qk_norm_rope(QkNormRope a, const T *Q, const T *K, T *Yq, T *Yk, int lanes, int items,
-                                                      bool vec) {
-    const int item = (int)((blockIdx.x * 256u + threadIdx.x) / (unsigned)lanes), lane = threadIdx.x % lanes, d = 8 * lane;
+// its value is read again (from the caches) rather than exchanged, and every
+// load is under way before the sum. The squares are summed in f64 and the
+// power of two of 1 / sqrt(mean) is applied apart: a row of large values does
+// not overflow, one of subnormal ones does not pass f32's range.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256) k_qk_norm_rope(QkNormRope a, const T *Q, const T *K, T *Yq, T *Yk, uint32_t items, bool vec) {
+    const uint32_t item = (blockIdx.x * 256u + threadIdx.x) / kLanes, all = a.heads + a.kv_heads, mine = min(item, items - 1);
+    const int lane = threadIdx.x % kLanes, d = 8 * lane;
     const bool there = item < items && d < a.dim;
-    const int all = a.heads + a.kv_heads, t = min(item, items - 1) / all, head = min(item, items - 1) % all;
-    const bool is_q = head < a.heads;
-    const int h = is_q ? head : head - a.heads;
+    const uint32_t t = mine / all, head = mine % all;
+    const bool is_q = head < (uint32_t)a.heads;
+    const uint32_t h = is_q ? head : head - a.heads;
     const Kv4View view = is_q ? a.q_view : a.k_view;
     const T *x = (is_q ? Q : K) + t * view.stride + h * view.head + view.offset;
     const float *gamma = is_q ? a.q_gamma : a.k_gamma;
     const int half = a.rotary / 2, position = a.positions[t];
-    float v[8] = {}, g[8] = {};
+    const bool turns = there && d < a.rotary, sides = half % 8 == 0;  // sides: all eight lie in one half
+    float v[8] = {}, g[8] = {}, o[8] = {}, og[8] = {}, c[8], s[8];
     if (there) {
         kv4::load8(x + d, vec, v);
         kv4::load8(gamma + d, true, g);
     }
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) sum += (double)v[i] * (double)v[i];
-    if (lanes > 1) sum += f8::moved<f8::kSwap1>(sum);
-    if (lanes > 2) sum += f8::moved<f8::kSwap2>(sum);
-    if (lanes > 4) sum += f8::moved<f8::kMirror8>(sum);
-    if (lanes > 8) sum += f8::moved<f8::kMirror16>(sum);
-    if (lanes > 16) sum += __shfl_xor(sum, 16, 64);
-    if (!there) return;
-    const double root = 1.0 / sqrt(sum / (double)a.dim + (double)a.eps);
-    const float inv = (float)__builtin_amdgcn_frexp_mant(root);
-    const int inv_exp = __builtin_amdgcn_frexp_exp(root);
-    const auto normed = [&](float value, float weight) { return __builtin_amdgcn_ldexpf(value, inv_exp) * inv * weight; };
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = normed(v[i], g[i]);
-    if (d < a.rotary) {
-        const bool inside = position >= 0 && position < a.context;
+    const bool inside = position >= 0 && position < a.context;
+    if (turns) {
         const int64_t angle = (int64_t)(inside ? position : 0) * half;
-        float o[8], og[8], c[8], s[8];
-        if (half % 8 == 0) {  // all eight on one side
+        if (sides) {
             const int other = d < half ? d + half : d - half, pair = d < half ? d : d - half;
             kv4::load8(x + other, vec, o);
             kv4::load8(gamma + other, true, og);
@@ -208,11 +195,31 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkNormRope a, const T *Q, 
                 c[i] = turned ? a.cos[angle + pair] : 1.0f, s[i] = turned ? a.sin[angle + pair] : 0.0f;
             }
         }
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum = fma((double)v[i], (double)v[i], sum);
+    if (kLanes > 1) sum += f8::moved<f8::kSwap1>(sum);
+    if (kLanes > 2) sum += f8::moved<f8::kSwap2>(sum);
+    if (kLanes > 4) sum += f8::moved<f8::kMirror8>(sum);
+    if (kLanes > 8) sum += f8::moved<f8::kMirror16>(sum);
+    if (kLanes > 16) sum += __shfl_xor(sum, 16, 64);
+    if (!there) return;
+    // 1 / sqrt: the unit's (2^-26 or better), one step of Newton's beyond what f32 shows
+    const double mean = sum / a.dim + (double)a.eps, guess = __builtin_amdgcn_rsq(mean);
+    const double root = mean > 0.0 && mean < INFINITY ? guess * (1.5 - 0.5 * mean * guess * guess) : guess;
+    const float inv = (float)__builtin_amdgcn_frexp_mant(root);
+    const int inv_exp = __builtin_amdgcn_frexp_exp(root);
+    const auto normed = [&](float value, float weight) { return __builtin_amdgcn_ldexpf(value, inv_exp) * inv * weight; };
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = normed(v[i], g[i]);
+    if (turns) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            if (d + i >= a.rotary) continue;
-            const float b = normed(o[i], og[i]);
-            y[i] = inside ? (d + i < half ? y[i] * c[i] - b * s[i] : y[i] * c[i] + b * s[i]) : NAN;
+            if (!sides && d + i >= a.rotary) continue;
+            const float b = normed(o[i], og[i]), turned = d + i < half ? -b : b;
+            y[i] = inside ? y[i] * c[i] + turned * s[i] : NAN;
         }
     }
     T *to = is_q ? Yq + ((int64_t)t * a.heads + h) * a.dim : Yk + ((int64_t)t * a.kv_heads + h) * a.dim;
@@ -221,50 +228,57 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkNormRope a, const T *Q, 
 
 int run_of(int longest) { return (longest + 62) / 64 + 1; }  // pages that as many positions can touch
 
+template <typename T>
+void norm_rope(sm_ctx *ctx, const QkNormRope &a, const T *Q, const T *K, T *Yq, T *Yk) {
+    int lanes = 1;
+    while (8 * lanes < a.dim) lanes *= 2;
+    const uint32_t items = (uint32_t)a.tokens * (a.heads + a.kv_heads);
+    const bool vec = a.q_view.multiple_of(8) && a.k_view.multiple_of(8);
+    const uint32_t grid = (uint32_t)(((uint64_t)items * lanes + 255) / 256);
+    switch (lanes) {
+        case 1: k_qk_norm_rope<T, 1><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
+        case 2: k_qk_norm_rope<T, 2><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
+        case 4: k_qk_norm_rope<T, 4><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
+        case 8: k_qk_norm_rope<T, 8><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
+        case 16: k_qk_norm_rope<T, 16><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
+        default: k_qk_norm_rope<T, 32><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
+    }
+}
+
 }  // namespace
 
 namespace smi {
 
 int kv4_write_launch(sm_ctx *ctx, const void *K, const Kv4View &kv, const void *V, const Kv4View &vv, bool bf16,
                      const Kv4Sequences &q, int heads, int dim, uint8_t *pool, int pages) {
-    const int run = run_of(q.longest);
-    const bool vec = kv.multiple_of(8);
-    const dim3 grid((uint32_t)(run * heads), q.count);
+    const int run = run_of(q.longest), pitch = kv4_pitch(dim);
+    const bool k_vec = kv.multiple_of(8), v_vec = vv.multiple_of(8);
+    const dim3 grid((uint32_t)(run * heads), q.count, 2 * (pitch / 64));
     if (bf16)
-        k_kv4_write<<<grid, 256, 0, ctx->stream>>>((const uint16_t *)K, kv, (const uint16_t *)V, vv, q, run, dim,
-                                                   kv4_pitch(dim), pool, pages, heads, vec);
+        k_kv4_write<<<grid, 256, 0, ctx->stream>>>((const uint16_t *)K, kv, (const uint16_t *)V, vv, q, run, dim, pitch, pool, pages,
+                                                   heads, k_vec, v_vec);
     else
-        k_kv4_write<<<grid, 256, 0, ctx->stream>>>((const float *)K, kv, (const float *)V, vv, q, run, dim, kv4_pitch(dim), pool,
-                                                   pages, heads, vec);
+        k_kv4_write<<<grid, 256, 0, ctx->stream>>>((const float *)K, kv, (const float *)V, vv, q, run, dim, pitch, pool, pages, heads,
+                                                   k_vec, v_vec);
     return launched(ctx);
 }
 
 int kv4_read_launch(sm_ctx *ctx, const uint8_t *pool, int pages, int heads, int dim, const Kv4Sequences &q, void *K,
                     const Kv4View &kv, void *V, const Kv4View &vv, bool bf16) {
-    const int run = run_of(q.longest);
-    const bool vec = kv.multiple_of(8);
-    const dim3 grid((uint32_t)(run * heads), q.count);
+    const int run = run_of(q.longest), pitch = kv4_pitch(dim);
+    const bool k_vec = kv.multiple_of(8), v_vec = vv.multiple_of(8);
+    const dim3 grid((uint32_t)(run * heads), q.count, 2 * (pitch / 64));
     if (bf16)
-        k_kv4_read<<<grid, 256, 0, ctx->stream>>>(pool, pages, heads, dim, kv4_pitch(dim), q, run, (uint16_t *)K, kv,
-                                                  (uint16_t *)V, vv, vec);
+        k_kv4_read<<<grid, 256, 0, ctx->stream>>>(pool, pages, heads, dim, pitch, q, run, (uint16_t *)K, kv, (uint16_t *)V, vv, k_vec,
+                                                  v_vec);
     else
-        k_kv4_read<<<grid, 256, 0, ctx->stream>>>(pool, pages, heads, dim, kv4_pitch(dim), q, run, (float *)K, kv, (float *)V, vv,
-                                                  vec);
+        k_kv4_read<<<grid, 256, 0, ctx->stream>>>(pool, pages, heads, dim, pitch, q, run, (float *)K, kv, (float *)V, vv, k_vec, v_vec);
     return launched(ctx);
 }
 
 int qk_norm_rope_launch(sm_ctx *ctx, const QkNormRope &a, const void *Q, const void *K, void *Yq, void *Yk, bool bf16) {
-    int lanes = 1;
-    while (8 * lanes < a.dim) lanes *= 2;
-    const int items = a.tokens * (a.heads + a.kv_heads);
-    const bool vec = a.q_view.multiple_of(8) && a.k_view.multiple_of(8);
-    const uint32_t grid = (uint32_t)(((int64_t)items * lanes + 255) / 256);
-    if (bf16)
-        k_qk_norm_rope<<<grid, 256, 0, ctx->stream>>>(a, (const uint16_t *)Q, (const uint16_t *)K, (uint16_t *)Yq, (uint16_t *)Yk,
-                                                      lanes, items, vec);
-    else
-        k_qk_norm_rope<<<grid, 256, 0, ctx->stream>>>(a, (const float *)Q, (const float *)K, (float *)Yq, (float *)Yk, lanes,
-                                                      items, vec);
+    if (bf16) norm_rope(ctx, a, (const uint16_t *)Q, (const uint16_t *)K, (uint16_t *)Yq, (uint16_t *)Yk);
+    else norm_rope(ctx, a, (const float *)Q, (const float *)K, (float *)Yq, (float *)Yk);
     return launched(ctx);
 }
 
