@@ -153,96 +153,109 @@ __global__ void __launch_bounds__(256) k_kv4_read(const uint8_t *pool, int pages
 }
 
 // ----------------------------------------------------------- norm and rotate
-// kLanes lanes (a power of two, 32 at most) a head, eight dimensions each.
-// The dimension that another is turned with lies half the rotated ones away:
-// its value is read again (from the caches) rather than exchanged, and every
-// load is under way before the sum. The squares are summed in f64 and the
+// kLanes lanes (a power of two, 16 at most) a head, twice eight dimensions
+// each. The dimension that another is turned with lies half the rotated ones
+// away: its value is read again (from the caches) rather than exchanged, and
+// every load is under way before the sum. The squares are summed in f64 and the
 // power of two of 1 / sqrt(mean) is applied apart: a row of large values does
-// not overflow, one of subnormal ones does not pass f32's range.
-template <typename T, int kLanes>
+// not overflow, one of subnormal ones does not pass f32's range. kSides: half
+// the rotated dimensions are a multiple of eight, so that all eight of a lane
+// lie on one side.
+template <typename T, int kLanes, bool kSides>
 __global__ void __launch_bounds__(256) k_qk_norm_rope(QkNormRope a, const T *Q, const T *K, T *Yq, T *Yk, uint32_t items, bool vec) {
-    const uint32_t item = (blockIdx.x * 256u + threadIdx.x) / kLanes, all = a.heads + a.kv_heads, mine = min(item, items - 1);
-    const int lane = threadIdx.x % kLanes, d = 8 * lane;
-    const bool there = item < items && d < a.dim;
-    const uint32_t t = mine / all, head = mine % all;
+    const uint32_t all = a.heads + a.kv_heads, first = blockIdx.x * (256 / kLanes), t0 = first / all, own = threadIdx.x / kLanes;
+    const int lane = threadIdx.x % kLanes;
+    const uint32_t place = first - t0 * all + min(own, items - 1 - first);
+    const uint32_t more = (uint32_t)(((float)place + 0.5f) / (float)all);  // place < 2^11 + 256: half a step off any border
+    const uint32_t t = t0 + more, head = place - more * all;
     const bool is_q = head < (uint32_t)a.heads;
     const uint32_t h = is_q ? head : head - a.heads;
     const Kv4View view = is_q ? a.q_view : a.k_view;
     const T *x = (is_q ? Q : K) + t * view.stride + h * view.head + view.offset;
     const float *gamma = is_q ? a.q_gamma : a.k_gamma;
     const int half = a.rotary / 2, position = a.positions[t];
-    const bool turns = there && d < a.rotary, sides = half % 8 == 0;  // sides: all eight lie in one half
-    float v[8] = {}, g[8] = {}, o[8] = {}, og[8] = {}, c[8], s[8];
-    if (there) {
-        kv4::load8(x + d, vec, v);
-        kv4::load8(gamma + d, true, g);
-    }
     const bool inside = position >= 0 && position < a.context;
-    if (turns) {
-        const int64_t angle = (int64_t)(inside ? position : 0) * half;
-        if (sides) {
+    const int64_t angle = (int64_t)(inside ? position : 0) * half;
+    float v[2][8], g[2][8], o[2][8], og[2][8], c[2][8], s[2][8];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int d = 8 * (lane + e * kLanes);
+        if (d < a.dim) {
+            kv4::load8(x + d, vec, v[e]);
+            kv4::load8(gamma + d, true, g[e]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[e][i] = 0.0f;
+        }
+        if (d >= a.rotary) continue;
+        if (kSides) {
             const int other = d < half ? d + half : d - half, pair = d < half ? d : d - half;
-            kv4::load8(x + other, vec, o);
-            kv4::load8(gamma + other, true, og);
-            kv4::load8(a.cos + angle + pair, true, c);
-            kv4::load8(a.sin + angle + pair, true, s);
+            kv4::load8(x + other, vec, o[e]);
+            kv4::load8(gamma + other, true, og[e]);
+            kv4::load8(a.cos + angle + pair, true, c[e]);
+            kv4::load8(a.sin + angle + pair, true, s[e]);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const bool turned = d + i < a.rotary;
-                const int other = d + i < half ? d + i + half : d + i - half, pair = d + i < half ? d + i : d + i - half;
-                o[i] = turned ? kv4::value(x[other]) : 0.0f, og[i] = turned ? gamma[other] : 0.0f;
-                c[i] = turned ? a.cos[angle + pair] : 1.0f, s[i] = turned ? a.sin[angle + pair] : 0.0f;
+                const int at = min(d + i, a.rotary - 1);
+                const int other = at < half ? at + half : at - half, pair = at < half ? at : at - half;
+                o[e][i] = kv4::value(x[other]), og[e][i] = gamma[other];
+                c[e][i] = a.cos[angle + pair], s[e][i] = a.sin[angle + pair];
             }
         }
     }
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) sum = fma((double)v[i], (double)v[i], sum);
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum = fma((double)v[e][i], (double)v[e][i], sum);
     if (kLanes > 1) sum += f8::moved<f8::kSwap1>(sum);
     if (kLanes > 2) sum += f8::moved<f8::kSwap2>(sum);
     if (kLanes > 4) sum += f8::moved<f8::kMirror8>(sum);
     if (kLanes > 8) sum += f8::moved<f8::kMirror16>(sum);
-    if (kLanes > 16) sum += __shfl_xor(sum, 16, 64);
-    if (!there) return;
+    if (first + own >= items) return;
     // 1 / sqrt: the unit's (2^-26 or better), one step of Newton's beyond what f32 shows
-    const double mean = sum / a.dim + (double)a.eps, guess = __builtin_amdgcn_rsq(mean);
+    const double mean = sum * (1.0 / a.dim) + (double)a.eps, guess = __builtin_amdgcn_rsq(mean);
     const double root = mean > 0.0 && mean < INFINITY ? guess * (1.5 - 0.5 * mean * guess * guess) : guess;
     const float inv = (float)__builtin_amdgcn_frexp_mant(root);
     const int inv_exp = __builtin_amdgcn_frexp_exp(root);
     const auto normed = [&](float value, float weight) { return __builtin_amdgcn_ldexpf(value, inv_exp) * inv * weight; };
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = normed(v[i], g[i]);
-    if (turns) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (!sides && d + i >= a.rotary) continue;
-            const float b = normed(o[i], og[i]), turned = d + i < half ? -b : b;
-            y[i] = inside ? y[i] * c[i] + turned * s[i] : NAN;
-        }
-    }
     T *to = is_q ? Yq + ((int64_t)t * a.heads + h) * a.dim : Yk + ((int64_t)t * a.kv_heads + h) * a.dim;
-    kv4::store8(to + d, true, y);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int d = 8 * (lane + e * kLanes);
+        if (d >= a.dim) continue;
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = normed(v[e][i], g[e][i]);
+        if (d < a.rotary) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (!kSides && d + i >= a.rotary) continue;
+                const float b = normed(o[e][i], og[e][i]), turned = d + i < half ? -b : b;
+                y[i] = inside ? y[i] * c[e][i] + turned * s[e][i] : NAN;
+            }
+        }
+        kv4::store8(to + d, true, y);
+    }
 }
 
 int run_of(int longest) { return (longest + 62) / 64 + 1; }  // pages that as many positions can touch
 
+template <typename T, int kLanes>
+void norm_rope(sm_ctx *ctx, const QkNormRope &a, const T *Q, const T *K, T *Yq, T *Yk) {
+    const uint32_t items = (uint32_t)a.tokens * (a.heads + a.kv_heads), grid = (items + 256 / kLanes - 1) / (256 / kLanes);
+    const bool vec = a.q_view.multiple_of(8) && a.k_view.multiple_of(8);
+    if (a.rotary % 16 == 0) k_qk_norm_rope<T, kLanes, true><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec);
+    else k_qk_norm_rope<T, kLanes, false><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec);
+}
 template <typename T>
 void norm_rope(sm_ctx *ctx, const QkNormRope &a, const T *Q, const T *K, T *Yq, T *Yk) {
-    int lanes = 1;
-    while (8 * lanes < a.dim) lanes *= 2;
-    const uint32_t items = (uint32_t)a.tokens * (a.heads + a.kv_heads);
-    const bool vec = a.q_view.multiple_of(8) && a.k_view.multiple_of(8);
-    const uint32_t grid = (uint32_t)(((uint64_t)items * lanes + 255) / 256);
-    switch (lanes) {
-        case 1: k_qk_norm_rope<T, 1><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
-        case 2: k_qk_norm_rope<T, 2><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
-        case 4: k_qk_norm_rope<T, 4><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
-        case 8: k_qk_norm_rope<T, 8><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
-        case 16: k_qk_norm_rope<T, 16><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
-        default: k_qk_norm_rope<T, 32><<<grid, 256, 0, ctx->stream>>>(a, Q, K, Yq, Yk, items, vec); break;
-    }
+    if (a.dim <= 16) norm_rope<T, 1>(ctx, a, Q, K, Yq, Yk);
+    else if (a.dim <= 32) norm_rope<T, 2>(ctx, a, Q, K, Yq, Yk);
+    else if (a.dim <= 64) norm_rope<T, 4>(ctx, a, Q, K, Yq, Yk);
+    else if (a.dim <= 128) norm_rope<T, 8>(ctx, a, Q, K, Yq, Yk);
+    else norm_rope<T, 16>(ctx, a, Q, K, Yq, Yk);
 }
 
 }  // namespace
