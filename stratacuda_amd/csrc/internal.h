@@ -319,7 +319,6 @@ int kv4_write_launch(sm_ctx *ctx, const void *K, const Kv4View &kv, const void *
                      const Kv4Sequences &q, int heads, int dim, uint8_t *pool, int pages);
 int kv4_read_launch(sm_ctx *ctx, const uint8_t *pool, int pages, int heads, int dim, const Kv4Sequences &q, void *K,
                     const Kv4View &kv, void *V, const Kv4View &vv, bool bf16);
-uint64_t kv4_attention_workspace(const Kv4Sequences &q, int heads, int kv_heads, int dim);
 int kv4_attention_launch(sm_ctx *ctx, const Kv4Attention &a, const void *Q, const uint8_t *pool, const void *G, void *Y, bool bf16,
                          void *workspace);
 

@@ -2,7 +2,7 @@
 // are checked here, before anything runs.
 #include <initializer_list>
 
-#include "internal.h"
+#include "kv4_shapes.h"
 
 using namespace smi;
 
@@ -181,7 +181,7 @@ int sm_kv4_attention_workspace(int tokens, int count, int longest, int table_pag
     if (int rc = check_heads(nullptr, what, heads, kv_heads, dim)) return rc;
     if (int rc = check_rows(nullptr, what, tokens, heads)) return rc;
     if (int rc = check_sequences(nullptr, what, tokens, count, longest, table_pages)) return rc;
-    *bytes = kv4_attention_workspace({count, tokens, longest, table_pages, nullptr, nullptr, nullptr}, heads, kv_heads, dim);
+    *bytes = kv4_workspace({count, tokens, longest, table_pages, nullptr, nullptr, nullptr}, heads, kv_heads, dim);
     return SM_OK;
 }
 
@@ -210,7 +210,7 @@ int sm_kv4_attention(sm_ctx *ctx, uint64_t Q, const int64_t *q_view, int type, i
     if (int rc = need_sequences(ctx, count, table_pages, starts, lengths, table)) return rc;
     if (int rc = need(ctx, pool, pool_bytes, "kv4 attention pool")) return rc;
     if (int rc = need(ctx, Y, (uint64_t)tokens * heads * dim * (type == SM_TYPE_BF16 ? 2 : 4), "kv4 attention Y")) return rc;
-    const uint64_t ws = kv4_attention_workspace(a.q, heads, kv_heads, dim);
+    const uint64_t ws = kv4_workspace(a.q, heads, kv_heads, dim);
     if (ws) {
         if (workspace_bytes < ws) return fail(ctx, SM_E_ARG, "workspace too small");
         if (int rc = need(ctx, workspace, ws, "workspace")) return rc;

@@ -11,10 +11,10 @@
 // the sum of three bf16 numbers (8 significant bits each, so all 24) and cost
 // three matrix instructions. For bf16 the probabilities are rounded to bf16,
 // half a step of 2^-8 relative, like the result; sums are f32's.
-#include <algorithm>
 #include <type_traits>
 
 #include "kv4_device.h"
+#include "kv4_shapes.h"
 #include "strata_device.h"
 
 namespace {
@@ -486,6 +486,7 @@ struct Prompt {
     // f32 queries of more than 128 dimensions would take more registers than two waves of a SIMD have
     static constexpr bool kThere = !kF32 || NC < 3;
     static constexpr int kWaves = 8, kThreads = 64 * kWaves, kRows = 32 * kWaves;
+    static_assert(kRows == kKv4PromptRows, "the shapes count on it");
     static constexpr int kHalves = NC > 2 || (kF32 && NC > 1) ? 1 : 2;  // of a page in a unit: what registers hold
     static constexpr int kUnit = 32 * kHalves, kTurns = 64 / kUnit;
     static constexpr int kPieces = 2 * NC;  // of 16 bytes, of a key's codes
@@ -1015,59 +1016,8 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) k_kv4_join(Kv
     }
 }
 
-// The least pages that are worth a piece: one a wave.
-constexpr int kLeast = 4;
-// From so many rows a wave joins a row's pieces: they fill the GPU.
-constexpr int kJoinRows = 512;
-constexpr int kPromptRows = 256;
-
-// Sixteen rows a workgroup, or 256. The first takes W (17 + p) of its turns, W workgroups of p pages on average (17 pages
-// are what a workgroup costs besides); the second half as many of theirs and 14 us more to begin and end with, but only
-// where several workgroups read the same pages, so from 1024 rows of a key-value head. Measured, in us, sixteen rows
-// against 256, 32 heads on 8 of dimension 128, bf16: 1024 tokens 32 and 45, 2048 tokens 81 and 66, 512 tokens over 4096
-// positions 60 and 52, 8 prompts of 512 tokens 95 and 62, 8 times 64 tokens over 4096 positions 67 and 114. Dimensions
-// up to 64 (16 heads, 4096 tokens 86 and 89, 512 over 32768 152 and 95) and f32 (512 over 8192 173 and 165, 8 of 512 tokens
-// 164 and 104) gain later; f32 of more than 128 dimensions has no second kind.
-constexpr int kPromptLeast = 1024;
-constexpr int64_t kPromptTurns = 53 << 10, kPromptTurnsF32 = 140 << 10, kPromptTurns64 = 220 << 10;
-
-struct Shape {
-    bool prompt;
-    int tile_rows, tiles, pieces, least;
-    uint64_t slots, part_bytes, stat_bytes, bytes;
-};
-Shape shape_of(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16) {
-    Shape s;
-    const int64_t rows = (int64_t)q.longest * (heads / kv_heads);
-    const int pitch = kv4_pitch(dim);
-    const int64_t pages = window > 0 ? std::min<int64_t>(q.table_pages, ((int64_t)window + q.longest) / 64 + 2) : q.table_pages;
-    const int64_t reached = std::max<int64_t>(pages - q.longest / 128, 1);  // a row's on average, of the longest sequence's
-    const int64_t turns = (int64_t)q.count * kv_heads * ((rows + 15) / 16) * (17 + reached);
-    s.prompt = (bf16 || pitch <= 128) && rows >= kPromptLeast &&
-               turns >= (pitch == 64 ? kPromptTurns64 : bf16 ? kPromptTurns : kPromptTurnsF32);
-    s.tile_rows = s.prompt ? kPromptRows : 16;
-    s.tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
-    s.least = kLeast;
-    const int64_t each = (int64_t)kv_heads * s.tiles, most = (int64_t)q.count * ((q.table_pages + s.least - 1) / s.least);
-    // Sixteen rows: a workgroup for each CU, or three for two CUs where registers leave room for three on each (32 sequences
-    // of dimension 128: 51 us with one for each, 42 with these). Prompts that leave CUs idle: what one round holds, two
-    // where most of the context is the prompt itself, whose first rows reach little of it (4096 tokens, 12 heads on 4 of
-    // dimension 192: 179 us whole, 128 in pieces).
-    const int64_t whole = each * q.count;
-    int64_t pieces = !s.prompt ? ((pitch > 128 || !bf16 ? 256 : 384) + each - 1) / each
-                     : whole >= 256 ? 1 : (64 * (int64_t)q.table_pages <= 2 * (int64_t)q.longest ? 512 : 256) / whole;
-    if (pieces > most) pieces = most;
-    s.pieces = pieces < 1 ? 1 : (int)pieces;
-    s.slots = (uint64_t)(s.pieces > 1 ? s.pieces + q.count : q.count);
-    s.part_bytes = s.pieces > 1 ? s.slots * each * s.tile_rows * pitch * 4 : 0;
-    s.stat_bytes = s.pieces > 1 ? s.slots * each * s.tile_rows * 8 : 0;
-    s.bytes = s.part_bytes + s.stat_bytes + (s.pieces > 1 ? (uint64_t)q.count * 8 : 0);
-    if (s.pieces == 1) s.least = q.table_pages + 1;  // one piece a sequence: as large as any
-    return s;
-}
-
 template <int NC, typename T>
-void launch(sm_ctx *ctx, Kv4Attention a, const Shape &s, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
+void launch(sm_ctx *ctx, Kv4Attention a, const Kv4Shape &s, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
     a.pieces = s.pieces, a.least = s.least;
     float *parts = (float *)workspace;
     float2 *stats = (float2 *)((char *)workspace + s.part_bytes);
@@ -1078,14 +1028,14 @@ void launch(sm_ctx *ctx, Kv4Attention a, const Shape &s, const T *Q, const uint8
     if (!s.prompt) k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
     if (s.pieces == 1) return;
     const uint32_t all = (uint32_t)a.q.longest * a.heads;
-    if ((int64_t)all * a.q.count < kJoinRows)
+    if ((int64_t)all * a.q.count < kKv4JoinRows)
         k_kv4_join<NC, T, 16><<<dim3(all, a.q.count), 1024, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
     else
         k_kv4_join<NC, T, 1><<<dim3((all + 3) / 4, a.q.count), 256, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
 }
 template <typename T>
 void launch(sm_ctx *ctx, const Kv4Attention &a, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
-    const Shape s = shape_of(a.q, a.heads, a.kv_heads, a.dim, a.window, sizeof(T) == 2);
+    const Kv4Shape s = kv4_shape(a.q, a.heads, a.kv_heads, a.dim, a.window, sizeof(T) == 2);
     switch (kv4_pitch(a.dim) / 64) {
         case 1: return launch<1, T>(ctx, a, s, Q, pool, G, Y, workspace);
         case 2: return launch<2, T>(ctx, a, s, Q, pool, G, Y, workspace);
@@ -1097,14 +1047,6 @@ void launch(sm_ctx *ctx, const Kv4Attention &a, const T *Q, const uint8_t *pool,
 }  // namespace
 
 namespace smi {
-
-uint64_t kv4_attention_workspace(const Kv4Sequences &q, int heads, int kv_heads, int dim) {
-    // enough for either type, with a window and without one
-    uint64_t most = 0;
-    for (int bf16 = 0; bf16 < 2; bf16++)
-        for (int window = 0; window < 2; window++) most = std::max(most, shape_of(q, heads, kv_heads, dim, window, bf16).bytes);
-    return most;
-}
 
 int kv4_attention_launch(sm_ctx *ctx, const Kv4Attention &a, const void *Q, const uint8_t *pool, const void *G, void *Y, bool bf16,
                          void *workspace) {

@@ -28,7 +28,6 @@ int kv4_read_launch(sm_ctx *ctx, const uint8_t *, int, int, int, const Kv4Sequen
                     bool) {
     return launch(ctx);
 }
-uint64_t kv4_attention_workspace(const Kv4Sequences &q, int, int, int) { return q.table_pages > 1 ? 4096 : 0; }
 int kv4_attention_launch(sm_ctx *ctx, const Kv4Attention &, const void *, const uint8_t *, const void *, void *, bool, void *) {
     return launch(ctx);
 }

@@ -72,11 +72,14 @@ WRITE = Call("sm_kv4_write", "K kv V vv type tokens count longest starts lengths
 READ = Call("sm_kv4_read", "pool pages kv_heads dim tokens count longest starts lengths table table_pages K kv V vv type",
             dict(SEQ, K=0x100, kv=None, V=0x200, vv=view(300, 100, 7), type=0, kv_heads=2, dim=72, pool=0x300, pages=9),
             dict(SEQ_NEED, K=5 * 144 * 4, V=(4 * 300 + 100 + 7 + 72) * 4, pool=9 * 2 * TILE), ("K", "V"))
+# 6 pieces of 4 pages and one more a sequence, of 2 heads' 16 rows: 128 sums and two statistics; 2 words a sequence
+WORKSPACE = (6 + 3) * 2 * 16 * (128 + 2) * 4 + 3 * 8
 ATTENTION = Call("sm_kv4_attention", "Q qv type tokens count longest starts lengths table table_pages pool pages heads kv_heads dim scale "
                  "window G gv Y ws bytes",
                  dict(SEQ, Q=0x100, qv=None, type=0, pool=0x300, pages=9, heads=6, kv_heads=2, dim=72, scale=0.1, window=0, G=0x400,
-                      gv=view(2000, 200, 72), Y=0x500, ws=0x600, bytes=4096),
-                 dict(SEQ_NEED, Q=5 * 432 * 4, G=(4 * 2000 + 5 * 200 + 144) * 4, pool=9 * 2 * TILE, Y=5 * 432 * 4, ws=4096), ("Y", "ws"))
+                      gv=view(2000, 200, 72), Y=0x500, ws=0x600, bytes=WORKSPACE),
+                 dict(SEQ_NEED, Q=5 * 432 * 4, G=(4 * 2000 + 5 * 200 + 144) * 4, pool=9 * 2 * TILE, Y=5 * 432 * 4, ws=WORKSPACE),
+                 ("Y", "ws"))
 CALLS = [ROPE, WRITE, READ, ATTENTION]
 
 
@@ -110,7 +113,7 @@ def test_outputs_are_no_inputs(lib, call):
 def test_numbers(lib, call):
     wrong = dict(type=[-1, 2], tokens=[0, -1], kv_heads=[0, -2, 4, 1025], dim=[0, 4, 68, 264, -8], heads=[0, 1, 5, 1026, -6],
                  count=[0, -1, 32769], longest=[0, 6, -1], table_pages=[0, -1], pages=[0, -1, (1 << 24) + 1], rotary=[0, 1, 35, 74, -2],
-                 context=[0, -1], eps=[-1.0, float("nan")], scale=[0.0, -1.0, float("nan"), float("inf"), 1e30], window=[-1], bytes=[4095])
+                 context=[0, -1], eps=[-1.0, float("nan")], scale=[0.0, -1.0, float("nan"), float("inf"), 1e30], window=[-1], bytes=[WORKSPACE - 1])
     big = {n: 1 << 50 for n in call.need}
     for name, values in wrong.items():
         if name not in call.values or (name == "kv_heads" and call in (WRITE, READ)):
@@ -123,7 +126,8 @@ def test_numbers(lib, call):
     assert call.run(lib, change={"tokens": 1 << 24}, sizes=big) == ARG
     if "table_pages" in call.values:
         assert call.run(lib, change={"table_pages": (1 << 24) // 3 + 1}, sizes=big) == ARG
-        assert call.run(lib, change={"table_pages": (1 << 24) // 3}, sizes=big) == 0
+        most = {"table_pages": (1 << 24) // 3, **({"bytes": 1 << 40} if call is ATTENTION else {})}
+        assert call.run(lib, change=most, sizes=big) == 0
 
 
 @pytest.mark.parametrize("call", CALLS, ids=lambda c: c.entry)
@@ -151,7 +155,9 @@ def test_no_gate_takes_no_view(lib):
 
 
 def test_no_workspace_where_none_is_needed(lib):
-    assert ATTENTION.run(lib, change={"table_pages": 1, "ws": 0, "bytes": 0}) == 0
+    """Four pages are one piece."""
+    assert ATTENTION.run(lib, change={"table_pages": 4, "ws": 0, "bytes": 0}) == 0
+    assert ATTENTION.run(lib, change={"table_pages": 5, "ws": 0, "bytes": 0}) == ARG
 
 
 def test_bytes_and_workspace(lib):
@@ -161,7 +167,7 @@ def test_bytes_and_workspace(lib):
         assert lib.sm_kv4_bytes(*args, ctypes.byref(n)) == ARG
     assert lib.sm_kv4_bytes(7, 3, 200, None) == ARG
     good = (5, 3, 4, 6, 6, 2, 72)
-    assert lib.sm_kv4_attention_workspace(*good, ctypes.byref(n)) == 0 and n.value == 4096
+    assert lib.sm_kv4_attention_workspace(*good, ctypes.byref(n)) == 0 and n.value == WORKSPACE
     assert lib.sm_kv4_attention_workspace(*good, None) == ARG
     for at in range(7):
         bad = list(good)
