@@ -348,7 +348,8 @@ int sm_f8_gate_up(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int co
  * page number outside [0, pages) stands for positions that are not there, and
  * a row before a sequence's position 0 has none. Rows of no sequence stay as
  * they were. Tables that give two written positions the same place leave
- * either's bytes there, or a mixture.
+ * either's bytes there, or a mixture, and so do starts that go back in an
+ * output row of the sequences around them.
  *
  * Types are SM_TYPE_F32 or SM_TYPE_BF16, one for all tensors of a call. dim is
  * a multiple of 8 from 8 to 256. A view is {stride, head, offset}: row t, head
@@ -394,11 +395,16 @@ int sm_kv4_read(sm_ctx *ctx, uint64_t pool, int pages, int kv_heads, int dim, in
  * kv_heads; key-value head h serves the heads from h * heads / kv_heads on.
  * scale is finite and > 0. Rows that have no position, or only scores of
  * -infinity, are 0. What positions outside a row's range hold does not count,
- * whatever it is. Sums and the softmax are in f32; for bf16 the probabilities
- * are rounded to bf16, for f32 nothing is rounded to fewer bits. Y [tokens x
- * heads x dim] is without gaps. The same inputs give the same bits. The
- * workspace holds sm_kv4_attention_workspace(...) bytes (0 where that is 0);
- * a call leaves nothing in it that a later call needs. */
+ * whatever it is. Sums and the softmax are in f32, and scores have to lie in
+ * its range. For f32 tensors nothing is rounded to fewer bits. For bf16 ones
+ * the probabilities are rounded to bf16 (2^-8 each), and in calls of many rows
+ * (from 1024 of a key-value head) the queries are taken as two 8-bit numbers
+ * each, off by 2^-22 of the row's largest at most, whose products with the
+ * codes may lose 7 * 2^-13 of their magnitudes in a score (1e-5 of it, usually).
+ * A query that is not finite spoils its own row and no other. Y [tokens x heads
+ * x dim] is without gaps. The same inputs give the same bits. The workspace
+ * holds sm_kv4_attention_workspace(...) bytes (0 where that is 0); a call leaves
+ * nothing in it that a later call needs. */
 int sm_kv4_attention_workspace(int tokens, int count, int longest, int table_pages, int heads, int kv_heads, int dim,
                                uint64_t *bytes);
 int sm_kv4_attention(sm_ctx *ctx, uint64_t Q, const int64_t *q_view, int type, int tokens, int count, int longest,

@@ -85,19 +85,41 @@ __device__ __forceinline__ void load8(const T *p, bool vec, float v[8]) {
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, bf16x2));
 }
+// 16 bytes of neighbours, kPer values, as they are and as numbers: a load apart
+// from what needs it, so that others follow before it is waited for. Without
+// `vec` value by value.
 template <typename T>
-__device__ __forceinline__ void store8(T *p, bool vec, const float v[8]) {
-    if constexpr (sizeof(T) == 4) {
-        if (vec) {
-            ((float4 *)p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            ((float4 *)p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+struct Piece16 {
+    static constexpr int kPer = 16 / sizeof(T);
+    T v[kPer];
+    template <bool vec>
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (vec) {
+            *(uint4 *)v = *(const uint4 *)p;
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = v[i];
+            for (int i = 0; i < kPer; i++) v[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) v[i] = 0;
+    }
+    __device__ __forceinline__ float at(int i) const { return value(v[i]); }
+};
+template <bool vec, typename T>
+__device__ __forceinline__ void store16(T *p, const float *v) {
+    constexpr int kPer = 16 / sizeof(T);
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (vec) {
+            *(float4 *)p = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; i++) p[i] = v[i];
         }
     } else {
         const uint32_t w[4] = {bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
-        if (vec) {
+        if constexpr (vec) {
             *(uint4 *)p = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
 #pragma unroll
