@@ -118,6 +118,35 @@ struct Args {
         napi_get_value_string_utf8(env, argv[i], &s[0], n + 1, &n);
         return s;
     }
+    // A view: null, or an array of three safe integers, which go to `to`.
+    const int64_t *view(size_t i, int64_t to[3]) {
+        napi_valuetype type = napi_undefined;
+        if (ok) napi_typeof(env, argv[i], &type);
+        if (!ok || type == napi_null) return nullptr;
+        bool is = false;
+        uint32_t n = 0;
+        if (napi_is_array(env, argv[i], &is) != napi_ok || !is || napi_get_array_length(env, argv[i], &n) != napi_ok || n != 3) {
+            ok = false;
+            type_error(env, "expected null or a view of three numbers");
+            return nullptr;
+        }
+        for (uint32_t j = 0; j < 3; j++) {
+            napi_value e;
+            double v = 0;
+            if (napi_get_element(env, argv[i], j, &e) != napi_ok || napi_get_value_double(env, e, &v) != napi_ok) {
+                ok = false;
+                type_error(env, "expected null or a view of three numbers");
+                return nullptr;
+            }
+            if (!(v >= -9007199254740991.0 && v <= 9007199254740991.0) || v != (double)(int64_t)v) {
+                ok = false;
+                napi_throw_range_error(env, nullptr, "a view's numbers must be safe integers");
+                return nullptr;
+            }
+            to[j] = (int64_t)v;
+        }
+        return to;
+    }
     // Bytes of a TypedArray, DataView, Buffer or ArrayBuffer.
     bool bytes(size_t i, void **data, size_t *len) {
         bool is = false;
@@ -501,6 +530,111 @@ napi_value F8GateUp(napi_env env, napi_callback_info info) {
         return nullptr;
     return undefined(env);
 }
+// qkNormRope(ctx, Q, qView, K, kView, type, tokens, heads, kvHeads, dim, qGamma, kGamma, eps, Cos, Sin, rotary, context, positions, Yq, Yk)
+napi_value QkNormRope(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(20)) return nullptr;
+    int64_t q[3], k[3];
+    sm_ctx *ctx = a.ctx(0);
+    uint64_t Q = a.u64(1);
+    const int64_t *qv = a.view(2, q);
+    uint64_t K = a.u64(3);
+    const int64_t *kv = a.view(4, k);
+    int type = a.i32(5), tokens = a.i32(6), heads = a.i32(7), kv_heads = a.i32(8), dim = a.i32(9);
+    uint64_t qg = a.u64(10), kg = a.u64(11);
+    const float eps = (float)a.num(12);
+    uint64_t Cos = a.u64(13), Sin = a.u64(14);
+    int rotary = a.i32(15), context = a.i32(16);
+    uint64_t positions = a.u64(17), Yq = a.u64(18), Yk = a.u64(19);
+    if (!a.ok || fail(env, ctx, sm_qk_norm_rope(ctx, Q, qv, K, kv, type, tokens, heads, kv_heads, dim, qg, kg, eps, Cos, Sin,
+                                                rotary, context, positions, Yq, Yk)))
+        return nullptr;
+    return undefined(env);
+}
+// kv4Bytes(pages, kvHeads, dim)
+napi_value Kv4Bytes(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(3)) return nullptr;
+    int pages = a.i32(0), kv_heads = a.i32(1), dim = a.i32(2);
+    uint64_t n = 0;
+    if (!a.ok || fail(env, nullptr, sm_kv4_bytes(pages, kv_heads, dim, &n))) return nullptr;
+    return number(env, (double)n);
+}
+// kv4Write(ctx, K, kView, V, vView, type, tokens, count, longest, starts, lengths, table, tablePages, kvHeads, dim, pool, pages)
+napi_value Kv4Write(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(17)) return nullptr;
+    int64_t k[3], v[3];
+    sm_ctx *ctx = a.ctx(0);
+    uint64_t K = a.u64(1);
+    const int64_t *kv = a.view(2, k);
+    uint64_t V = a.u64(3);
+    const int64_t *vv = a.view(4, v);
+    int type = a.i32(5), tokens = a.i32(6), count = a.i32(7), longest = a.i32(8);
+    uint64_t starts = a.u64(9), lengths = a.u64(10), table = a.u64(11);
+    int table_pages = a.i32(12), kv_heads = a.i32(13), dim = a.i32(14);
+    uint64_t pool = a.u64(15);
+    int pages = a.i32(16);
+    if (!a.ok || fail(env, ctx, sm_kv4_write(ctx, K, kv, V, vv, type, tokens, count, longest, starts, lengths, table, table_pages,
+                                             kv_heads, dim, pool, pages)))
+        return nullptr;
+    return undefined(env);
+}
+// kv4Read(ctx, pool, pages, kvHeads, dim, tokens, count, longest, starts, lengths, table, tablePages, K, kView, V, vView, type)
+napi_value Kv4Read(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(17)) return nullptr;
+    int64_t k[3], v[3];
+    sm_ctx *ctx = a.ctx(0);
+    uint64_t pool = a.u64(1);
+    int pages = a.i32(2), kv_heads = a.i32(3), dim = a.i32(4), tokens = a.i32(5), count = a.i32(6), longest = a.i32(7);
+    uint64_t starts = a.u64(8), lengths = a.u64(9), table = a.u64(10);
+    int table_pages = a.i32(11);
+    uint64_t K = a.u64(12);
+    const int64_t *kv = a.view(13, k);
+    uint64_t V = a.u64(14);
+    const int64_t *vv = a.view(15, v);
+    int type = a.i32(16);
+    if (!a.ok || fail(env, ctx, sm_kv4_read(ctx, pool, pages, kv_heads, dim, tokens, count, longest, starts, lengths, table,
+                                            table_pages, K, kv, V, vv, type)))
+        return nullptr;
+    return undefined(env);
+}
+// kv4AttentionWorkspace(tokens, count, longest, tablePages, heads, kvHeads, dim)
+napi_value Kv4AttentionWorkspace(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(7)) return nullptr;
+    int tokens = a.i32(0), count = a.i32(1), longest = a.i32(2), table_pages = a.i32(3), heads = a.i32(4), kv_heads = a.i32(5),
+        dim = a.i32(6);
+    uint64_t n = 0;
+    if (!a.ok || fail(env, nullptr, sm_kv4_attention_workspace(tokens, count, longest, table_pages, heads, kv_heads, dim, &n)))
+        return nullptr;
+    return number(env, (double)n);
+}
+// kv4Attention(ctx, Q, qView, type, tokens, count, longest, starts, lengths, table, tablePages, pool, pages, heads, kvHeads, dim, scale,
+//              window, G, gView, Y, workspace, workspaceBytes)
+napi_value Kv4Attention(napi_env env, napi_callback_info info) {
+    Args a(env, info);
+    if (!a.need(23)) return nullptr;
+    int64_t q[3], g[3];
+    sm_ctx *ctx = a.ctx(0);
+    uint64_t Q = a.u64(1);
+    const int64_t *qv = a.view(2, q);
+    int type = a.i32(3), tokens = a.i32(4), count = a.i32(5), longest = a.i32(6);
+    uint64_t starts = a.u64(7), lengths = a.u64(8), table = a.u64(9);
+    int table_pages = a.i32(10);
+    uint64_t pool = a.u64(11);
+    int pages = a.i32(12), heads = a.i32(13), kv_heads = a.i32(14), dim = a.i32(15);
+    const float scale = (float)a.num(16);
+    int window = a.i32(17);
+    uint64_t G = a.u64(18);
+    const int64_t *gv = a.view(19, g);
+    uint64_t Y = a.u64(20), ws = a.u64(21), wsb = a.u64(22);
+    if (!a.ok || fail(env, ctx, sm_kv4_attention(ctx, Q, qv, type, tokens, count, longest, starts, lengths, table, table_pages,
+                                                 pool, pages, heads, kv_heads, dim, scale, window, G, gv, Y, ws, wsb)))
+        return nullptr;
+    return undefined(env);
+}
 // synthNormal(ctx, dst, offsetBytes, n, seed, stream, sigma) and
 // synthUniformPm(ctx, dst, offsetBytes, n, seed, stream, amp)
 napi_value SynthNormal(napi_env env, napi_callback_info info) {
@@ -647,6 +781,12 @@ napi_value ModuleInit(napi_env env, napi_value exports) {
                {"f8Project", F8Project},
                {"f8GateUpWorkspace", F8GateUpWorkspace},
                {"f8GateUp", F8GateUp},
+               {"qkNormRope", QkNormRope},
+               {"kv4Bytes", Kv4Bytes},
+               {"kv4Write", Kv4Write},
+               {"kv4Read", Kv4Read},
+               {"kv4AttentionWorkspace", Kv4AttentionWorkspace},
+               {"kv4Attention", Kv4Attention},
                {"synthNormal", SynthNormal},
                {"synthUniformPm", SynthUniformPm},
                {"synthBlobs", SynthBlobs},

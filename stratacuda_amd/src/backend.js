@@ -387,6 +387,67 @@ export class HipBackend {
             this.owned(a.workspace, 'workspace'), a.workspace.byteLength);
         this.dispatches++;
     }
+    // ------------------------- attention over a 4-bit cache (kind 'hip')
+    // A cache is {pool, pages, kvHeads, dim}: pages of 64 positions;
+    // include/strata_mi355x.h has the layout. kv4Cache allocates one, all
+    // zeros; free its pool as any other buffer. Sequences are {count, tokens,
+    // longest, starts, lengths, table, tablePages} with three i32 buffers, read
+    // when a call runs. A view is [stride, head, offset] in values, left out:
+    // rows of heads of dim values without gaps. type: 'f32' (left out) or
+    // 'bf16', for all tensors of a call.
+    kv4Cache(pages, kvHeads, dim) {
+        return {pool: this.allocBytes(this.addon.kv4Bytes(pages, kvHeads, dim), 'u32'), pages, kvHeads, dim};
+    }
+    kv4Sequences(q) {
+        if (!q) throw Error('Invalid HIP sequences');
+        return [q.tokens, q.count, q.longest, this.owned(q.starts, 'starts'), this.owned(q.lengths, 'lengths'),
+            this.owned(q.table, 'table'), q.tablePages];
+    }
+    kv4Pool(cache) {
+        if (!cache) throw Error('Invalid HIP cache');
+        return this.owned(cache.pool, 'pool');
+    }
+    // Each head of a.Q [tokens x heads x dim] and a.K [tokens x kvHeads x dim] normed and turned by its row's position, into
+    // a.Yq and a.Yk.
+    qkNormRope(a) {
+        this.assertAlive();
+        this.addon.qkNormRope(this.ctx, this.owned(a.Q, 'Q'), a.qView || null, this.owned(a.K, 'K'), a.kView || null,
+            f8Type(a.type), a.tokens, a.heads, a.kvHeads, a.dim, this.owned(a.qGamma, 'qGamma'), this.owned(a.kGamma, 'kGamma'),
+            a.eps, this.owned(a.cos, 'cos'), this.owned(a.sin, 'sin'), a.rotary, a.context, this.owned(a.positions, 'positions'),
+            this.owned(a.Yq, 'Yq'), this.owned(a.Yk, 'Yk'));
+        this.dispatches++;
+    }
+    // The rows of a.K and a.V into the last positions of their sequences.
+    kv4Write(a) {
+        this.assertAlive();
+        const pool = this.kv4Pool(a.cache);
+        this.addon.kv4Write(this.ctx, this.owned(a.K, 'K'), a.kView || null, this.owned(a.V, 'V'), a.vView || null,
+            f8Type(a.type), ...this.kv4Sequences(a.sequences), a.cache.kvHeads, a.cache.dim, pool, a.cache.pages);
+        this.dispatches++;
+    }
+    // The last positions of the sequences, as many as they have rows, as numbers into a.K and a.V.
+    kv4Read(a) {
+        this.assertAlive();
+        const pool = this.kv4Pool(a.cache);
+        this.addon.kv4Read(this.ctx, pool, a.cache.pages, a.cache.kvHeads, a.cache.dim, ...this.kv4Sequences(a.sequences),
+            this.owned(a.K, 'K'), a.kView || null, this.owned(a.V, 'V'), a.vView || null, f8Type(a.type));
+        this.dispatches++;
+    }
+    // 0: none is needed.
+    kv4AttentionWorkspaceBytes(sequences, heads, cache) {
+        return this.addon.kv4AttentionWorkspace(sequences.tokens, sequences.count, sequences.longest, sequences.tablePages, heads,
+            cache.kvHeads, cache.dim);
+    }
+    // a.Y = softmax(a.scale * a.Q . keys) . values over each row's positions (the last a.window of them), times sigmoid(a.gate).
+    kv4Attention(a) {
+        this.assertAlive();
+        const pool = this.kv4Pool(a.cache);
+        this.addon.kv4Attention(this.ctx, this.owned(a.Q, 'Q'), a.qView || null, f8Type(a.type), ...this.kv4Sequences(a.sequences),
+            pool, a.cache.pages, a.heads, a.cache.kvHeads, a.cache.dim, a.scale, a.window || 0, a.gate ? this.owned(a.gate, 'gate') : 0,
+            (a.gate && a.gateView) || null, this.owned(a.Y, 'Y'), a.workspace ? this.owned(a.workspace, 'workspace') : 0,
+            a.workspace ? a.workspace.byteLength : 0);
+        this.dispatches++;
+    }
     // Seeded synthetic data, bit-identical to the CPU oracle's generator.
     synthNormal(buffer, n, seed, stream, sigma, offsetBytes) {
         this.addon.synthNormal(this.ctx, this.owned(buffer, 'synth'), offsetBytes || 0, n, seed, stream, sigma);
