@@ -7,9 +7,16 @@
 
 namespace smi {
 
-// The least pages that are worth a piece: one a wave.
+// The least pages that are worth a piece: one a wave. 2048 positions of 24 heads on 2 of dimension 256, f32: 16.9 us, 16.7 with
+// 2 and 19.5 with 8.
 constexpr int kKv4Least = 4;
-// From so many rows a wave joins a row's pieces: they fill the GPU.
+// Rows that reach up to so many pages are not cut: two or three turns of four pages take less than the launch that joins
+// them. In pieces of 4 pages and whole, us: 500 positions, 32 heads on 8 of dimension 128 in bf16, 11.0 and 8.8 (32 sequences 11.9 and
+// 10.0), 24 heads on 2 of 256 in f32 18.0 and 17.2; 700 positions 10.9 and 9.5 (32 sequences 14.3 and 11.1) but 17.5 and 19.9
+(bf16 14.6 and 15.6): f32 and more than 128 dimensions, whose turns are longer, from fewer pages.
+constexpr int kKv4Whole = 12, kKv4WholeWide = 8;
+// From so many rows a wave joins a row's pieces, else sixteen do. Sixteen against one, us: 24 rows of 128 pieces 26 and 47, 64
+// rows of 32 14.8 and 16.8, 256 rows of 43 22.6 and 22.4, 512 rows of 25 38.8 and 37.3, 1024 rows 46.5 and 42.6.
 constexpr int kKv4JoinRows = 512;
 constexpr int kKv4PromptRows = 256;
 
@@ -28,26 +35,35 @@ struct Kv4Shape {
     int tile_rows, tiles, pieces, least;
     uint64_t slots, part_bytes, stat_bytes, bytes;
 };
-inline Kv4Shape kv4_shape(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16) {
-    Kv4Shape s;
+// The pages that a sequence's rows reach at most.
+inline int64_t kv4_pages(const Kv4Sequences &q, int window) {
+    return window > 0 ? std::min<int64_t>(q.table_pages, ((int64_t)window + q.longest) / 64 + 2) : q.table_pages;
+}
+inline bool kv4_prompt(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16) {
     const int64_t rows = (int64_t)q.longest * (heads / kv_heads);
     const int pitch = kv4_pitch(dim);
-    const int64_t pages = window > 0 ? std::min<int64_t>(q.table_pages, ((int64_t)window + q.longest) / 64 + 2) : q.table_pages;
-    const int64_t reached = std::max<int64_t>(pages - q.longest / 128, 1);  // a row's on average, of the longest sequence's
+    const int64_t reached = std::max<int64_t>(kv4_pages(q, window) - q.longest / 128, 1);  // a row's on average, of the longest sequence's
     const int64_t turns = (int64_t)q.count * kv_heads * ((rows + 15) / 16) * (17 + reached);
-    s.prompt = (bf16 || pitch <= 128) && rows >= kKv4PromptLeast &&
-               turns >= (pitch == 64 ? kKv4PromptTurns64 : bf16 ? kKv4PromptTurns : kKv4PromptTurnsF32);
+    return (bf16 || pitch <= 128) && rows >= kKv4PromptLeast &&
+           turns >= (pitch == 64 ? kKv4PromptTurns64 : bf16 ? kKv4PromptTurns : kKv4PromptTurnsF32);
+}
+inline Kv4Shape kv4_cut(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16, bool prompt) {
+    Kv4Shape s;
+    const int64_t rows = (int64_t)q.longest * (heads / kv_heads), pages = kv4_pages(q, window);
+    const int pitch = kv4_pitch(dim);
+    const bool wide = pitch > 128 || !bf16;
+    s.prompt = prompt;
     s.tile_rows = s.prompt ? kKv4PromptRows : 16;
     s.tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
     s.least = kKv4Least;
     const int64_t each = (int64_t)kv_heads * s.tiles;
-    const int64_t most = q.table_pages <= s.least ? 1 : (int64_t)q.count * ((q.table_pages + s.least - 1) / s.least);
+    const int64_t most = pages <= (wide ? kKv4WholeWide : kKv4Whole) ? 1 : (int64_t)q.count * ((q.table_pages + s.least - 1) / s.least);
     // Sixteen rows: a workgroup for each CU, or three for two CUs where registers leave room for three on each (32 sequences
     // of dimension 128: 51 us with one for each, 42 with these). Prompts that leave CUs idle: what one round holds, two
     // where most of the context is the prompt itself, whose first rows reach little of it (4096 tokens, 12 heads on 4 of
     // dimension 192: 179 us whole, 128 in pieces).
     const int64_t whole = each * q.count;
-    int64_t pieces = !s.prompt ? ((pitch > 128 || !bf16 ? 256 : 384) + each - 1) / each
+    int64_t pieces = !s.prompt ? ((wide ? 256 : 384) + each - 1) / each
                      : whole >= 256 ? 1 : (64 * (int64_t)q.table_pages <= 2 * (int64_t)q.longest ? 512 : 256) / whole;
     if (pieces > most) pieces = most;
     s.pieces = pieces < 1 ? 1 : (int)pieces;
@@ -58,12 +74,16 @@ inline Kv4Shape kv4_shape(const Kv4Sequences &q, int heads, int kv_heads, int di
     if (s.pieces == 1) s.least = q.table_pages + 1;  // one piece a sequence: as large as any
     return s;
 }
+inline Kv4Shape kv4_shape(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16) {
+    return kv4_cut(q, heads, kv_heads, dim, window, bf16, kv4_prompt(q, heads, kv_heads, dim, window, bf16));
+}
 
-// Enough for either type, with a window and without one: a window only decides which kernel it is.
+// Enough for either type and every window: the narrowest and none tell which kernels it may be, and none has the most pieces.
 inline uint64_t kv4_workspace(const Kv4Sequences &q, int heads, int kv_heads, int dim) {
     uint64_t most = 0;
     for (int bf16 = 0; bf16 < 2; bf16++)
-        for (int window = 0; window < 2; window++) most = std::max(most, kv4_shape(q, heads, kv_heads, dim, window, bf16).bytes);
+        for (int window = 0; window < 2; window++)
+            most = std::max(most, kv4_cut(q, heads, kv_heads, dim, 0, bf16, kv4_prompt(q, heads, kv_heads, dim, window, bf16)).bytes);
     return most;
 }
 

@@ -1,5 +1,5 @@
 """Attention over a 4-bit cache by the kernel of many rows, and by both with
-long contexts, on the GPU against 64 bits (kv4_plain). test_kv4_rules.py holds
+long contexts and in pieces, on the GPU against 64 bits (kv4_plain). test_kv4_rules.py holds
 the batches to the kernels. Queries and codes are those whose scores are exact
 (test_gpu_kv4): in bf16 a query is one e4m3 number then, and products of eight
 neighbours, of one scale, lie less than 2^6 apart. No counterpart in the
@@ -231,7 +231,7 @@ def test_sequences_that_are_none(be, name):
     b.free()
 
 
-@pytest.mark.parametrize("name,type", [("WHOLE", "bf16"), ("PIECES", "bf16"), ("PIECES", "f32")])
+@pytest.mark.parametrize("name,type", [("WHOLE", "bf16"), ("PIECES", "bf16"), ("PIECES", "f32"), ("FEW", "f32"), ("SOME", "bf16")])
 def test_captured_and_replayed(be, name, type):
     """A graph takes the lengths and tables that stand there when it runs, as an eager call does."""
     rng = np.random.default_rng(8)
@@ -283,6 +283,32 @@ def test_more_than_64_pages(be, hole, type, dim):
         gone = np.clip(positions - 65 * 64 + 1, 0, 64)
         positions = positions - gone
     some(b, q, run_attention(be, b, q, scale, type), scale, type, 0, rows, positions, held=(k, v))
+    b.free()
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 24, 128, 192, 200, 256])
+@pytest.mark.parametrize("name", ["FEW", "SOME"])
+@pytest.mark.parametrize("window", (0,) + batches.LONG_WINDOWS)
+def test_few_rows_in_pieces(be, window, name, dim, type):
+    """Sixteen rows a workgroup over a part of the context, with a gate and a page that is none; views that no wide load fits."""
+    rng = np.random.default_rng(dim)
+    which = getattr(batches, name)
+    heads = which["heads"]
+    b = batch(be, rng, which, dim)
+    q, g = queries(rng, (b.tokens, heads, dim)), plain.bf16(rng.normal(0, 4, (b.tokens, heads, dim)))
+    qv, gv = (heads * dim + heads + 11, dim + 1, 3), (heads * dim + 5, dim, 1)
+    scale = dim ** -0.5 / 4
+    got = run_attention(be, b, q, scale, type, window=window, gate=g, q_view=qv, gate_view=gv)
+    check(b, q, got, scale, type, window=window, gate=g)
+    if not window:  # positions 64 to 127 of the longest sequence are not there
+        b.table[0, 1] = -7
+        be.write(b.seqs.table, b.table)
+        got = run_attention(be, b, q, scale, type, gate=g, q_view=qv, gate_view=gv)
+        n, length = b.sequences[0]
+        both = [plain.get(b.host, b.kv, dim, b.page(0, p), p % 64) for p in range(length) if not 64 <= p < 128]
+        held = tuple(np.stack([x[i] for x in both]) for i in (0, 1))
+        some(b, q, got, scale, type, 0, np.arange(n), length - n - 64 + np.arange(n), held=held, gate=g)
     b.free()
 
 

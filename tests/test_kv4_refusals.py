@@ -58,8 +58,8 @@ class Call:
             lib.stub_free(ctx)
 
 
-SEQ = dict(tokens=5, count=3, longest=4, starts=0x10, lengths=0x20, table=0x30, table_pages=6)
-SEQ_NEED = dict(starts=16, lengths=12, table=72)
+SEQ = dict(tokens=5, count=3, longest=4, starts=0x10, lengths=0x20, table=0x30, table_pages=18)
+SEQ_NEED = dict(starts=16, lengths=12, table=216)
 TILE = 68 * 128  # bytes of a page's tile of dim 72 to 128
 ROPE = Call("sm_qk_norm_rope", "Q qv K kv type tokens heads kv_heads dim qg kg eps Cos Sin rotary context positions Yq Yk",
             dict(Q=0x100, qv=view(2000, 200, 72), K=0x200, kv=None, type=0, tokens=5, heads=6, kv_heads=2, dim=72, qg=0x300, kg=0x400,
@@ -72,8 +72,8 @@ WRITE = Call("sm_kv4_write", "K kv V vv type tokens count longest starts lengths
 READ = Call("sm_kv4_read", "pool pages kv_heads dim tokens count longest starts lengths table table_pages K kv V vv type",
             dict(SEQ, K=0x100, kv=None, V=0x200, vv=view(300, 100, 7), type=0, kv_heads=2, dim=72, pool=0x300, pages=9),
             dict(SEQ_NEED, K=5 * 144 * 4, V=(4 * 300 + 100 + 7 + 72) * 4, pool=9 * 2 * TILE), ("K", "V"))
-# 6 pieces of 4 pages and one more a sequence, of 2 heads' 16 rows: 128 sums and two statistics; 2 words a sequence
-WORKSPACE = (6 + 3) * 2 * 16 * (128 + 2) * 4 + 3 * 8
+# 15 pieces of 4 pages and one more a sequence, of 2 heads' 16 rows: 128 sums and two statistics; 2 words a sequence
+WORKSPACE = (15 + 3) * 2 * 16 * (128 + 2) * 4 + 3 * 8
 ATTENTION = Call("sm_kv4_attention", "Q qv type tokens count longest starts lengths table table_pages pool pages heads kv_heads dim scale "
                  "window G gv Y ws bytes",
                  dict(SEQ, Q=0x100, qv=None, type=0, pool=0x300, pages=9, heads=6, kv_heads=2, dim=72, scale=0.1, window=0, G=0x400,
@@ -155,9 +155,9 @@ def test_no_gate_takes_no_view(lib):
 
 
 def test_no_workspace_where_none_is_needed(lib):
-    """Four pages are one piece."""
-    assert ATTENTION.run(lib, change={"table_pages": 4, "ws": 0, "bytes": 0}) == 0
-    assert ATTENTION.run(lib, change={"table_pages": 5, "ws": 0, "bytes": 0}) == ARG
+    """Eight pages are one piece in either type."""
+    assert ATTENTION.run(lib, change={"table_pages": 8, "ws": 0, "bytes": 0}) == 0
+    assert ATTENTION.run(lib, change={"table_pages": 9, "ws": 0, "bytes": 0}) == ARG
 
 
 def test_bytes_and_workspace(lib):
@@ -166,7 +166,7 @@ def test_bytes_and_workspace(lib):
     for args in ((0, 3, 200), (7, 0, 200), (7, 3, 201), (7, 3, 0), ((1 << 24) + 1, 3, 200)):
         assert lib.sm_kv4_bytes(*args, ctypes.byref(n)) == ARG
     assert lib.sm_kv4_bytes(7, 3, 200, None) == ARG
-    good = (5, 3, 4, 6, 6, 2, 72)
+    good = (5, 3, 4, 18, 6, 2, 72)
     assert lib.sm_kv4_attention_workspace(*good, ctypes.byref(n)) == 0 and n.value == WORKSPACE
     assert lib.sm_kv4_attention_workspace(*good, None) == ARG
     for at in range(7):

@@ -48,6 +48,11 @@ def test_the_gpu_tests_reach_every_kernel(rules):
         assert s.prompt and s.pieces == 1 and batches.LONG["sequences"][0][1] > 64 * 64
     for dim in (192, 256):  # f32 has no kernel of many rows there
         assert not of(rules, batches.WHOLE, dim, "f32").prompt
+    for type, dim in batches.TYPES:
+        for name in ("FEW", "SOME"):
+            for window in (0,) + batches.LONG_WINDOWS:
+                s = of(rules, getattr(batches, name), dim, type, window)
+                assert not s.prompt and (s.pieces > 4 if window in (0, 1000) else s.pieces == 1)
     for type in ("bf16", "f32"):
         s = of(rules, batches.LONG_ROWS, 64, type)
         assert not s.prompt and sum(-(-length // 64) for _, length in batches.LONG_ROWS["sequences"]) > 64 * s.pieces
@@ -79,9 +84,10 @@ def test_shapes_and_workspace(rules):
 
 
 def test_no_workspace_for_short_tables(rules):
-    for width in range(1, 5):
-        assert rules.rule_workspace(3, 4, width, 6, 2, 72) == 0
-    assert rules.rule_workspace(3, 4, 5, 6, 2, 72) > 0
+    for width in range(1, 20):
+        assert (rules.rule_workspace(3, 4, width, 6, 2, 72) == 0) == (width <= 8)
+        for bf16, most in ((0, 8), (1, 12)):
+            assert (rules.shape(3, 4, width, 6, 2, 72, 0, bf16).pieces == 1) == (width <= most)
 
 
 def test_more_work_never_returns_to_sixteen_rows(rules):
