@@ -13,7 +13,7 @@ constexpr int kKv4Least = 4;
 // Rows that reach up to so many pages are not cut: two or three turns of four pages take less than the launch that joins
 // them. In pieces of 4 pages and whole, us: 500 positions, 32 heads on 8 of dimension 128 in bf16, 11.0 and 8.8 (32 sequences 11.9 and
 // 10.0), 24 heads on 2 of 256 in f32 18.0 and 17.2; 700 positions 10.9 and 9.5 (32 sequences 14.3 and 11.1) but 17.5 and 19.9
-(bf16 14.6 and 15.6): f32 and more than 128 dimensions, whose turns are longer, from fewer pages.
+// (bf16 14.6 and 15.6): f32 and more than 128 dimensions, whose turns are longer, from fewer pages.
 constexpr int kKv4Whole = 12, kKv4WholeWide = 8;
 // From so many rows a wave joins a row's pieces, else sixteen do. Sixteen against one, us: 24 rows of 128 pieces 26 and 47, 64
 // rows of 32 14.8 and 16.8, 256 rows of 43 22.6 and 22.4, 512 rows of 25 38.8 and 37.3, 1024 rows 46.5 and 42.6.
