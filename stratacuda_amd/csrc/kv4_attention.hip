@@ -72,15 +72,19 @@ __device__ __forceinline__ float sum_of_halves(float v) {
 }
 
 // ---------------------------------------------------------------- the shares
-// A sequence's pages are cut into pieces of equally many pages; piece number
-// `slot` of all sequences' is a workgroup's. Small ones are whole turns of a
-// workgroup's kTurn pages: 2 sequences of 8192 positions, 32 heads on 8 of
-// dimension 128, take 13.5 us in pieces of 8 pages and 14.8 in pieces of 6.
-// Larger ones are as equal as they can be (32 such sequences 42.3 and 42.9). A sequence with rows has one
-// piece at least.
+// A workgroup takes a tile of a sequence's rows for one key-value head and a
+// piece of its pages. Where no sequence is cut, the tiles of all sequences lie
+// in blockIdx.x one after another: a batch of one long prompt and many single
+// tokens has no more workgroups than it has tiles. Else blockIdx.y is the piece
+// of all sequences', of equally many pages; a sequence with rows has one at
+// least. Small pieces are whole turns of a workgroup's kTurn pages: 2
+// sequences of 8192 positions, 32 heads on 8 of dimension 128, take 13.5 us in
+// pieces of 8 pages and 14.8 in pieces of 6. Larger ones are as equal as they
+// can be (32 such sequences 42.3 and 42.9).
 struct Piece {
     int s, first, end;  // the sequence and the pages; s = -1: there is no such piece
     int number, count;  // which of the sequence's pieces it is
+    int tile;           // of the sequence's rows
     kv4::Span span;
 };
 // The pages that the sequence's rows reach.
@@ -90,28 +94,34 @@ __device__ __forceinline__ int2 pages_of(const kv4::Span &a, int window) {
     return make_int2(lo, max((a.length + 63) / 64, lo));
 }
 __device__ __forceinline__ int pieces_in(const int2 &p, int n, int each) { return n > 0 ? max((p.y - p.x + each - 1) / each, 1) : 0; }
-template <int kTurn>
-__device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int least, int slot) {
-    const int lane = threadIdx.x % 64;
+template <int kTileRows, int kTurn>
+__device__ Piece piece_of(const Kv4Attention &a) {
+    const Kv4Sequences &q = a.q;
+    const int lane = threadIdx.x % 64, at_x = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
     const auto sequence = [&](int s) { return s < q.count ? kv4::span(q, s) : kv4::Span{0, 0, 0}; };
-    int total = 0;
     const kv4::Span a0 = sequence(lane);
-    for (int at = 0; at < q.count; at += 64) {
-        const kv4::Span a = at == 0 ? a0 : sequence(at + lane);
-        const int2 p = pages_of(a, window);
-        int some = a.n > 0 ? p.y - p.x : 0;
-        if (q.count > 1)
+    const bool whole = a.pieces == 1;
+    const int slot = whole ? at_x : blockIdx.y;
+    int each = 0;
+    if (!whole) {
+        int total = 0;
+        for (int at = 0; at < q.count; at += 64) {
+            const kv4::Span b = at == 0 ? a0 : sequence(at + lane);
+            const int2 p = pages_of(b, a.window);
+            int some = b.n > 0 ? p.y - p.x : 0;
+            if (q.count > 1)
 #pragma unroll
-            for (int i = 1; i < 64; i *= 2) some += __shfl_xor(some, i, 64);
-        total += __builtin_amdgcn_readfirstlane(some);
+                for (int i = 1; i < 64; i *= 2) some += __shfl_xor(some, i, 64);
+            total += __builtin_amdgcn_readfirstlane(some);
+        }
+        each = max(a.least, (total + a.pieces - 1) / a.pieces);
+        if (each < 4 * kTurn) each = (each + kTurn - 1) / kTurn * kTurn;
     }
-    int each = max(least, (total + pieces - 1) / pieces);
-    if (each < 4 * kTurn) each = (each + kTurn - 1) / kTurn * kTurn;
     int before = 0;
     for (int at = 0; at < q.count; at += 64) {
-        const kv4::Span a = at == 0 ? a0 : sequence(at + lane);
-        const int2 p = pages_of(a, window);
-        const int mine = pieces_in(p, a.n, each);
+        const kv4::Span b = at == 0 ? a0 : sequence(at + lane);
+        const int2 p = pages_of(b, a.window);
+        const int mine = whole ? (b.n * group + kTileRows - 1) / kTileRows : pieces_in(p, b.n, each);
         int upto = mine;  // with this lane's
         if (q.count > 1)
 #pragma unroll
@@ -125,12 +135,13 @@ __device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int lea
             // the same in all lanes: kept, and what it leads to, in scalar registers
             const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
             const int count = of(mine), number = slot - before - (of(upto) - count), first = of(p.x), end = of(p.y);
-            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count,
-                    {of(a.row), of(a.n), of(a.length)}};
+            const kv4::Span span = {of(b.row), of(b.n), of(b.length)};
+            if (whole) return {at + who, first, end, 0, 1, number, span};
+            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count, at_x, span};
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
-    return {-1, 0, 0, 0, 0, {0, 0, 0}};
+    return {-1, 0, 0, 0, 0, 0, {0, 0, 0}};
 }
 
 // ------------------------------------------------------------------ 16 rows
@@ -143,6 +154,12 @@ __device__ Piece piece_of(const Kv4Sequences &q, int window, int pieces, int lea
 // one key (its block: one scale), or two dimensions of 16 positions' values.
 // The next page's keys are on their way while this one's probabilities are
 // made, its values during the products.
+//
+// Long contexts are bound by memory (24 heads on 2 of dimension 256, bf16, one
+// token over 131072 positions: 71 MB in 20 us and 6.7 to join them; 32
+// sequences of 32 heads on 8 of 128: 161 MB in 37 us, 4.4 TB/s, and 4.2), short
+// ones by what follows one another: the sequences' numbers, page numbers, keys,
+// values (2048 positions, f32: 12 us and 4.3).
 template <int NC, bool F32>
 struct Rows16 {
     static constexpr int kPitch = 64 * NC, kBlocks = 2 * NC;
@@ -219,11 +236,11 @@ __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd
     constexpr int kPitch = R::kPitch, kTiles = kPitch / 16, kLine = kPitch + 4;
     const uint32_t lane = threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const Piece piece = piece_of<4>(a.q, a.window, a.pieces, a.least, blockIdx.y);
+    const Piece piece = piece_of<16, 4>(a);
     if (piece.s < 0) return;
     if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
     const kv4::Span span = piece.span;
-    const int head = blockIdx.x % a.kv_heads, tile = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
+    const int head = blockIdx.x % a.kv_heads, tile = piece.tile, group = a.heads / a.kv_heads;
     const int rows = span.n * group - 16 * tile;  // of the sequence, from this tile's first on
     if (rows <= 0) return;
     const int first = span.length - span.n;       // the first new token's position
@@ -484,11 +501,16 @@ __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd
 // cuts products 2^13 below the largest of eight neighbours: at most 7 * 2^-13
 // of a score's products' magnitudes are lost, 1e-5 for ordinary ones, where
 // probabilities are rounded by 2^-8. Queries of f32 take bf16's unit.
+//
+// Bound by the matrix units and by what their clock allows: 8192 tokens, 32
+// heads on 8 of dimension 128, bf16, 490 to 520 us, 1.06 to 1.12 PFLOP/s; 512
+// tokens behind 32256 positions, 24 heads on 2 of 256, 349 to 376 us, 1.09 to
+// 1.17 (a library's product of 16384^3 reaches 1.35).
 template <int NC, typename T>
 struct Prompt {
     static constexpr bool kF32 = sizeof(T) == 4;
     static constexpr int kPitch = 64 * NC, kBlocks = 2 * NC, kParts = kF32 ? 3 : 1;
-    // f32 queries of more than 128 dimensions would take more registers than two waves of a SIMD have
+    // f32 queries of more than 128 dimensions would take more registers than two waves of a SIMD have: sixteen rows then
     static constexpr bool kThere = !kF32 || NC < 3;
     static constexpr int kWaves = 8, kThreads = 64 * kWaves, kRows = 32 * kWaves;
     static_assert(kRows == kKv4PromptRows, "the shapes count on it");
@@ -518,12 +540,13 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
     __shared__ uint64_t s_nan[4][kBlocks];         // values that are NaN for some rows and not there for others
     const uint32_t lane = threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const Piece piece = piece_of<1>(a.q, a.window, a.pieces, a.least, blockIdx.y);
+    const Piece piece = piece_of<R::kRows, 1>(a);
     if (piece.s < 0) return;
     if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
     const kv4::Span span = piece.span;
-    // the longest rows first
-    const int head = blockIdx.x % a.kv_heads, tile = tiles - 1 - blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
+    const int head = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+    // a sequence's longest rows first
+    const int tile = (a.pieces == 1 ? (span.n * group + R::kRows - 1) / R::kRows : tiles) - 1 - piece.tile;
     const int rows = span.n * group - R::kRows * tile;
     if (rows <= 0) return;
     const int first = span.length - span.n;
@@ -1027,7 +1050,7 @@ void launch(sm_ctx *ctx, Kv4Attention a, const Kv4Shape &s, const T *Q, const ui
     float *parts = (float *)workspace;
     float2 *stats = (float2 *)((char *)workspace + s.part_bytes);
     a.info = s.pieces > 1 ? (int2 *)((char *)workspace + s.part_bytes + s.stat_bytes) : nullptr;
-    const dim3 grid((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots);
+    const dim3 grid = s.pieces > 1 ? dim3((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots) : dim3((uint32_t)(a.kv_heads * s.units));
     if constexpr (Prompt<NC, T>::kThere)
         if (s.prompt) k_kv4_prompt<NC, T><<<grid, Prompt<NC, T>::kThreads, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
     if (!s.prompt) k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);

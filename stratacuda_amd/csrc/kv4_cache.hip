@@ -11,21 +11,50 @@ using namespace smi;
 // keys or of its values; a thread 16 bytes of neighbouring dimensions of some
 // positions, four threads (bf16) or eight a block of 32, so that a wave's loads
 // and stores are without gaps (with 32 bytes a thread f32 values took 147 us
-// where they take 58). Keys' codes lie in memory as the threads have them;
+// where they take 58: 4 sequences of up to 16384 positions, 2 heads of 256
+// dimensions). Keys' codes lie in memory as the threads have them;
 // values' (whose bytes are two dimensions of a position, 16 positions together)
 // pass through LDS on their way, so that both sides are read and written in
 // pieces of 16 bytes. 64 dimensions of one kind a workgroup: enough of them for
-// one token each of 32 sequences, 5 us to write and 4 to read. 8 heads of 128
-// dimensions, 4 x 16384 positions: read into bf16 in 38 us, 3.9 TB/s.
+// one token each of 32 sequences of 8 heads of 128, 5 us to write and 4 to
+// read. The 4 sequences are read into bf16 in 38 us, 3.9 TB/s.
 struct Share {
     int head, part, page;  // `part`: which 64 dimensions; page -1: none
     int lo, hi;            // the page's positions that have rows; none: lo = hi
     int64_t row;           // position 0's
 };
+// run > 0: sequence blockIdx.y, the blockIdx.x % run-th page that its rows
+// touch. run = 0: the pages of all sequences' rows lie in blockIdx.x one after
+// another, and a workgroup looks for its own.
 __device__ __forceinline__ Share share_of(const Kv4Sequences &q, int run, int heads, int pages) {
-    const int s = blockIdx.y, h = blockIdx.x / run, parts = gridDim.z / 2;
-    const kv4::Span a = kv4::span(q, s);
-    const int first = a.length - a.n, at = (first >> 6) + (int)(blockIdx.x % run);  // first may lie before 0
+    int s = blockIdx.y, h, number;
+    kv4::Span a;
+    if (run > 0) {
+        h = blockIdx.x / run, number = blockIdx.x % run;
+        a = kv4::span(q, s);
+    } else {
+        const int unit = blockIdx.x / heads, lane = threadIdx.x % 64;
+        h = blockIdx.x % heads, number = 0, a = {0, 0, 0};
+        for (int at = 0, before = 0; at < q.count; at += 64) {
+            const kv4::Span b = at + lane < q.count ? kv4::span(q, at + lane) : kv4::Span{0, 0, 0};
+            const int mine = b.n > 0 ? ((b.length - 1) >> 6) - ((b.length - b.n) >> 6) + 1 : 0;
+            int upto = mine;
+#pragma unroll
+            for (int i = 1; i < 64; i *= 2) {
+                const int other = __shfl_up(upto, i, 64);
+                if (lane >= i) upto += other;
+            }
+            const uint64_t past = __ballot(before + upto > unit && mine > 0);
+            if (past) {
+                const int who = __ffsll((unsigned long long)past) - 1;
+                const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
+                s = at + who, number = unit - before - (of(upto) - of(mine)), a = {of(b.row), of(b.n), of(b.length)};
+                break;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
+    }
+    const int first = a.length - a.n, at = (first >> 6) + number, parts = gridDim.z / 2;  // first may lie before 0
     if (a.n == 0 || at * 64 >= a.length) return {h, 0, -1, 0, 0, 0};
     return {h, (int)blockIdx.z % parts, kv4::page_of(q, s, at, pages), max(first - at * 64, 0), min(a.length - at * 64, 64),
             (int64_t)a.row + at * 64 - first};
@@ -275,7 +304,20 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkNormRope a, const T *Q, 
     }
 }
 
-int run_of(int longest) { return (longest + 62) / 64 + 1; }  // pages that as many positions can touch
+// A launch's first two dimensions, and the share_of()'s run: each sequence as many pages as the longest one's rows can
+// touch, or, where fewer than half of these can be there, all sequences' together. 255 sequences' single tokens and a prompt
+// of 2048, 8 heads of 128 dimensions, are written in 36 us, and in 135 by the first; where all have as many rows the search
+// costs more (32 single tokens about 1 us).
+struct Pages {
+    int run;
+    uint32_t x, y;
+};
+Pages pages_of(const Kv4Sequences &q, int heads) {
+    const int run = (q.longest + 62) / 64 + 1;
+    const int64_t all = q.tokens / 64 + 2 * (int64_t)q.count;
+    if ((int64_t)run * q.count > 2 * all) return {0, (uint32_t)(all * heads), 1};
+    return {run, (uint32_t)(run * heads), (uint32_t)q.count};
+}
 
 template <typename T, int kLanes>
 void norm_rope(sm_ctx *ctx, const QkNormRope &a, const T *Q, const T *K, T *Yq, T *Yk) {
@@ -301,9 +343,10 @@ namespace smi {
 
 int kv4_write_launch(sm_ctx *ctx, const void *K, const Kv4View &kv, const void *V, const Kv4View &vv, bool bf16,
                      const Kv4Sequences &q, int heads, int dim, uint8_t *pool, int pages) {
-    const int run = run_of(q.longest), pitch = kv4_pitch(dim), per = bf16 ? 8 : 4;
+    const int pitch = kv4_pitch(dim), per = bf16 ? 8 : 4;
+    const auto [run, x, y] = pages_of(q, heads);
     const bool vec = kv.multiple_of(per) && vv.multiple_of(per);
-    const dim3 grid((uint32_t)(run * heads), q.count, 2 * (pitch / 64));
+    const dim3 grid(x, y, 2 * (pitch / 64));
 #define SM_WRITE(T, VEC) \
     k_kv4_write<T, VEC><<<grid, 256, 0, ctx->stream>>>((const T *)K, kv, (const T *)V, vv, q, run, dim, pitch, pool, pages, heads)
     if (bf16 && vec) SM_WRITE(uint16_t, true);
@@ -316,9 +359,10 @@ int kv4_write_launch(sm_ctx *ctx, const void *K, const Kv4View &kv, const void *
 
 int kv4_read_launch(sm_ctx *ctx, const uint8_t *pool, int pages, int heads, int dim, const Kv4Sequences &q, void *K,
                     const Kv4View &kv, void *V, const Kv4View &vv, bool bf16) {
-    const int run = run_of(q.longest), pitch = kv4_pitch(dim), per = bf16 ? 8 : 4;
+    const int pitch = kv4_pitch(dim), per = bf16 ? 8 : 4;
+    const auto [run, x, y] = pages_of(q, heads);
     const bool vec = kv.multiple_of(per) && vv.multiple_of(per);
-    const dim3 grid((uint32_t)(run * heads), q.count, 2 * (pitch / 64));
+    const dim3 grid(x, y, 2 * (pitch / 64));
 #define SM_READ(T, VEC) \
     k_kv4_read<T, VEC><<<grid, 256, 0, ctx->stream>>>(pool, pages, heads, dim, pitch, q, run, (T *)K, kv, (T *)V, vv)
     if (bf16 && vec) SM_READ(uint16_t, true);

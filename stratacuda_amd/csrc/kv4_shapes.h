@@ -33,17 +33,26 @@ constexpr int64_t kKv4PromptTurns = 53 << 10, kKv4PromptTurnsF32 = 140 << 10, kK
 struct Kv4Shape {
     bool prompt;
     int tile_rows, tiles, pieces, least;
+    int64_t units;  // kv4_units
     uint64_t slots, part_bytes, stat_bytes, bytes;
 };
 // The pages that a sequence's rows reach at most.
 inline int64_t kv4_pages(const Kv4Sequences &q, int window) {
     return window > 0 ? std::min<int64_t>(q.table_pages, ((int64_t)window + q.longest) / 64 + 2) : q.table_pages;
 }
+// Tiles of all sequences at most.
+inline int64_t kv4_units(const Kv4Sequences &q, int group, int tile_rows) {
+    const int64_t rows = (int64_t)q.longest * group;
+    return std::min(q.count * ((rows + tile_rows - 1) / tile_rows), (int64_t)q.tokens * group / tile_rows + q.count);
+}
 inline bool kv4_prompt(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16) {
     const int64_t rows = (int64_t)q.longest * (heads / kv_heads);
     const int pitch = kv4_pitch(dim);
     const int64_t reached = std::max<int64_t>(kv4_pages(q, window) - q.longest / 128, 1);  // a row's on average, of the longest sequence's
     const int64_t turns = (int64_t)q.count * kv_heads * ((rows + 15) / 16) * (17 + reached);
+    // a prompt among many single tokens, each of which would take 256 rows (255 tokens over 1000 positions each and 2048 new
+    // ones: 152 us, where 256 rows a tile and as many tiles for each sequence took 1920)
+    if (8 * kv4_units(q, heads / kv_heads, kKv4PromptRows) > kv4_units(q, heads / kv_heads, 16)) return false;
     return (bf16 || pitch <= 128) && rows >= kKv4PromptLeast &&
            turns >= (pitch == 64 ? kKv4PromptTurns64 : bf16 ? kKv4PromptTurns : kKv4PromptTurnsF32);
 }
@@ -56,6 +65,7 @@ inline Kv4Shape kv4_cut(const Kv4Sequences &q, int heads, int kv_heads, int dim,
     s.tile_rows = s.prompt ? kKv4PromptRows : 16;
     s.tiles = (int)((rows + s.tile_rows - 1) / s.tile_rows);
     s.least = kKv4Least;
+    s.units = kv4_units(q, heads / kv_heads, s.tile_rows);
     const int64_t each = (int64_t)kv_heads * s.tiles;
     const int64_t most = pages <= (wide ? kKv4WholeWide : kKv4Whole) ? 1 : (int64_t)q.count * ((q.table_pages + s.least - 1) / s.least);
     // Sixteen rows: a workgroup for each CU, or three for two CUs where registers leave room for three on each (32 sequences
@@ -65,7 +75,9 @@ inline Kv4Shape kv4_cut(const Kv4Sequences &q, int heads, int kv_heads, int dim,
     const int64_t whole = each * q.count;
     int64_t pieces = !s.prompt ? ((wide ? 256 : 384) + each - 1) / each
                      : whole >= 256 ? 1 : (64 * (int64_t)q.table_pages <= 2 * (int64_t)q.longest ? 512 : 256) / whole;
+    // pieces come for every tile of the longest sequence: not where nearly all of these would be empty
     if (pieces > most) pieces = most;
+    if ((int64_t)s.tiles * q.count > 4 * s.units) pieces = 1;
     s.pieces = pieces < 1 ? 1 : (int)pieces;
     s.slots = (uint64_t)(s.pieces > 1 ? s.pieces + q.count : q.count);
     s.part_bytes = s.pieces > 1 ? s.slots * each * s.tile_rows * pitch * 4 : 0;

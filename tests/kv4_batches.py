@@ -6,10 +6,12 @@ the width of the page tables. No counterpart in the reference."""
 WHOLE = dict(sequences=[(70, 200), (130, 300), (1, 129), (33, 33), (3, 3)] + [(0, 9)] * 19, heads=64, kv=1, width=8)
 PIECES = dict(sequences=[(17, 1500), (130, 700), (5, 0), (1, 64), (96, 256), (2, 130)], heads=16, kv=2, width=400)
 # more than 64 pages a workgroup
-LONG = dict(sequences=[(130, 4300)] + [(0, 9)] * 6, heads=64, kv=8, width=70)
+LONG = dict(sequences=[(130, 4300)] + [(0, 9)] * 3, heads=128, kv=8, width=70)
 # 16 rows a workgroup, in pieces: of a row by sixteen waves joined, and by one
 FEW = dict(sequences=[(1, 1500), (3, 700), (2, 0), (1, 64), (1, 1100)], heads=8, kv=2, width=40)
 SOME = dict(sequences=[(20, 1500), (16, 700), (5, 0), (1, 64)], heads=8, kv=2, width=40)
+# a prompt among single tokens
+MIXED = dict(sequences=[(1, 100)] * 20 + [(200, 300)] + [(1, 1000 - 40 * i) for i in range(24)], heads=24, kv=2, width=16)
 LONG_WINDOWS = (70, 300, 1000)
 # more than 64 pages each; more than 128 pieces of a row
 LONG_ROWS = dict(sequences=[(96, 96)] + [(2, 4700)] * 7, heads=8, kv=1, width=74)

@@ -5,13 +5,13 @@
 #include "../stratacuda_amd/csrc/kv4_shapes.h"
 
 extern "C" {
-// {many rows' kernel, tile rows, tiles, pieces, least, slots, workspace bytes}
-void rule_shape(int count, int longest, int table_pages, int heads, int kv_heads, int dim, int window, int bf16, long long *to) {
-    const smi::Kv4Shape s = smi::kv4_shape({count, 1, longest, table_pages, nullptr, nullptr, nullptr}, heads, kv_heads, dim, window, bf16);
+// {many rows' kernel, tile rows, tiles, pieces, least, slots, workspace bytes, units}
+void rule_shape(int count, int tokens, int longest, int table_pages, int heads, int kv_heads, int dim, int window, int bf16, long long *to) {
+    const smi::Kv4Shape s = smi::kv4_shape({count, tokens, longest, table_pages, nullptr, nullptr, nullptr}, heads, kv_heads, dim, window, bf16);
     to[0] = s.prompt, to[1] = s.tile_rows, to[2] = s.tiles, to[3] = s.pieces, to[4] = s.least, to[5] = (long long)s.slots,
-    to[6] = (long long)s.bytes;
+    to[6] = (long long)s.bytes, to[7] = s.units;
 }
-unsigned long long rule_workspace(int count, int longest, int table_pages, int heads, int kv_heads, int dim) {
-    return smi::kv4_workspace({count, 1, longest, table_pages, nullptr, nullptr, nullptr}, heads, kv_heads, dim);
+unsigned long long rule_workspace(int count, int tokens, int longest, int table_pages, int heads, int kv_heads, int dim) {
+    return smi::kv4_workspace({count, tokens, longest, table_pages, nullptr, nullptr, nullptr}, heads, kv_heads, dim);
 }
 }

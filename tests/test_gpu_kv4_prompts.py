@@ -312,6 +312,51 @@ def test_few_rows_in_pieces(be, window, name, dim, type):
     b.free()
 
 
+@pytest.mark.parametrize("type,dim", [("bf16", 128), ("f32", 72)])
+def test_writing_a_prompt_among_single_tokens(be, type, dim):
+    """Rows before position 0, a sequence without positions and one that is none among them; more than 64 sequences."""
+    rng = np.random.default_rng(dim)
+    sequences = [(1, 100)] * 40 + [(500, 530), (3, 2), (4, 0), (0, 7), (1, 129)] + [(1, 1 + i) for i in range(60)]
+    kv = 2
+    b = Batch(be, rng, sequences, kv, dim, extra_rows=2, table_pages=9)
+    assert (500 + 62) // 64 + 1 > 2 * (b.tokens / 64 / len(sequences) + 2)  # pages of all sequences together
+    lengths = b.lengths.copy()
+    lengths[-1] = 9 * 64 + 1
+    be.write(b.seqs.lengths, lengths)
+    k, v = (plain.bf16(rng.normal(0, 1, (b.tokens, kv, dim))) for _ in range(2))
+    K, V = (be.alloc(plain.bits(x, type)) for x in (k, v))
+    want = b.host.copy()
+    back = [np.full(k.shape, 5.0), np.full(k.shape, 5.0)]
+    for s, (n, length) in enumerate(sequences[:-1]):
+        for i in range(n):
+            row, p = b.starts[s] + i, length - n + i
+            for x in back:
+                x[row] = 0
+            if p >= 0:
+                plain.put(want, kv, dim, b.page(s, p), p % 64, k[row].astype(np.float64), v[row].astype(np.float64))
+                back[0][row], back[1][row] = plain.get(want, kv, dim, b.page(s, p), p % 64)
+    be.kv4_write(K, V, b.seqs, b.pool, b.pages, kv, dim, type=type)
+    assert np.array_equal(be.read_bytes(b.pool), want)
+    for buf in (K, V):
+        be.write_bytes(buf, plain.bits(np.full(k.size, 5.0, np.float32), type).view(np.uint8))
+    be.kv4_read(b.pool, b.pages, kv, dim, b.seqs, K, V, type=type)
+    for buf, x in zip((K, V), back):
+        assert np.array_equal(plain.from_bits(be.read_bytes(buf), type)[:k.size].reshape(k.shape), x)
+        be.free(buf)
+    b.free()
+
+
+@pytest.mark.parametrize("type,dim", [("bf16", 128), ("bf16", 256), ("f32", 64), ("f32", 256)])
+def test_a_prompt_among_single_tokens(be, type, dim):
+    rng = np.random.default_rng(dim)
+    which = batches.MIXED
+    b = batch(be, rng, which, dim)
+    q = queries(rng, (b.tokens, which["heads"], dim))
+    scale = dim ** -0.5 / 4
+    check(b, q, run_attention(be, b, q, scale, type), scale, type)
+    b.free()
+
+
 @pytest.mark.parametrize("type", ["f32", "bf16"])
 @pytest.mark.parametrize("name,dim", [("LONG_ROWS", 64), ("LONG_ROWS", 192), ("FAR_ROWS", 64)])
 def test_long_contexts_of_few_rows(be, name, dim, type):
