@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkNormRope a, const T *Q, 
 // A launch's first two dimensions, and the share_of()'s run: each sequence as many pages as the longest one's rows can
 // touch, or, where fewer than half of these can be there, all sequences' together. 255 sequences' single tokens and a prompt
 // of 2048, 8 heads of 128 dimensions, are written in 36 us, and in 135 by the first; where all have as many rows the search
-// costs more (32 single tokens about 1 us).
+// costs more (4 sequences of up to 16384 positions read in 44 us, in 38 without it).
 struct Pages {
     int run;
     uint32_t x, y;
