@@ -348,8 +348,8 @@ int sm_f8_gate_up(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int co
  * page number outside [0, pages) stands for positions that are not there, and
  * a row before a sequence's position 0 has none. Rows of no sequence stay as
  * they were. Tables that give two written positions the same place leave
- * either's bytes there, or a mixture, and so do starts that go back in an
- * output row of the sequences around them.
+ * either's bytes there, or a mixture. Starts that go back leave either's
+ * result, a mixture or what was there in rows of the sequences around them.
  *
  * Types are SM_TYPE_F32 or SM_TYPE_BF16, one for all tensors of a call. dim is
  * a multiple of 8 from 8 to 256. A view is {stride, head, offset}: row t, head

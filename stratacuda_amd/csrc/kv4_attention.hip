@@ -229,8 +229,7 @@ __device__ __forceinline__ void four(uint32_t w, uint32_t scales, uint32_t low[2
 
 template <int NC, typename T>
 __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd)) k_kv4_rows(Kv4Attention a, const T *Q, const uint8_t *pool,
-                                                                                            const T *G, T *Y, float *parts, float2 *stats,
-                                                                                            int tiles) {
+                                                                                            const T *G, T *Y, float *parts, float2 *stats) {
     constexpr bool F32 = sizeof(T) == 4;
     using R = Rows16<NC, F32>;
     constexpr int kPitch = R::kPitch, kTiles = kPitch / 16, kLine = kPitch + 4;
@@ -1053,7 +1052,7 @@ void launch(sm_ctx *ctx, Kv4Attention a, const Kv4Shape &s, const T *Q, const ui
     const dim3 grid = s.pieces > 1 ? dim3((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots) : dim3((uint32_t)(a.kv_heads * s.units));
     if constexpr (Prompt<NC, T>::kThere)
         if (s.prompt) k_kv4_prompt<NC, T><<<grid, Prompt<NC, T>::kThreads, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
-    if (!s.prompt) k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
+    if (!s.prompt) k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats);
     if (s.pieces == 1) return;
     const uint32_t all = (uint32_t)a.q.longest * a.heads;
     if ((int64_t)all * a.q.count < kKv4JoinRows)
