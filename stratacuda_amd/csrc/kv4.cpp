@@ -200,7 +200,8 @@ int sm_kv4_attention(sm_ctx *ctx, uint64_t Q, const int64_t *q_view, int type, i
     if (!(scale > 0.0f && scale < 1e30f)) return bad(ctx, what, "scale must be > 0 and below 1e30");
     if (window < 0) return bad(ctx, what, "window must be >= 0");
     Kv4Attention a = {{count, tokens, longest, table_pages, (const int *)starts, (const int *)lengths, (const int *)table},
-                      pages, heads, kv_heads, dim, window, scale * 1.44269504088896340736f, {}, {}, false, 0, 0, nullptr};
+                      pages, heads, kv_heads, dim, kv4_window(window, table_pages), scale * 1.44269504088896340736f,
+                      {}, {}, false, 0, 0, nullptr};
     if (int rc = take_view(ctx, what, q_view, tokens, heads, dim, type, false, &a.q_view, &q_bytes)) return rc;
     if (int rc = take_view(ctx, what, G ? g_view : nullptr, tokens, heads, dim, type, false, &a.g_view, &g_bytes)) return rc;
     a.vec = a.q_view.multiple_of(8);

@@ -36,6 +36,9 @@ struct Kv4Shape {
     int64_t units;  // kv4_units
     uint64_t slots, part_bytes, stat_bytes, bytes;
 };
+// A window past every position of the tables is none (0). Any other is below 2^30 and a row's position above -2^24, so that
+// the kernels' differences of the two stay within 32 bits.
+inline int kv4_window(int window, int table_pages) { return window >= 64 * (int64_t)table_pages ? 0 : window; }
 // The pages that a sequence's rows reach at most.
 inline int64_t kv4_pages(const Kv4Sequences &q, int window) {
     return window > 0 ? std::min<int64_t>(q.table_pages, ((int64_t)window + q.longest) / 64 + 2) : q.table_pages;
