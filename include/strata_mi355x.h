@@ -354,8 +354,10 @@ int sm_f8_gate_up(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int co
  * Types are SM_TYPE_F32 or SM_TYPE_BF16, one for all tensors of a call. dim is
  * a multiple of 8 from 8 to 256. A view is {stride, head, offset}: row t, head
  * h, dimension d lies at t * stride + h * head + offset + d, in values; all
- * three are >= 0, rows of an output do not overlap; 0 (no view): rows of
- * heads of dim values. Outputs must not be buffers that the call reads.
+ * three are from 0 to 2^40; 0 (no view): rows of heads of dim values. An
+ * output's rows lie one after another, each with all its heads, or its heads
+ * do, each with all its rows. Outputs are buffers that the call does not read,
+ * and each another one.
  * count is at most 2^15; count * table_pages, tokens * heads and pages at most
  * 2^24.
  * Nothing is allocated and nothing waits: every entry may be captured. */

@@ -33,8 +33,10 @@ int take_view(sm_ctx *ctx, const char *what, const int64_t *v, int tokens, int h
     for (int64_t n : {view->stride, view->head, view->offset})
         if (n < 0 || n > kMaxPlace) return bad(ctx, what, "a view's numbers must be 0 to 2^40");
     if (view->stride > kMaxPlace / tokens || view->head > kMaxPlace / heads) return bad(ctx, what, "a view reaches past 2^40 values");
-    if (apart && ((heads > 1 && view->head < dim) || (tokens > 1 && view->stride < (heads - 1) * view->head + dim)))
-        return bad(ctx, what, "an output's rows overlap");
+    // one after another, rows with their heads or heads with their rows
+    const bool rows = (heads == 1 || view->head >= dim) && (tokens == 1 || view->stride >= (heads - 1) * view->head + dim);
+    const bool by_head = (tokens == 1 || view->stride >= dim) && (heads == 1 || view->head >= (tokens - 1) * view->stride + dim);
+    if (apart && !rows && !by_head) return bad(ctx, what, "an output's rows overlap");
     *bytes = (uint64_t)((tokens - 1) * view->stride + (heads - 1) * view->head + view->offset + dim) * (type == SM_TYPE_BF16 ? 2 : 4);
     return SM_OK;
 }

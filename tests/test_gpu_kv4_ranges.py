@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import kv4_batches as batches
+import kv4_plain as plain
 from kv4_compare import expect
 from test_gpu_kv4 import Batch, queries, run_attention
 
@@ -58,4 +59,25 @@ def test_a_window_and_rows_before_position_0(be, window, name, type, dim):
     q = queries(rng, (b.tokens, which["heads"], dim))
     scale = dim ** -0.5 / 4
     expect(b, q, run_attention(be, b, q, scale, type, window=window), scale, type, window=window)
+    b.free()
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+def test_read_heads_first(be, type):
+    """Keys and values as an array of heads has them, each head's rows together."""
+    rng = np.random.default_rng(3)
+    kv, dim = 3, 72
+    b = Batch(be, rng, [(70, 130), (5, 3), (1, 64)], kv, dim, extra_rows=1)
+    n = b.tokens
+    K, V = (be.alloc(plain.bits(np.full(n * kv * dim + 8, 7, np.float32), type)) for _ in range(2))
+    be.kv4_read(b.pool, b.pages, kv, dim, b.seqs, K, V, k_view=(dim, n * dim, 8), v_view=(dim, n * dim, 0), type=type)
+    for buf, which, offset in ((K, 0, 8), (V, 1, 0)):
+        got = plain.from_bits(be.read_bytes(buf), type)[offset:offset + n * kv * dim].reshape(kv, n, dim)
+        for s, (rows, length) in enumerate(b.sequences):
+            for i in range(rows):
+                p = length - rows + i
+                want = plain.get(b.host, kv, dim, b.page(s, p), p % 64)[which] if p >= 0 else np.zeros((kv, dim))
+                assert np.array_equal(got[:, b.starts[s] + i], want), (s, i)
+        assert np.all(got[:, b.rows:] == 7)
+        be.free(buf)
     b.free()
