@@ -397,9 +397,11 @@ int sm_kv4_read(sm_ctx *ctx, uint64_t pool, int pages, int kv_heads, int dim, in
  * kv_heads; key-value head h serves the heads from h * heads / kv_heads on.
  * scale is finite and > 0. Rows that have no position, or only scores of
  * -infinity, are 0. What positions outside a row's range hold does not count,
- * whatever it is. Sums and the softmax are in f32, and scores have to lie in
- * its range. For f32 tensors nothing is rounded to fewer bits. For bf16 ones
- * the probabilities are rounded to bf16 (2^-8 each), and in calls of many rows
+ * whatever it is. Sums and the softmax are in f32. Scores, before and after the
+ * scale, have to lie below 2^126 in magnitude, f32 queries below 2^127; weights
+ * are up to 2^8 until their sum divides them, so values times the number of
+ * positions below 2^119. For f32 tensors nothing is rounded to fewer bits. For
+ * bf16 ones the probabilities are rounded to bf16 (2^-8 each), and in calls of many rows
  * (from 1024 of a key-value head) the queries are taken as two 8-bit numbers
  * each, off by 2^-22 of the row's largest at most, whose products with the
  * codes may lose 7 * 2^-13 of their magnitudes in a score (1e-5 of it, usually).

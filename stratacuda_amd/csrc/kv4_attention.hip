@@ -48,6 +48,22 @@ __device__ __forceinline__ uint32_t here(uint32_t v) {
     return v;
 }
 
+// Exponents past 2^30. A row's maximum is a rounded product there, off by 2^6 and more from its own scores' exact ones: the
+// difference could leave f32 where there is none. So these rows take their scores times the power of two at or above the
+// scale: exact, and numbers that differ do so by 2^6 at least, in powers of two, of which nothing is left in f32. A score of
+// the maximum counts 1, any other 0.
+constexpr float kFar = 0x1p30f;
+__device__ __forceinline__ float far_scale(float scale_log2) {
+    return __uint_as_float((__float_as_uint(scale_log2) + 0x7fffffu) & 0x7f800000u);
+}
+// Whether one of the exponents is far, or -infinity: no score.
+__device__ __forceinline__ bool special(float a, float b) { return fmaxf(fabsf(a), fabsf(b)) >= kFar; }
+// The score of a row with such a maximum m: what e to the power of it is, 1 or 0; NaN stays.
+__device__ __forceinline__ float far_score(float s, float scale, float m) {
+    const float d = m == kNone ? s : fmaf(s, scale, -m);
+    return d < 0.0f ? kNone : d;
+}
+
 // The larger of a lane's value and those of the lanes 16, 32 and 48 away.
 __device__ __forceinline__ float max_of_quarters(float v) {
     const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -354,21 +370,30 @@ __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd
         for (int g = 0; g < 4; g++)
 #pragma unroll
             for (int i = 0; i < 4; i++) top = fmaxf(top, s[g][i]);
-        top = max_of_quarters(top) * a.scale_log2;
+        const float best = max_of_quarters(top);
+        top = best * a.scale_log2;
+        float from = m;
         // the maximum is raised once scores pass it by 2^8: any number near it does
-        if (__any(top > m + 8.0f || (m == kNone && top > kNone))) {
-            const float to = fmaxf(m, top), by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
-            m = to;
+        if (__any(top > m + 8.0f || special(top, m))) {
+            if (fabsf(top) >= kFar) top = best * far_scale(a.scale_log2);
+            const float to = top > m + 8.0f ? top : m, by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            m = from = to;
             sum *= by;
 #pragma unroll
             for (int t = 0; t < kTiles; t++) o[t] *= by;
+            if (special(m, 0.0f)) {
+                from = 0.0f;
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[g][i] = far_score(s[g][i], far_scale(a.scale_log2), m);
+            }
         }
-        const float from = m == kNone ? 0.0f : -m;
 #pragma unroll
         for (int g = 0; g < 4; g++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], a.scale_log2, from));
+                s[g][i] = __builtin_amdgcn_exp2f(fmaf(s[g][i], a.scale_log2, -from));
                 sum += s[g][i];
             }
         uint32_t poison = 0;  // bit b: a block b of NaN at a position that the row has
@@ -826,23 +851,32 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
         for (int h = 0; h < kHalves; h++)
 #pragma unroll
             for (int i = 0; i < 16; i++) top = fmaxf(top, s[h][i]);
-        top = max_of_halves(top) * a.scale_log2;
+        const float best = max_of_halves(top);
+        top = best * a.scale_log2;
+        float from = m;
         // the maximum is raised once scores pass it by 2^8: any number near it does
-        if (__any(top > m + 8.0f || (m == kNone && top > kNone))) {
-            const float to = fmaxf(m, top), by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
-            m = to;
+        if (__any(top > m + 8.0f || special(top, m))) {
+            if (fabsf(top) >= kFar) top = best * far_scale(a.scale_log2);
+            const float to = top > m + 8.0f ? top : m, by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            m = from = to;
             sum *= by;
 #pragma unroll
             for (int b = 0; b < kBlocks; b++) o[b] *= by;
+            if (special(m, 0.0f)) {
+                from = 0.0f;
+#pragma unroll
+                for (int h = 0; h < kHalves; h++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[h][i] = far_score(s[h][i], far_scale(a.scale_log2), m);
+            }
         }
-        const float from = m == kNone ? 0.0f : -m;
         float sums[2] = {sum, 0.0f};
 #pragma unroll
         for (int h = 0; h < kHalves; h++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[h][2 * j], a.scale_log2, from));
-                const float y = __builtin_amdgcn_exp2f(fmaf(s[h][2 * j + 1], a.scale_log2, from));
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[h][2 * j], a.scale_log2, -from));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[h][2 * j + 1], a.scale_log2, -from));
                 sums[j % 2] += x;
                 sums[j % 2] += y;
                 if constexpr (R::kF32) {
