@@ -312,6 +312,8 @@ struct Kv4Attention {
     // each sequence which is its first and how many they are
     int pieces, least;
     int2 *info;
+    // or, where rows differ: into how many pieces all tiles' pages, and for how many tiles (0: not so)
+    int budget, units;
 };
 // Unchecked launchers on raw device pointers (kv4_cache.hip, kv4_attention.hip).
 int qk_norm_rope_launch(sm_ctx *ctx, const QkNormRope &a, const void *Q, const void *K, void *Yq, void *Yk, bool bf16);

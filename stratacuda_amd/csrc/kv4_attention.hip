@@ -102,6 +102,7 @@ struct Piece {
     int number, count;  // which of the sequence's pieces it is
     int tile;           // of the sequence's rows
     kv4::Span span;
+    int at;             // where the piece's results go: the place of its first tile's first head
 };
 // The pages that the sequence's rows reach.
 __device__ __forceinline__ int2 pages_of(const kv4::Span &a, int window) {
@@ -152,12 +153,67 @@ __device__ Piece piece_of(const Kv4Attention &a) {
             const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
             const int count = of(mine), number = slot - before - (of(upto) - count), first = of(p.x), end = of(p.y);
             const kv4::Span span = {of(b.row), of(b.n), of(b.length)};
-            if (whole) return {at + who, first, end, 0, 1, number, span};
-            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count, at_x, span};
+            if (whole) return {at + who, first, end, 0, 1, number, span, 0};
+            return {at + who, first + number * each, min(first + (number + 1) * each, end), number, count, at_x, span, (int)(blockIdx.y * gridDim.x)};
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
-    return {-1, 0, 0, 0, 0, 0, {0, 0, 0}};
+    return {-1, 0, 0, 0, 0, 0, {0, 0, 0}, 0};
+}
+// The same where rows differ and contexts are long: tiles and pieces of all sequences in blockIdx.x, a sequence's pieces one
+// after another, in each all its tiles. Pieces are of equally many pages, so many that all tiles' pages make a.budget pieces
+// and each tile's last one a part of one more. Where starts that go back make more tiles than the launch was sized for, no
+// sequence is cut, and nothing is left in the workspace. Block 0 says where each sequence's pieces begin.
+template <int kTileRows>
+__device__ Piece piece_by_rows(const Kv4Attention &a) {
+    const Kv4Sequences &q = a.q;
+    const int lane = threadIdx.x % 64, slot = blockIdx.x / a.kv_heads, group = a.heads / a.kv_heads;
+    const auto sequence = [&](int s) { return s < q.count ? kv4::span(q, s) : kv4::Span{0, 0, 0}; };
+    const auto tiles_of = [&](const kv4::Span &b) { return (b.n * group + kTileRows - 1) / kTileRows; };
+    int64_t pages = 0;
+    int tiles = 0;
+    for (int at = 0; at < q.count; at += 64) {
+        const kv4::Span b = sequence(at + lane);
+        const int2 p = pages_of(b, a.window);
+        pages += (int64_t)tiles_of(b) * (p.y - p.x), tiles += tiles_of(b);
+    }
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) pages += __shfl_xor(pages, i, 64), tiles += __shfl_xor(tiles, i, 64);
+    int each = kv4::kMostPages;
+    if (tiles <= a.units) each = (int)min(max((pages + a.budget - 1) / a.budget, (int64_t)a.least), (int64_t)kv4::kMostPages);
+    each = __builtin_amdgcn_readfirstlane(each);
+    Piece found = {-1, 0, 0, 0, 0, 0, {0, 0, 0}, 0};
+    for (int at = 0, before = 0; at < q.count; at += 64) {
+        const kv4::Span b = sequence(at + lane);
+        const int2 p = pages_of(b, a.window);
+        const int many = pieces_in(p, b.n, each), mine = many * tiles_of(b);
+        int upto = mine;
+#pragma unroll
+        for (int i = 1; i < 64; i *= 2) {
+            const int other = __shfl_up(upto, i, 64);
+            if (lane >= i) upto += other;
+        }
+        if (blockIdx.x == 0 && threadIdx.x < 64 && at + lane < q.count) a.info[at + lane] = make_int2(before + upto - mine, many);
+        const uint64_t past = __ballot(before + upto > slot && mine > 0);
+        if (past && found.s < 0) {
+            const int who = __ffsll((unsigned long long)past) - 1;
+            const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, who); };
+            const kv4::Span span = {of(b.row), of(b.n), of(b.length)};
+            const int step = tiles_of(span), local = slot - before - (of(upto) - of(mine)), number = local / step, first = of(p.x);
+            found = {at + who, first + number * each, min(first + (number + 1) * each, of(p.y)), number, of(many), local - number * step,
+                     span, (slot - (local - number * step)) * a.kv_heads};
+            if (blockIdx.x > 0) break;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return found;
+}
+
+// Either by the kernel's type: the second beside the first would cost one token over 2048 positions 0.5 us of 16.7.
+template <int kTileRows, int kTurn, bool kByRows>
+__device__ __forceinline__ Piece share(const Kv4Attention &a) {
+    if constexpr (kByRows) return piece_by_rows<kTileRows>(a);
+    else return piece_of<kTileRows, kTurn>(a);
 }
 
 // ------------------------------------------------------------------ 16 rows
@@ -243,7 +299,7 @@ __device__ __forceinline__ void four(uint32_t w, uint32_t scales, uint32_t low[2
     high[0] = __builtin_amdgcn_perm(b, a, 0x07060302u), high[1] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
-template <int NC, typename T>
+template <int NC, typename T, bool kByRows>
 __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd)) k_kv4_rows(Kv4Attention a, const T *Q, const uint8_t *pool,
                                                                                             const T *G, T *Y, float *parts, float2 *stats) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -251,7 +307,7 @@ __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd
     constexpr int kPitch = R::kPitch, kTiles = kPitch / 16, kLine = kPitch + 4;
     const uint32_t lane = threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const Piece piece = piece_of<16, 4>(a);
+    const Piece piece = share<16, 4, kByRows>(a);
     if (piece.s < 0) return;
     if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
     const kv4::Span span = piece.span;
@@ -480,7 +536,7 @@ __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd
         // a sum that is not a number, of scores that are none, stays one
         all += s_m[w][r] == kNone ? (s_sum[w][r] == 0.0f ? 0.0f : NAN) : s_sum[w][r] * by[w];
     }
-    const int64_t part = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 16 + r;
+    const int64_t part = (int64_t)(piece.at + tile * a.kv_heads + head) * 16 + r;
     const int tok = (16 * tile + r) / group, h = head * group + (16 * tile + r) % group;
     const int64_t out = ((int64_t)(span.row + tok) * a.heads + h) * a.dim;
     const T *g = G ? G + (int64_t)(span.row + tok) * a.g_view.stride + h * a.g_view.head + a.g_view.offset : nullptr;
@@ -552,7 +608,7 @@ struct Prompt {
     }
 };
 
-template <int NC, typename T>
+template <int NC, typename T, bool kByRows>
 __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Attention a, const T *Q, const uint8_t *pool, const T *G,
                                                                           T *Y, float *parts, float2 *stats, int tiles) {
     using R = Prompt<NC, T>;
@@ -564,7 +620,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
     __shared__ uint64_t s_nan[4][kBlocks];         // values that are NaN for some rows and not there for others
     const uint32_t lane = threadIdx.x % 64;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const Piece piece = piece_of<R::kRows, 1>(a);
+    const Piece piece = share<R::kRows, 1, kByRows>(a);
     if (piece.s < 0) return;
     if (a.info && piece.number == 0 && blockIdx.x == 0 && threadIdx.x == 0) a.info[piece.s] = make_int2(blockIdx.y, piece.count);
     const kv4::Span span = piece.span;
@@ -966,7 +1022,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
     if (32 * wave + (int)(lane % 32) >= rows) return;
     const int kq = lane / 32;
     sum = sum_of_halves(sum);
-    const int64_t part = ((int64_t)blockIdx.y * gridDim.x + tile * a.kv_heads + head) * R::kRows + 32 * wave + lane % 32;
+    const int64_t part = (int64_t)(piece.at + tile * a.kv_heads + head) * R::kRows + 32 * wave + lane % 32;
     const int64_t out = ((int64_t)(span.row + token) * a.heads + hq) * a.dim;
     const T *g = G ? G + (int64_t)(span.row + token) * a.g_view.stride + hq * a.g_view.head + a.g_view.offset : nullptr;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -998,7 +1054,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
 template <int NC, typename T, int kWaves>
 __global__ void __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) k_kv4_join(Kv4Attention a, const T *G, T *Y, const float *parts,
                                                                               const float2 *stats, const int2 *info, int tiles,
-                                                                              int tile_rows) {
+                                                                              int row_bits) {
     constexpr int kPitch = 64 * NC, kSome = 8;
     const int s = blockIdx.y, group = a.heads / a.kv_heads;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -1008,9 +1064,12 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) k_kv4_join(Kv
     if (token >= span.n) return;
     const int2 pieces = info[s];  // the first, how many
     if (pieces.y <= 1) return;
-    const int head = h / group, row = token * group + h % group;
-    const int64_t step = (int64_t)a.kv_heads * tiles * tile_rows;
-    const int64_t base = ((int64_t)row / tile_rows * a.kv_heads + head) * tile_rows + row % tile_rows + pieces.x * step;
+    const int head = h / group, row = token * group + h % group, tile = row >> row_bits;
+    // tiles from a piece to the next: as many for all sequences, or (0) the sequence's own, and the first piece's tile is named
+    int apart = tiles, first = pieces.x * tiles;
+    if (tiles == 0) apart = (span.n * group + (1 << row_bits) - 1) >> row_bits, first = pieces.x;
+    const int64_t step = (int64_t)a.kv_heads * apart << row_bits;
+    const int64_t base = ((int64_t)((first + tile) * a.kv_heads + head) << row_bits) + row - (tile << row_bits);
     float top = kNone, all = 0.0f, v[NC] = {};
     const int share = (pieces.y + kWaves - 1) / kWaves, from = kWaves == 1 ? 0 : wave * share, end = min(from + share, pieces.y);
     for (int c0 = from; c0 < end; c0 += kSome) {
@@ -1079,20 +1138,29 @@ __global__ void __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) k_kv4_join(Kv
 
 template <int NC, typename T>
 void launch(sm_ctx *ctx, Kv4Attention a, const Kv4Shape &s, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {
-    a.pieces = s.pieces, a.least = s.least;
+    a.pieces = s.pieces, a.least = s.budget > 0 ? kKv4FarLeast : s.least, a.budget = s.budget, a.units = (int)s.units;
     float *parts = (float *)workspace;
     float2 *stats = (float2 *)((char *)workspace + s.part_bytes);
-    a.info = s.pieces > 1 ? (int2 *)((char *)workspace + s.part_bytes + s.stat_bytes) : nullptr;
-    const dim3 grid = s.pieces > 1 ? dim3((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots) : dim3((uint32_t)(a.kv_heads * s.units));
-    if constexpr (Prompt<NC, T>::kThere)
-        if (s.prompt) k_kv4_prompt<NC, T><<<grid, Prompt<NC, T>::kThreads, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
-    if (!s.prompt) k_kv4_rows<NC, T><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats);
-    if (s.pieces == 1) return;
+    const bool cut = s.pieces > 1 || s.budget > 0;
+    a.info = cut ? (int2 *)((char *)workspace + s.part_bytes + s.stat_bytes) : nullptr;
+    const dim3 grid = s.pieces > 1 ? dim3((uint32_t)(a.kv_heads * s.tiles), (uint32_t)s.slots)
+                                   : dim3((uint32_t)(a.kv_heads * (s.units + s.budget)));
+    const auto run = [&](auto by_rows) {
+        if constexpr (Prompt<NC, T>::kThere)
+            if (s.prompt)
+                k_kv4_prompt<NC, T, by_rows><<<grid, Prompt<NC, T>::kThreads, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats, s.tiles);
+        if (!s.prompt) k_kv4_rows<NC, T, by_rows><<<grid, 256, 0, ctx->stream>>>(a, Q, pool, G, Y, parts, stats);
+    };
+    if (s.budget > 0) run(std::true_type());
+    else run(std::false_type());
+    if (!cut) return;
+    const int tiles = s.budget > 0 ? 0 : s.tiles, row_bits = s.prompt ? 8 : 4;
+    static_assert(kKv4PromptRows == 1 << 8, "a tile's rows");
     const uint32_t all = (uint32_t)a.q.longest * a.heads;
     if ((int64_t)all * a.q.count < kKv4JoinRows)
-        k_kv4_join<NC, T, 16><<<dim3(all, a.q.count), 1024, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
+        k_kv4_join<NC, T, 16><<<dim3(all, a.q.count), 1024, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, tiles, row_bits);
     else
-        k_kv4_join<NC, T, 1><<<dim3((all + 3) / 4, a.q.count), 256, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, s.tiles, s.tile_rows);
+        k_kv4_join<NC, T, 1><<<dim3((all + 3) / 4, a.q.count), 256, 0, ctx->stream>>>(a, G, Y, parts, stats, a.info, tiles, row_bits);
 }
 template <typename T>
 void launch(sm_ctx *ctx, const Kv4Attention &a, const T *Q, const uint8_t *pool, const T *G, T *Y, void *workspace) {

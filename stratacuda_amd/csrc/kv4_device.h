@@ -16,6 +16,7 @@ using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 
 constexpr int kPage = SM_KV4_PAGE;
+constexpr int kMostPages = 1 << 24;  // of a sequence
 
 // Byte offsets of a tile's parts.
 __device__ __forceinline__ int value_codes(int pitch) { return 32 * pitch; }

@@ -30,11 +30,26 @@ constexpr int kKv4PromptRows = 256;
 constexpr int kKv4PromptLeast = 1024;
 constexpr int64_t kKv4PromptTurns = 53 << 10, kKv4PromptTurnsF32 = 140 << 10, kKv4PromptTurns64 = 220 << 10;
 
+// Sequences whose rows differ (a prompt or some tokens among single ones), so that they have two thirds or less of the tiles
+// which as many of the longest one's would make, are cut by rows: equal pieces of all tiles' pages. In tables of so many
+// pages, and where their tiles leave CUs idle; 256 rows a workgroup from the larger number on where the rule for equal
+// sequences makes three pieces or more. Pieces of at least kKv4FarLeast pages. In us, by that rule and by rows, 24 heads on 2
+// of dimension 256, bf16: 512 tokens and one over 32768 positions each 1376 and 393 (two of 16384: 703 and 220, of 8192: 370
+// and 134), 64 tokens and four single ones over 131072 positions 1221 and 77, 96 tokens and 8 over 9000 91 and 28, 8, 5, 3
+// and 1 tokens over 32768 and fewer 71 and 54 (f32 64 and 54). Where the tiles are fewer by less: 2 tokens and 7 single ones
+// over 1000 positions in a table for 8200 20.7 and 30.8. Least 8, 16 and 32: 96 tokens and 8 27, 28 and 33; 16 tokens and
+// 3 over 8192, 32 heads on 8 of 128 in f32, 32, 32 and 27.
+constexpr int kKv4Far = 512, kKv4FarRows = 128, kKv4FarLeast = 16;
+
 struct Kv4Shape {
     bool prompt;
-    int tile_rows, tiles, pieces, least;
-    int64_t units;  // kv4_units
-    uint64_t slots, part_bytes, stat_bytes, bytes;
+    int tile_rows, tiles;
+    int64_t units;      // kv4_units
+    // pieces of all sequences' pages, of at least so many, for each of the longest one's tiles; 1: none is cut
+    int pieces, least;
+    uint64_t slots, bytes;
+    int budget;         // or, where none is: pieces of all tiles' pages, for each sequence's own tiles; 0: no
+    uint64_t part_bytes, stat_bytes, workspace;
 };
 // A window past every position of the tables is none (0). Any other is below 2^30 and a row's position above -2^24, so that
 // the kernels' differences of the two stay within 32 bits.
@@ -59,7 +74,8 @@ inline bool kv4_prompt(const Kv4Sequences &q, int heads, int kv_heads, int dim, 
     return (bf16 || pitch <= 128) && rows >= kKv4PromptLeast &&
            turns >= (pitch == 64 ? kKv4PromptTurns64 : bf16 ? kKv4PromptTurns : kKv4PromptTurnsF32);
 }
-inline Kv4Shape kv4_cut(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16, bool prompt) {
+inline Kv4Shape kv4_cut(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16, bool prompt,
+                        bool by_rows = true) {
     Kv4Shape s;
     const int64_t rows = (int64_t)q.longest * (heads / kv_heads), pages = kv4_pages(q, window);
     const int pitch = kv4_pitch(dim);
@@ -78,27 +94,37 @@ inline Kv4Shape kv4_cut(const Kv4Sequences &q, int heads, int kv_heads, int dim,
     const int64_t whole = each * q.count;
     int64_t pieces = !s.prompt ? ((wide ? 256 : 384) + each - 1) / each
                      : whole >= 256 ? 1 : (64 * (int64_t)q.table_pages <= 2 * (int64_t)q.longest ? 512 : 256) / whole;
-    // pieces come for every tile of the longest sequence: not where nearly all of these would be empty
     if (pieces > most) pieces = most;
-    if ((int64_t)s.tiles * q.count > 4 * s.units) pieces = 1;
+    // By rows: where one workgroup fills a CU, as many as one round holds, each tile's last pieces with them; else those besides.
+    const bool alone = s.prompt || (!bf16 && pitch > 128);  // one workgroup a CU
+    const int64_t fill = (!s.prompt && !wide ? 384 : 256) / kv_heads, budget = alone ? fill - s.units : fill;
+    const bool far = pages >= (s.prompt && pieces > 2 ? kKv4Far : kKv4FarRows);
+    s.budget = by_rows && far && 3 * s.units <= 2 * (int64_t)s.tiles * q.count && budget >= s.units ? (int)budget : 0;
+    // pieces come for every tile of the longest sequence: not where nearly all of these would be empty
+    if (s.budget || (int64_t)s.tiles * q.count > 4 * s.units) pieces = 1;
     s.pieces = pieces < 1 ? 1 : (int)pieces;
     s.slots = (uint64_t)(s.pieces > 1 ? s.pieces + q.count : q.count);
-    s.part_bytes = s.pieces > 1 ? s.slots * each * s.tile_rows * pitch * 4 : 0;
-    s.stat_bytes = s.pieces > 1 ? s.slots * each * s.tile_rows * 8 : 0;
-    s.bytes = s.part_bytes + s.stat_bytes + (s.pieces > 1 ? (uint64_t)q.count * 8 : 0);
-    if (s.pieces == 1) s.least = q.table_pages + 1;  // one piece a sequence: as large as any
+    const uint64_t held = s.budget ? (uint64_t)kv_heads * (s.units + s.budget) : s.pieces > 1 ? s.slots * each : 0;
+    s.part_bytes = held * s.tile_rows * pitch * 4;
+    s.stat_bytes = held * s.tile_rows * 8;
+    s.workspace = held ? s.part_bytes + s.stat_bytes + (uint64_t)q.count * 8 : 0;
+    s.bytes = s.pieces > 1 ? s.workspace : 0;
+    if (s.pieces == 1) s.least = q.table_pages + 1;
     return s;
 }
 inline Kv4Shape kv4_shape(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16) {
     return kv4_cut(q, heads, kv_heads, dim, window, bf16, kv4_prompt(q, heads, kv_heads, dim, window, bf16));
 }
 
-// Enough for either type and every window: the narrowest and none tell which kernels it may be, and none has the most pieces.
+// Enough for either type and every window: the narrowest and none tell which kernels it may be, and none has the most pieces,
+// or those by rows in their place.
 inline uint64_t kv4_workspace(const Kv4Sequences &q, int heads, int kv_heads, int dim) {
     uint64_t most = 0;
     for (int bf16 = 0; bf16 < 2; bf16++)
-        for (int window = 0; window < 2; window++)
-            most = std::max(most, kv4_cut(q, heads, kv_heads, dim, 0, bf16, kv4_prompt(q, heads, kv_heads, dim, window, bf16)).bytes);
+        for (int window = 0; window < 2; window++) {
+            const bool prompt = kv4_prompt(q, heads, kv_heads, dim, window, bf16);
+            for (const bool by_rows : {false, true}) most = std::max(most, kv4_cut(q, heads, kv_heads, dim, 0, bf16, prompt, by_rows).workspace);
+        }
     return most;
 }
 

@@ -20,3 +20,7 @@ FAR_ROWS = dict(sequences=[(1, 520 * 64 - 5)], heads=4, kv=1, width=520)
 TYPES = [("bf16", 64), ("bf16", 40), ("bf16", 128), ("bf16", 72), ("bf16", 192), ("bf16", 256), ("bf16", 200), ("f32", 64), ("f32", 24),
          ("f32", 128), ("f32", 104)]  # those that have the many rows' kernel
 WINDOWS = (1, 63, 64, 65, 100)
+
+# sequences' rows differ, in tables of long contexts: each sequence's own tiles cut, of 16 rows and of 256
+UNLIKE = dict(sequences=[(1, 1500), (60, 2900), (0, 9), (1, 64), (5, 0), (1, 6500), (7, 4)], heads=12, kv=2, width=200)
+UNLIKE_PROMPT = dict(sequences=[(1, 5000), (130, 3000), (0, 9), (17, 2200), (20, 7)], heads=32, kv=2, width=600)
