@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd
         // the maximum is raised once scores pass it by 2^8: any number near it does
         if (__any(top > m + 8.0f || special(top, m))) {
             if (fabsf(top) >= kFar) top = best * far_scale(a.scale_log2);
-            const float to = top > m + 8.0f ? top : m, by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            const float to = __any(top > m + 8.0f) ? fmaxf(m, top) : m, by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
             m = from = to;
             sum *= by;
 #pragma unroll
@@ -913,7 +913,7 @@ __global__ void __launch_bounds__((Prompt<NC, T>::kThreads)) k_kv4_prompt(Kv4Att
         // the maximum is raised once scores pass it by 2^8: any number near it does
         if (__any(top > m + 8.0f || special(top, m))) {
             if (fabsf(top) >= kFar) top = best * far_scale(a.scale_log2);
-            const float to = top > m + 8.0f ? top : m, by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
+            const float to = __any(top > m + 8.0f) ? fmaxf(m, top) : m, by = m == kNone ? 0.0f : __builtin_amdgcn_exp2f(m - to);
             m = from = to;
             sum *= by;
 #pragma unroll

@@ -109,7 +109,7 @@ inline Kv4Shape kv4_cut(const Kv4Sequences &q, int heads, int kv_heads, int dim,
     s.stat_bytes = held * s.tile_rows * 8;
     s.workspace = held ? s.part_bytes + s.stat_bytes + (uint64_t)q.count * 8 : 0;
     s.bytes = s.pieces > 1 ? s.workspace : 0;
-    if (s.pieces == 1) s.least = q.table_pages + 1;
+    if (s.pieces == 1) s.least = q.table_pages + 1;  // what is not cut is one piece, as large as any; no launch reads it
     return s;
 }
 inline Kv4Shape kv4_shape(const Kv4Sequences &q, int heads, int kv_heads, int dim, int window, bool bf16) {
