@@ -358,8 +358,8 @@ int sm_f8_gate_up(sm_ctx *ctx, uint64_t X, uint64_t x_scales, int tokens, int co
  * output's rows lie one after another, each with all its heads, or its heads
  * do, each with all its rows. Outputs are buffers that the call does not read,
  * and each another one.
- * count is at most 2^15; count * table_pages, tokens * heads and pages at most
- * 2^24.
+ * heads is at most 1024, count 2^15; count * table_pages, pages and tokens *
+ * heads (of a call's queries and keys together) are at most 2^24.
  * Nothing is allocated and nothing waits: every entry may be captured. */
 #define SM_KV4_PAGE 64
 
@@ -395,20 +395,20 @@ int sm_kv4_read(sm_ctx *ctx, uint64_t pool, int pages, int kv_heads, int dim, in
  * v_t, over the positions t <= p that are there, t > p - window where window
  * is not 0; times sigmoid(G) where G is not 0. heads is a multiple of
  * kv_heads; key-value head h serves the heads from h * heads / kv_heads on.
- * scale is finite and > 0. Rows that have no position, or only scores of
+ * scale is > 0 and below 1e30. Rows that have no position, or only scores of
  * -infinity, are 0. What positions outside a row's range hold does not count,
  * whatever it is. Sums and the softmax are in f32. Scores, before and after the
  * scale, have to lie below 2^126 in magnitude, f32 queries below 2^127; weights
  * are up to 2^8 until their sum divides them, so values times the number of
  * positions below 2^119. For f32 tensors nothing is rounded to fewer bits. For
- * bf16 ones the probabilities are rounded to bf16 (2^-8 each), and in calls of many rows
- * (from 1024 of a key-value head) the queries are taken as two 8-bit numbers
- * each, off by 2^-22 of the row's largest at most, whose products with the
- * codes may lose 7 * 2^-13 of their magnitudes in a score (1e-5 of it, usually).
- * A query that is not finite spoils its own row and no other. Y [tokens x heads
- * x dim] is without gaps. The same inputs give the same bits. The workspace
- * holds sm_kv4_attention_workspace(...) bytes (0 where that is 0); a call leaves
- * nothing in it that a later call needs. */
+ * bf16 ones the probabilities are rounded to bf16 (2^-8 each), and in calls of
+ * many rows (from 1024 of a key-value head) the queries are taken as two 8-bit
+ * numbers each, off by 2^-22 of the row's largest at most, whose products with
+ * the codes may lose 7 * 2^-13 of their magnitudes in a score (1e-5 of it,
+ * usually). A query that is not finite spoils its own row and no other. Y
+ * [tokens x heads x dim] is without gaps. The same inputs give the same bits.
+ * The workspace holds sm_kv4_attention_workspace(...) bytes (0 where that is
+ * 0); a call leaves nothing in it that a later call needs. */
 int sm_kv4_attention_workspace(int tokens, int count, int longest, int table_pages, int heads, int kv_heads, int dim,
                                uint64_t *bytes);
 int sm_kv4_attention(sm_ctx *ctx, uint64_t Q, const int64_t *q_view, int type, int tokens, int count, int longest,
