@@ -417,7 +417,11 @@ class Backend:
     # offset) in values, None: rows of heads of dim values without gaps.
     @staticmethod
     def _view(view):
-        return None if view is None else (ctypes.c_int64 * 3)(*view)
+        if view is None:
+            return None
+        if len(view) != 3:  # two would pass with an offset of 0
+            raise ArgumentError(-2, "a view is (stride, head, offset)")
+        return (ctypes.c_int64 * 3)(*view)
 
     def qk_norm_rope(self, Q, K, tokens, heads, kv_heads, dim, q_gamma, k_gamma, eps, Cos, Sin, rotary, context, positions,
                      Yq, Yk, q_view=None, k_view=None, type="f32"):
