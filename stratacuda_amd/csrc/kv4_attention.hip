@@ -582,15 +582,16 @@ __global__ void __launch_bounds__(256, (Rows16<NC, sizeof(T) == 4>::kWavesOfSimd
 // of a score's products' magnitudes are lost, 1e-5 for ordinary ones, where
 // probabilities are rounded by 2^-8. Queries of f32 take bf16's unit.
 //
-// Bound by the matrix units and by what their clock allows: 8192 tokens, 32
-// heads on 8 of dimension 128, bf16, 490 to 520 us, 1.06 to 1.12 PFLOP/s; 512
-// tokens behind 32256 positions, 24 heads on 2 of 256, 349 to 376 us, 1.09 to
-// 1.17 (a library's product of 16384^3 reaches 1.35).
+// From some thousand tokens on bound by the matrix units and by what their clock allows: 8192 tokens, 32 heads on 8 of
+// dimension 128, bf16, 481 to 521 us, 1.06 to 1.14 PFLOP/s (520 to 585 where calls follow without a pause); 512 tokens
+// behind 32256 positions, 24 heads on 2 of 256, 348 to 376 us, 1.09 to 1.18 (a library's product of 16384^3 reaches 1.35).
+// Fewer are not: each workgroup takes 14 us to begin and end, and those of a prompt's first rows end long before the last.
 template <int NC, typename T>
 struct Prompt {
     static constexpr bool kF32 = sizeof(T) == 4;
     static constexpr int kPitch = 64 * NC, kBlocks = 2 * NC, kParts = kF32 ? 3 : 1;
-    // f32 queries of more than 128 dimensions would take more registers than two waves of a SIMD have: sixteen rows then
+    // f32 queries of more than 128 dimensions would take, in this shape, more registers than two waves of a SIMD have: sixteen
+    // rows a workgroup then
     static constexpr bool kThere = !kF32 || NC < 3;
     static constexpr int kWaves = 8, kThreads = 64 * kWaves, kRows = 32 * kWaves;
     static_assert(kRows == kKv4PromptRows, "the shapes count on it");
