@@ -22,17 +22,20 @@ def limit(size, y, length, exponent, type):
     return off + (2.0 ** -8 * (size + np.abs(y)) if type == "bf16" else 0) + 1e-30
 
 
-def expect(b, q, got, scale, type, window=0, gate=None, fill=9.0, left=()):
-    """Every row of batch b against 64 bits; the rows of the sequences `left`, and those of none, as they were."""
+def expect(b, q, got, scale, type, window=0, gate=None, fill=9.0, left=(), most=1 << 30):
+    """Every row of batch b against 64 bits, of sequences of more than `most` rows that many, the first and last ones among them,
+    the others for being numbers; the rows of the sequences `left`, and those of none, as they were."""
     for s, (n, length) in enumerate(b.sequences):
         a = b.starts[s]
         if s in left:
             assert np.all(got[a:a + n] == fill), s
             continue
         k, v = b.held(s)
-        y, size = plain.attention(q[a:a + n].astype(np.float64), length - n + np.arange(n), k, v, scale, window,
-                                  None if gate is None else gate[a:a + n].astype(np.float64))
+        assert np.isfinite(got[a:a + n]).all(), s
+        at = np.unique(np.linspace(0, n - 1, min(n, most)).astype(int)) if n else np.arange(0)
+        y, size = plain.attention(q[a + at].astype(np.float64), length - n + at, k, v, scale, window,
+                                  None if gate is None else gate[a + at].astype(np.float64))
         exponent = scale * LOG2E * np.abs(q).max() * (np.abs(k).sum(-1).max() if k.size else 0)
-        bad = outside(got[a:a + n], y, limit(size, y, length, exponent, type))
-        assert not bad.any(), (s, int(bad.sum()), np.argwhere(bad)[:4], got[a:a + n][bad][:4], y[bad][:4])
+        bad = outside(got[a + at], y, limit(size, y, length, exponent, type))
+        assert not bad.any(), (s, int(bad.sum()), np.argwhere(bad)[:4], got[a + at][bad][:4], y[bad][:4])
     assert np.all(got[b.rows:] == fill)
