@@ -34,7 +34,7 @@ constexpr int64_t kKv4PromptTurns = 53 << 10, kKv4PromptTurnsF32 = 140 << 10, kK
 // which as many of the longest one's would make, are cut by rows: equal pieces of all tiles' pages. In tables of so many
 // pages, and where their tiles leave CUs idle; 256 rows a workgroup from the larger number on where the rule for equal
 // sequences makes three pieces or more. Pieces of at least kKv4FarLeast pages. In us, by that rule and by rows, 24 heads on 2
-// of dimension 256, bf16: 512 tokens and one over 32768 positions each 1376 and 393 (two of 16384: 703 and 220, of 8192: 370
+// of dimension 256, bf16: 512 tokens and one over 32768 positions each 1376 and 393 (over 16384 703 and 220, over 8192 370
 // and 134), 64 tokens and four single ones over 131072 positions 1221 and 77, 96 tokens and 8 over 9000 91 and 28, 8, 5, 3
 // and 1 tokens over 32768 and fewer 71 and 54 (f32 64 and 54). Where the tiles are fewer by less: 2 tokens and 7 single ones
 // over 1000 positions in a table for 8200 20.7 and 30.8. Least 8, 16 and 32: 96 tokens and 8 27, 28 and 33; 16 tokens and
